@@ -1,0 +1,279 @@
+// agz_fp8.hip — matrices in 8 bits (e4m3 with one power-of-two scale per block of 128) and their product on the matrix units
+// (include/agz.h agz_fp8_quantize / agz_fp8_matmul): the layers of the network, forward and backward (DenseNet.jl:161-198, 294-304).
+#include "agz_ops.hpp"
+
+namespace agz {
+namespace ops {
+
+constexpr int FB = 128;                        // a block: 128 along the contracted axis
+
+__device__ __forceinline__ float finite_abs(float x) { x = fabsf(x); return x < INFINITY ? x : 0.0f; }
+// two values times inv (a power of two), rounded to e4m3; NaN and infinities: NaN
+__device__ __forceinline__ uint32_t enc2(float a, float b, float inv) {
+    a = fabsf(a) < INFINITY ? a * inv : NAN;
+    b = fabsf(b) < INFINITY ? b * inv : NAN;
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xFFFFu;
+}
+
+struct QuantPar {
+    const void *x, *gate;
+    int64_t rows, cols, ld;
+    uint8_t *q, *s, *qt, *st;
+    int64_t pitch, spitch, tpitch, tspitch;     // of q, s and of qt, st
+    float* part;                                // column sums of a tile of rows: [row tiles][cols]
+};
+
+// One workgroup per tile of 128 x 128; wave w holds rows 32 w .. 32 w + 31, lane l the columns 2 l, 2 l + 1, all in registers: a row's 128
+// columns are one wave, 32 rows of a column one lane.
+template <typename T, int BR, bool ROW, bool COL>
+__global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
+    __shared__ float red[4][FB];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t r0 = (int64_t)blockIdx.y * FB + w * 32, c0 = (int64_t)blockIdx.x * FB, c = c0 + lane * 2;
+    float v[32][2];
+#pragma unroll
+    for (int k = 0; k < 32; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const bool in = r0 + k < p.rows && c + e < p.cols;
+            const int64_t at = (r0 + k) * p.ld + c + e;
+            v[k][e] = in ? to_f(((const T*)p.x)[at]) : 0.0f;
+            if (in && p.gate && !(to_f(((const T*)p.gate)[at]) > 0.0f)) v[k][e] = 0.0f;
+        }
+    int tile_byte = 0;
+    if (BR == FB) {
+        float m = 0.0f;
+        for (int k = 0; k < 32; ++k) m = fmaxf(m, fmaxf(finite_abs(v[k][0]), finite_abs(v[k][1])));
+        m = wave_max(m);
+        if (lane == 0) red[w][0] = m;
+        __syncthreads();
+        tile_byte = scale_byte(fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])));
+    }
+    if (ROW) {
+        for (int k = 0; k < 32; ++k) {
+            if (r0 + k >= p.rows) break;
+            const int b = BR == FB ? tile_byte : scale_byte(wave_max(fmaxf(finite_abs(v[k][0]), finite_abs(v[k][1]))));
+            *(uint16_t*)(p.q + (r0 + k) * p.pitch + c) = (uint16_t)enc2(v[k][0], v[k][1], inv_scale_of(b));
+            if (lane == 0) p.s[(r0 + k) * p.spitch + blockIdx.x] = (uint8_t)b;
+            if (blockIdx.x == gridDim.x - 1 && lane > 0 && blockIdx.x + lane < p.spitch) p.s[(r0 + k) * p.spitch + blockIdx.x + lane] = 127;
+        }
+    }
+    if (COL) {
+        int b[2] = {tile_byte, tile_byte};
+        if (BR == 1) {
+            for (int e = 0; e < 2; ++e) {
+                float m = 0.0f;
+                for (int k = 0; k < 32; ++k) m = fmaxf(m, finite_abs(v[k][e]));
+                red[w][lane * 2 + e] = m;
+            }
+            __syncthreads();
+            for (int e = 0; e < 2; ++e) {
+                const int l = lane * 2 + e;
+                b[e] = scale_byte(fmaxf(fmaxf(red[0][l], red[1][l]), fmaxf(red[2][l], red[3][l])));
+            }
+        }
+        for (int e = 0; e < 2; ++e) {
+            if (c + e >= p.cols) continue;
+            const float inv = inv_scale_of(b[e]);
+            uint32_t o[8];
+            for (int k = 0; k < 8; ++k) o[k] = enc2(v[4 * k][e], v[4 * k + 1][e], inv) | enc2(v[4 * k + 2][e], v[4 * k + 3][e], inv) << 16;
+            uint4* to = (uint4*)(p.qt + (c + e) * p.tpitch + r0);
+            to[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            if (w == 0) {
+                p.st[(c + e) * p.tspitch + blockIdx.y] = (uint8_t)b[e];
+                if (blockIdx.y == gridDim.y - 1) for (int k = 1; blockIdx.y + k < p.tspitch; ++k) p.st[(c + e) * p.tspitch + blockIdx.y + k] = 127;
+            }
+        }
+        if (p.part) {
+            __syncthreads();
+            for (int e = 0; e < 2; ++e) {
+                float sum = 0.0f;
+                for (int k = 0; k < 32; ++k) sum += v[k][e];
+                red[w][lane * 2 + e] = sum;
+            }
+            __syncthreads();
+            if (threadIdx.x < FB && c0 + threadIdx.x < p.cols)
+                p.part[(int64_t)blockIdx.y * p.cols + c0 + threadIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void k_colsum(const float* part, int64_t tiles, int64_t cols, float* out) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float s = 0.0f;
+    for (int64_t i = 0; i < tiles; ++i) s += part[i * cols + c];
+    out[c] = s;
+}
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+struct MatPar {
+    const uint8_t *qa, *sa, *qb, *sb;
+    int64_t m, n, k, pitch, spitch;
+    const void* bias; int bias_dtype, relu;
+    void* out; int out_dtype; int64_t ldo;
+};
+
+__device__ __forceinline__ float load_as(const void* p, int dtype, int64_t i) {
+    return dtype == AGZ_F32 ? ((const float*)p)[i] : dtype == AGZ_BF16 ? to_f(((const bf16*)p)[i]) : to_f(((const f16*)p)[i]);
+}
+__device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float x) {
+    if (dtype == AGZ_F32) ((float*)p)[i] = x;
+    else if (dtype == AGZ_BF16) ((bf16*)p)[i] = from_f<bf16>(x);
+    else ((f16*)p)[i] = from_f<f16>(x);
+}
+__device__ __forceinline__ i32x8 load32(const uint8_t* p) {
+    const i32x4 a = *(const i32x4*)p, b = *(const i32x4*)(p + 16);
+    return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds 32 of the 128 k of row l % 16 of A and of B — the same 32 for both, so which does not matter —
+// and one scale byte for them (byte SEL of a word); all four lanes of a row have the block's.  Result: column l % 16, rows 4 (l / 16) + i.
+template <int SEL> __device__ __forceinline__ f32x4 mma(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, SEL, sa, SEL, sb);
+}
+
+// The matrix unit adds the products of 8 values in groups of eight, cut off at 2^-13 of the group's largest (measured: beside a product of 2^16 one of 2^3
+// in the same eight counts, one of 2^2 does not; between groups it keeps 24 bits): 3e-5 of the result's norm on normally distributed values, a
+// seventieth of the rounding of a 16-bit result.  Two kinds of results need more: those in 32 bits, and those behind a relu, whose signs decide which
+// gradients pass (measured on 32768 x 512 x 512: with the products of 8 bits some signs next to 0 change and dw is 2.4e-3 off, with these it is not).
+// Their values become bf16 on the way (exact, the scale applied: 4 bits of mantissa, 8 of exponent) for v_mfma_f32_16x16x32_bf16, at half the rate.
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+struct Wide { bf16x8_t v[4]; };
+__device__ __forceinline__ Wide widen(i32x8 q, int byte) {
+    Wide o;
+    const float s = __uint_as_float((uint32_t)byte << 23);       // (the conversion takes the exponent's bits: 2^(byte - 127), also for byte 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)q[2 * i + h], s, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)q[2 * i + h], s, true);
+            o.v[i][4 * h] = lo[0]; o.v[i][4 * h + 1] = lo[1]; o.v[i][4 * h + 2] = hi[0]; o.v[i][4 * h + 3] = hi[1];
+        }
+    return o;
+}
+__device__ __forceinline__ f32x4 mma_wide(const Wide& a, const Wide& b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+}
+
+// the simple form: a wave per 64 x 64 of the result, operands straight from memory, a workgroup of 2 x 2 waves
+template <bool WIDE> __global__ __launch_bounds__(256) void k_matmul_fp8(MatPar p) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int64_t m0 = (int64_t)blockIdx.x * 128 + (w >> 1) * 64, n0 = (int64_t)blockIdx.y * 128 + (w & 1) * 64;
+    if (m0 >= p.m || n0 >= p.n) return;
+    const uint8_t *a[4], *b[4];
+    const int *sa[4], *sb[4];
+    for (int i = 0; i < 4; ++i) {
+        int64_t r = m0 + i * 16 + l16; r = r < p.m ? r : p.m - 1;
+        int64_t c = n0 + i * 16 + l16; c = c < p.n ? c : p.n - 1;
+        a[i] = p.qa + r * p.pitch + g * 32; sa[i] = (const int*)(p.sa + r * p.spitch);
+        b[i] = p.qb + c * p.pitch + g * 32; sb[i] = (const int*)(p.sb + c * p.spitch);
+    }
+    f32x4 acc[4][4] = {};
+    const int kb = (int)((p.k + FB - 1) / FB);
+    for (int k = 0; k < kb; ++k) {
+        i32x8 av[4], bv[4];
+        int as[4], bs[4];
+        for (int i = 0; i < 4; ++i) {
+            av[i] = load32(a[i] + (int64_t)k * FB); bv[i] = load32(b[i] + (int64_t)k * FB);
+            as[i] = sa[i][k >> 2] >> 8 * (k & 3); bs[i] = sb[i][k >> 2] >> 8 * (k & 3);
+        }
+        if constexpr (WIDE) {
+            Wide bw[4];
+            for (int j = 0; j < 4; ++j) bw[j] = widen(bv[j], bs[j] & 0xFF);
+            for (int i = 0; i < 4; ++i) { const Wide aw = widen(av[i], as[i] & 0xFF); for (int j = 0; j < 4; ++j) acc[i][j] = mma_wide(aw, bw[j], acc[i][j]); }
+        } else {
+            for (int i = 0; i < 4; ++i) for (int j = 0; j < 4; ++j) acc[i][j] = mma<0>(av[i], bv[j], acc[i][j], as[i], bs[j]);
+        }
+    }
+    for (int i = 0; i < 4; ++i) for (int j = 0; j < 4; ++j) {
+        const int64_t c = n0 + j * 16 + l16;
+        if (c >= p.n) continue;
+        const float bias = p.bias ? load_as(p.bias, p.bias_dtype, c) : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+            const int64_t r = m0 + i * 16 + g * 4 + e;
+            if (r >= p.m) continue;
+            float y = acc[i][j][e] + bias;
+            if (p.relu) y = y < 0.0f ? 0.0f : y;             // (NaN stays NaN)
+            store_as(p.out, p.out_dtype, r * p.ldo + c, y);
+        }
+    }
+}
+
+}  // namespace ops
+}  // namespace agz
+
+using namespace agz::ops;
+
+static bool too_large(int64_t a) { return a > (1ll << 31) - 256; }
+
+extern "C" {
+
+int64_t agz_fp8_pitch(int64_t cols) { return cols < 0 ? -1 : up(cols, FB); }
+int64_t agz_fp8_scale_pitch(int64_t cols) { return cols < 0 ? -1 : up(cdiv(cols, FB), 4); }
+int64_t agz_fp8_colsum_ws(int64_t rows, int64_t cols) { return rows < 0 || cols < 0 ? -1 : cdiv(rows, FB) * cols * 4; }
+
+int agz_fp8_quantize(int device, void* stream, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* gate, int block_rows,
+                     void* q, void* s, void* qt, void* st, float* colsum, void* ws, int64_t ws_bytes) {
+    if (!good_dtype(dtype)) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: unknown dtype %d", dtype);
+    if (rows < 0 || cols < 0 || too_large(rows) || too_large(cols)) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: %lld x %lld", (long long)rows, (long long)cols);
+    if (ld < 0) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: a negative stride");
+    if (block_rows != 1 && block_rows != FB) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: blocks of %d rows (1 or 128)", block_rows);
+    if (rows > 0 && cols > 0 && (!q != !s || !qt != !st || (!q && !qt))) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: q with s and / or qt with st");
+    if (colsum && rows > 0 && cols > 0 && (!qt || !ws || ws_bytes < agz_fp8_colsum_ws(rows, cols) || !aligned(ws, 16))) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: colsum needs qt and its workspace");
+    OnDevice on(device);
+    if (on.rc != AGZ_OK) return on.rc;
+    if (cols == 0 || (rows == 0 && !colsum)) return AGZ_OK;
+    if (rows > 0) {
+        if (!x || !aligned(x, esize(dtype)) || !aligned(gate, esize(dtype)) || !aligned(q, 16) || !aligned(s, 4) || !aligned(qt, 16) || !aligned(st, 4))
+            return fail(AGZ_ERR_ARG, "agz_fp8_quantize: x missing, or a pointer that is not aligned (q, qt: to 16 bytes, scales: to 4)");
+        QuantPar p{x, gate, rows, cols, ld, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st, up(cols, FB), up(cdiv(cols, FB), 4), up(rows, FB), up(cdiv(rows, FB), 4), colsum ? (float*)ws : nullptr};
+        const dim3 grid((uint32_t)cdiv(cols, FB), (uint32_t)cdiv(rows, FB));
+        if (grid.y > 65535u) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: more than 65535 x 128 rows");
+        const int rc = by_dtype(dtype, [&](auto T) {
+            using X = decltype(T);
+            if (block_rows == 1) {
+                if (q && qt) return launch(k_quantize<X, 1, true, true>, grid, dim3(256), 0, stream, p);
+                if (q) return launch(k_quantize<X, 1, true, false>, grid, dim3(256), 0, stream, p);
+                return launch(k_quantize<X, 1, false, true>, grid, dim3(256), 0, stream, p);
+            }
+            if (q && qt) return launch(k_quantize<X, FB, true, true>, grid, dim3(256), 0, stream, p);
+            if (q) return launch(k_quantize<X, FB, true, false>, grid, dim3(256), 0, stream, p);
+            return launch(k_quantize<X, FB, false, true>, grid, dim3(256), 0, stream, p);
+        });
+        if (rc != AGZ_OK) return rc;
+    }
+    if (colsum) return launch(k_colsum, dim3((uint32_t)cdiv(cols, 256)), dim3(256), 0, stream, (const float*)ws, cdiv(rows, FB), cols, colsum);
+    return AGZ_OK;
+}
+
+int64_t agz_fp8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
+    if (m < 0 || n < 0 || k < 0 || too_large(m) || too_large(n) || too_large(k)) return -1;
+    return 0;
+}
+
+int agz_fp8_matmul(int device, void* stream, int64_t m, int64_t n, int64_t k, const void* qa, const void* sa, const void* qb, const void* sb,
+                   const void* bias, int bias_dtype, int relu, void* out, int out_dtype, int64_t ldo, void* ws, int64_t ws_bytes) {
+    const int64_t need = agz_fp8_matmul_workspace(m, n, k);
+    if (need < 0) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
+    if (!good_dtype(out_dtype) || (bias && !good_dtype(bias_dtype))) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: unknown dtype");
+    if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 16))) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: a workspace of %lld bytes, 16-byte aligned", (long long)need);
+    OnDevice on(device);
+    if (on.rc != AGZ_OK) return on.rc;
+    if (m == 0 || n == 0) return AGZ_OK;
+    if (!out || ldo < n || !aligned(out, esize(out_dtype)) || (bias && !aligned(bias, esize(bias_dtype)))) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: out with a row stride of at least %lld, aligned to its type", (long long)n);
+    if (k > 0 && (!qa || !sa || !qb || !sb || !aligned(qa, 16) || !aligned(qb, 16) || !aligned(sa, 4) || !aligned(sb, 4)))
+        return fail(AGZ_ERR_ARG, "agz_fp8_matmul: values aligned to 16 bytes and scales to 4");
+    MatPar p{(const uint8_t*)qa, (const uint8_t*)sa, (const uint8_t*)qb, (const uint8_t*)sb, m, n, k, up(k, FB), up(cdiv(k, FB), 4), bias, bias_dtype, relu, out, out_dtype, ldo};
+    if (cdiv(n, 128) > 65535) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: more than 65535 x 128 columns");
+    return launch(out_dtype == AGZ_F32 || relu ? k_matmul_fp8<true> : k_matmul_fp8<false>, dim3((uint32_t)cdiv(m, 128), (uint32_t)cdiv(n, 128)), dim3(256), 0, stream, p);
+}
+
+}  // extern "C"

@@ -37,6 +37,19 @@ class SelfplayStats(C.Structure):
                 ("search_seconds", C.c_double), ("total_seconds", C.c_double)]
 
 
+class LogProbArgs(C.Structure):                     # agz_logprob_args
+    _fields_ = [("n", C.c_int64), ("a", C.c_int64), ("logits", C.c_void_p), ("ld", C.c_int64), ("dtype", C.c_int32), ("top", C.c_int32),
+                ("mask", C.c_void_p), ("ld_mask", C.c_int64), ("moves", C.c_void_p), ("target", C.c_void_p), ("ld_target", C.c_int64),
+                ("move_logp", C.c_void_p), ("entropy", C.c_void_p), ("target_logp", C.c_void_p), ("top_logp", C.c_void_p),
+                ("top_move", C.c_void_p), ("stats", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class AdamWOptions(C.Structure):                    # agz_adamw_options
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("seed", C.c_uint32), ("tensor_base", C.c_int32),
+                ("step", C.c_int64), ("step_dev", C.c_void_p)]
+
+
 def build_library():
     """Compile libagz.so for gfx950 (hipcc cross-compiles without a GPU)."""
     subprocess.check_call(["make", "-s", "-C", CSRC])
@@ -111,5 +124,21 @@ def load_library():
         L.agz_comm_post_status.argtypes = [vp, C.c_int]
         L.agz_comm_get_statuses.argtypes = [vp, C.POINTER(C.c_int32)]
         L.agz_allgather_samples_status.argtypes = [vp, vp, C.c_int, i64p, C.POINTER(C.c_int32)]
+    if hasattr(L, "agz_ops_last_error") or not os.environ.get("AGZ_LIB_PATH"):
+        i64, i32 = C.c_int64, C.c_int
+        L.agz_ops_last_error.argtypes = []
+        L.agz_ops_last_error.restype = C.c_char_p
+        L.agz_logprob_workspace.argtypes = [i64, i64, C.c_int32]
+        L.agz_logprob_forward.argtypes = [i32, vp, C.POINTER(LogProbArgs)]
+        L.agz_logprob_backward.argtypes = [i32, vp, C.POINTER(LogProbArgs), vp, vp, vp, vp, vp, i64]
+        L.agz_fp8_pitch.argtypes = L.agz_fp8_scale_pitch.argtypes = [i64]
+        L.agz_fp8_colsum_ws.argtypes = [i64, i64]
+        L.agz_fp8_quantize.argtypes = [i32, vp, vp, i32, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp, vp, i64]
+        L.agz_fp8_matmul_workspace.argtypes = [i64, i64, i64]
+        L.agz_fp8_matmul.argtypes = [i32, vp, i64, i64, i64, vp, vp, vp, vp, vp, i32, i32, vp, i32, i64, vp, i64]
+        L.agz_adamw_state_elements.argtypes = [i32, vp]
+        L.agz_adamw_step.argtypes = [i32, vp, C.POINTER(AdamWOptions), i32, vp, vp, vp, vp, vp, vp, vp]
+        for n in ("logprob_workspace", "fp8_pitch", "fp8_scale_pitch", "fp8_colsum_ws", "fp8_matmul_workspace", "adamw_state_elements"):
+            getattr(L, "agz_" + n).restype = i64
     _LIB = L
     return L

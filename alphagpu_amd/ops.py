@@ -1,0 +1,423 @@
+"""Operators on device tensors: what a network learns with (include/agz.h "operators on tensors in DEVICE memory").
+
+    log_probs(logits, moves, ...)            log probabilities of given moves, entropy, best alternatives, expected log probability; differentiable
+    quantize_fp8, matmul_fp8, linear_fp8     matrices in 8 bits with a scale for each block of 128, and their products; differentiable
+    AdamW                                    one step over many tensors, states in 32 or 8 bits
+
+The reference does this in Flux (train.jl:12-15, :50; DenseNet.jl:161-198).  Tensors are torch tensors on a GPU; the work runs on the current
+stream of their device, nothing waits for it, and it can be captured into a graph.  Wrong arguments raise ValueError before anything is
+queued, errors of the library AgzError.  There is no CPU path.
+"""
+import ctypes as C
+from collections import namedtuple
+
+import torch
+
+from . import lib as _lib
+
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+TOP_MAX = 32
+FP8, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _lib_call(rc, L):
+    if rc != 0:
+        raise _lib.AgzError(rc, L.agz_ops_last_error().decode())
+
+
+def _need(ok, text):
+    if not ok:
+        raise ValueError(text)
+
+
+def _on_gpu(t, name, device=None):
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise ValueError(f"{name}: a tensor on a GPU is needed (there is no CPU path)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the others on {device}")
+
+
+def _float_type(t, name):
+    if t.dtype not in _CODE:
+        raise ValueError(f"{name}: float32, bfloat16 or float16, not {t.dtype}")
+
+
+def _rows(t, name):
+    """[rows][cols] with the columns next to each other; the row stride."""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: two dimensions are needed, not {t.dim()}")
+    if t.shape[1] > 1 and t.stride(1) != 1 and t.numel():
+        raise ValueError(f"{name}: the columns of a row have to lie next to each other (stride {t.stride(1)}): use contiguous()")
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# log probabilities
+# ---------------------------------------------------------------------------------------------------------------------------------------
+LogProbs = namedtuple("LogProbs", "move entropy target top top_move")
+
+
+def _log_probs_args(logits, moves, mask, target, top):
+    dev = logits.device
+    n, a = logits.shape
+    q = _lib.LogProbArgs(n=n, a=a, logits=logits.data_ptr(), ld=_rows(logits, "logits"), dtype=_CODE[logits.dtype], top=top)
+    if mask is not None:
+        q.mask, q.ld_mask = mask.data_ptr(), (mask.stride(0) if mask.shape[0] > 1 else 0)
+    if moves is not None:
+        q.moves = moves.data_ptr()
+    if target is not None:
+        q.target, q.ld_target = target.data_ptr(), _rows(target, "target")
+    return q, dev, n, a
+
+
+def _log_probs_forward(logits, moves, mask, target, top):
+    L = _lib.load_library()
+    q, dev, n, a = _log_probs_args(logits, moves, mask, target, top)
+    # the outputs share one allocation: [stats 4][move][entropy][target][top_logp top][top_move top] x n
+    width = 6 + (target is not None) + 2 * top
+    need = L.agz_logprob_workspace(n, a, top)
+    flat = torch.empty(width * n, dtype=torch.float32, device=dev)
+    at = 4 * n
+    stats, parts = flat[:at], []
+    for want, w in ((moves is not None, 1), (True, 1), (target is not None, 1), (top > 0, top), (top > 0, top)):
+        parts.append(flat[at:at + w * n].view(*((n,) if w == 1 and len(parts) < 3 else (n, w))) if want else None)
+        at += w * n if want else 0
+    move, entropy, tl, tops, top_move = parts
+    if top:
+        top_move = top_move.view(torch.int32)
+    q.stats, q.move_logp, q.entropy, q.target_logp, q.top_logp, q.top_move = map(_ptr, (stats, move, entropy, tl, tops, top_move))
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        q.workspace, q.workspace_bytes = ws.data_ptr(), need
+    _lib_call(L.agz_logprob_forward(dev.index, _stream(dev), C.byref(q)), L)
+    return stats, move, entropy, tl, tops, top_move
+
+
+class _LogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, moves, mask, target, top):
+        stats, *out = _log_probs_forward(logits, moves, mask, target, top)
+        ctx.set_materialize_grads(False)
+        ctx.top = top
+        ctx.save_for_backward(logits, moves, mask, target, out[4], stats)
+        if out[4] is not None:
+            ctx.mark_non_differentiable(out[4])
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_move, g_entropy, g_target, g_top, _):
+        logits, moves, mask, target, top_move, stats = ctx.saved_tensors
+        if g_move is None and g_entropy is None and g_target is None and g_top is None:
+            return None, None, None, None, None
+        L = _lib.load_library()
+        q, dev, n, a = _log_probs_args(logits, moves, mask, target, ctx.top)
+        q.stats, q.top_move = stats.data_ptr(), _ptr(top_move)
+        g = [None if x is None else x.contiguous() for x in (g_move, g_entropy, g_target, g_top)]
+        dx = torch.empty((n, a), dtype=logits.dtype, device=dev)
+        _lib_call(L.agz_logprob_backward(dev.index, _stream(dev), C.byref(q), *map(_ptr, g), dx.data_ptr(), max(a, 1)), L)
+        return dx, None, None, None, None
+
+
+def log_probs(logits, moves=None, mask=None, target=None, top=0):
+    """Log probabilities of moves under rows of logits [n, a] (float32, bfloat16 or float16) -> LogProbs of float32 tensors:
+
+        move      [n]       of the given `moves` (whole numbers [n]; 0 where the move is < 0 or >= a: none given; -inf where it is not allowed)
+        entropy   [n]       of the distribution
+        target    [n]       sum_j target_j logp_j: minus the cross entropy against `target` [n, a] (float32; a constant for the gradient)
+        top       [n, top]  of the `top` (at most 32) most probable moves, most probable first, equal logits by index
+        top_move  [n, top]  those moves (int32; -1, with -inf, where fewer are allowed)
+
+    None for what was not asked for.  `mask` (bool or uint8; [n, a], or [1, a] / [a] for all rows): the moves that are allowed; a logit of -inf
+    is not allowed either.  A row without an allowed move has entropy 0 and gradient 0; a row with NaN or +inf among the allowed is NaN.
+    Differentiable in the logits through move, entropy, target and top."""
+    _on_gpu(logits, "logits")
+    _float_type(logits, "logits")
+    _rows(logits, "logits")
+    n, a = logits.shape
+    dev = logits.device
+    _need(a >= 1, "logits: no actions")
+    _need(isinstance(top, int) and 0 <= top <= min(TOP_MAX, a), f"top: 0 to {TOP_MAX} and at most the number of actions, not {top!r}")
+    if moves is not None:
+        _on_gpu(moves, "moves", dev)
+        _need(moves.shape == (n,) and moves.dtype in (torch.int64, torch.int32), f"moves: int64 or int32 [{n}], not {moves.dtype} {list(moves.shape)}")
+        if moves.dtype != torch.int64 or not moves.is_contiguous():
+            moves = moves.long().contiguous()
+    if mask is not None:
+        _on_gpu(mask, "mask", dev)
+        _need(mask.dtype in (torch.bool, torch.uint8), f"mask: bool or uint8, not {mask.dtype}")
+        if mask.dim() == 1:
+            mask = mask[None]
+        _need(mask.dim() == 2 and mask.shape[0] in (1, n) and mask.shape[1] == a, f"mask: [{n}, {a}], [1, {a}] or [{a}], not {list(mask.shape)}")
+        _rows(mask, "mask")
+    if target is not None:
+        _on_gpu(target, "target", dev)
+        _need(target.dtype == torch.float32 and target.shape == (n, a), f"target: float32 [{n}, {a}], not {target.dtype} {list(target.shape)}")
+        _need(not target.requires_grad, "target: a constant is needed (detach() it)")
+        _rows(target, "target")
+    if logits.requires_grad and torch.is_grad_enabled():
+        return LogProbs(*_LogProbs.apply(logits, moves, mask, target, top))
+    return LogProbs(*_log_probs_forward(logits, moves, mask, target, top)[1:])
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# products in 8 bits
+# ---------------------------------------------------------------------------------------------------------------------------------------
+class Fp8Matrix:
+    """A matrix [rows, cols] in 8 bits: q [rows, cols rounded up to 128] (float8_e4m3fn; zeros behind cols) and scale [rows, blocks of 128
+    columns rounded up to 4] (float8_e8m0fnu).  Entry (i, j) is q[i, j] * scale[i, j // 128]."""
+    __slots__ = ("q", "scale", "rows", "cols")
+
+    def __init__(self, rows, cols, device):
+        self.rows, self.cols = rows, cols
+        self.q = torch.empty((rows, -(-cols // 128) * 128), dtype=FP8, device=device)
+        self.scale = torch.empty((rows, -(-cols // 512) * 4), dtype=E8M0, device=device)
+
+    def dequantize(self):
+        """The values it stands for, in float32."""
+        s = self.scale.float()[:, :self.q.shape[1] // 128]
+        return (self.q.float().view(self.rows, -1, 128) * s[:, :, None]).view(self.rows, -1)[:, :self.cols]
+
+    @classmethod
+    def of(cls, q, scale, rows, cols):
+        m = cls.__new__(cls)
+        m.q, m.scale, m.rows, m.cols = q, scale, rows, cols
+        return m
+
+
+def _quantize(x, block_rows, straight, transposed, gate=None, colsum=False):
+    """(x in 8 bits or None, its transpose in 8 bits or None, column sums or None) of x [rows, cols]."""
+    L = _lib.load_library()
+    dev = x.device
+    ld = _rows(x, "x")
+    r, c = x.shape
+    a = Fp8Matrix(r, c, dev) if straight else None
+    t = Fp8Matrix(c, r, dev) if transposed else None
+    sums = ws = None
+    need = 0
+    if colsum:
+        sums = torch.empty(c, dtype=torch.float32, device=dev)
+        need = L.agz_fp8_colsum_ws(r, c)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    _lib_call(L.agz_fp8_quantize(dev.index, _stream(dev), x.data_ptr(), _CODE[x.dtype], r, c, ld, _ptr(gate), block_rows,
+                                 a and a.q.data_ptr() or None, a and a.scale.data_ptr() or None, t and t.q.data_ptr() or None, t and t.scale.data_ptr() or None,
+                                 _ptr(sums), _ptr(ws), need), L)
+    return a, t, sums
+
+
+def quantize_fp8(x, block_rows=1, transposed=False):
+    """x [rows, cols] (float32, bfloat16 or float16) -> Fp8Matrix, of x or (transposed) of its transpose, with one scale per block of
+    block_rows (1, or 128 for weights) x 128 along the columns of the result.  Scales are the smallest powers of two with |x| <= 448 scale; NaN
+    and infinities become NaN."""
+    _on_gpu(x, "x")
+    _float_type(x, "x")
+    _need(block_rows in (1, 128), f"block_rows: 1 or 128, not {block_rows!r}")
+    with torch.no_grad():
+        a, t, _ = _quantize(x.detach(), block_rows, not transposed, bool(transposed))
+    return t if transposed else a
+
+
+def _product(a, b, bias, relu, dtype):
+    L = _lib.load_library()
+    dev = a.q.device
+    out = torch.empty((a.rows, b.rows), dtype=dtype, device=dev)
+    need = L.agz_fp8_matmul_workspace(a.rows, b.rows, a.cols)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib_call(L.agz_fp8_matmul(dev.index, _stream(dev), a.rows, b.rows, a.cols, a.q.data_ptr(), a.scale.data_ptr(), b.q.data_ptr(), b.scale.data_ptr(),
+                               _ptr(bias), 0 if bias is None else _CODE[bias.dtype], int(relu), out.data_ptr(), _CODE[dtype], max(b.rows, 1), _ptr(ws), need), L)
+    return out
+
+
+def _check_bias(bias, n, dev):
+    if bias is not None:
+        _on_gpu(bias, "bias", dev)
+        _float_type(bias, "bias")
+        _need(bias.shape == (n,) and (n < 2 or bias.stride(0) == 1), f"bias: [{n}], contiguous, not {list(bias.shape)}")
+
+
+def matmul_fp8(a, b, bias=None, relu=False, dtype=torch.bfloat16):
+    """relu?(a b^T + bias) of two Fp8Matrix with the same number of columns: [a.rows, b.rows] in `dtype`; sums in 32 bits, rounded once."""
+    _need(isinstance(a, Fp8Matrix) and isinstance(b, Fp8Matrix), "a and b: Fp8Matrix (quantize_fp8) are needed")
+    _need(a.cols == b.cols, f"a has {a.cols} columns, b {b.cols}")
+    _need(a.q.device == b.q.device, "a and b are on different devices")
+    _need(dtype in _CODE, f"dtype: float32, bfloat16 or float16, not {dtype}")
+    _check_bias(bias, b.rows, a.q.device)
+    with torch.no_grad():
+        return _product(a, b, None if bias is None else bias.detach(), relu, dtype)
+
+
+class Fp8Weight:
+    """Weights [out, in] laid out once for linear_fp8 calls that need no gradient of them."""
+    __slots__ = ("matrix",)
+
+    def __init__(self, w):
+        self.matrix = quantize_fp8(w, block_rows=128)
+
+
+class _LinearFp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, relu):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        a, at, _ = _quantize(x, 1, True, need_w)
+        b, bt, _ = _quantize(w, 128, True, need_x)
+        y = _product(a, b, bias, relu, x.dtype)
+        ctx.relu, ctx.types, ctx.shape = relu, (x.dtype, w.dtype, None if bias is None else bias.dtype), (x.shape[0], w.shape[0], w.shape[1])
+        ctx.save_for_backward(*(at and (at.q, at.scale) or (None, None)), *(bt and (bt.q, bt.scale) or (None, None)), y if relu else None)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        atq, ats, btq, bts, y = ctx.saved_tensors
+        m, n, k = ctx.shape
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dy = dy.contiguous()
+        d, dt, sums = _quantize(dy, 1, need_x, need_w or need_b, gate=y, colsum=need_b)
+        dx = _product(d, Fp8Matrix.of(btq, bts, k, n), None, False, ctx.types[0]) if need_x else None
+        dw = _product(dt, Fp8Matrix.of(atq, ats, k, m), None, False, ctx.types[1]) if need_w else None
+        db = sums.to(ctx.types[2]) if need_b else None
+        return dx, dw, db, None
+
+
+def linear_fp8(x, w, bias=None, relu=False):
+    """relu?(x w^T + bias) with x [..., in] and w [out, in] held in 8 bits for the product: x in blocks of 1 x 128, w in blocks of 128 x 128.
+    The result has the type of x.  w: a tensor (float32, bfloat16 or float16; quantised in the call), or Fp8Weight.  Differentiable in x, w and bias:
+    dx = dy w and dw = dy^T x are products in 8 bits too (dy in blocks of 1 x 128 along what is summed over), dbias sums in 32 bits."""
+    _on_gpu(x, "x")
+    _float_type(x, "x")
+    dev = x.device
+    _need(x.dim() >= 1, "x: at least one dimension is needed")
+    ready = isinstance(w, Fp8Weight)
+    if ready:
+        n, k = w.matrix.rows, w.matrix.cols
+        _need(w.matrix.q.device == dev, f"w is on {w.matrix.q.device}, x on {dev}")
+    else:
+        _on_gpu(w, "w", dev)
+        _float_type(w, "w")
+        _rows(w, "w")
+        n, k = w.shape
+    _need(x.shape[-1] == k, f"x has {x.shape[-1]} columns, w {k}")
+    _check_bias(bias, n, dev)
+    two = x if x.dim() == 2 else x.reshape(-1, k)
+    _rows(two, "x")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not ready and w.requires_grad)):
+        _need(not ready, "w: gradients need the weights themselves, not Fp8Weight")
+        y = _LinearFp8.apply(two, w, bias, bool(relu))
+    else:
+        a, _, _ = _quantize(two, 1, True, False)
+        b = w.matrix if ready else _quantize(w, 128, True, False)[0]
+        y = _product(a, b, bias, relu, x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# AdamW
+# ---------------------------------------------------------------------------------------------------------------------------------------
+class AdamW:
+    """AdamW (decoupled weight decay) over many tensors in one launch, in place:
+
+        m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    params: contiguous tensors of one type on one device that do not overlap.  bits = 32: states m, v in float32.  bits = 8: m and r = sqrt(v) in
+    float8_e4m3fn with one power-of-two scale per 128 elements, rounded up or down at random in proportion (from `seed`, the step and the
+    element: equal calls give equal results).  The states of all tensors lie in the buffers m, v (or m, m_scale, r, r_scale), tensor i from element offsets[i] on.
+    capturable: the number of the step is kept on the device, so that a step captured into a graph counts on in its replays."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, seed=0, capturable=False):
+        self.params = list(params)
+        _need(self.params, "params: none")
+        _need(bits in (8, 32), f"bits: 8 or 32, not {bits!r}")
+        _need(lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas), "lr, eps, weight_decay >= 0 and betas in [0, 1) are needed")
+        dev, kind, ends = self.params[0].device if isinstance(self.params[0], torch.Tensor) else None, None, []
+        for i, p in enumerate(self.params):
+            _on_gpu(p, f"params[{i}]", dev)
+            _float_type(p, f"params[{i}]")
+            kind = kind or p.dtype
+            _need(p.dtype == kind, f"params[{i}] is {p.dtype}, the first {kind}: one AdamW for each type")
+            _need(p.is_contiguous(), f"params[{i}] is not contiguous")
+            if p.numel():
+                ends.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), i))
+        ends.sort()
+        for (_, end, i), (start, _, j) in zip(ends, ends[1:]):
+            _need(end <= start, f"params[{i}] and params[{j}] overlap")
+        self.device, self.lr, self.betas, self.eps, self.weight_decay, self.bits, self.seed = dev, lr, tuple(betas), eps, weight_decay, bits, int(seed)
+        count = len(self.params)
+        self._numel = (C.c_int64 * count)(*[p.numel() for p in self.params])
+        self.offsets, at = [], 0
+        for p in self.params:
+            self.offsets.append(at)
+            at += -(-p.numel() // 128) * 128
+        if bits == 32:
+            self.m, self.v = (torch.zeros(at, dtype=torch.float32, device=dev) for _ in range(2))
+        else:
+            self.m, self.r = (torch.zeros(at, dtype=torch.uint8, device=dev).view(FP8) for _ in range(2))
+            self.m_scale, self.r_scale = (torch.full((at // 128,), 127, dtype=torch.uint8, device=dev).view(E8M0) for _ in range(2))
+        self.steps = 0
+        self.step_dev = torch.zeros((), dtype=torch.int64, device=dev) if capturable else None
+
+    def _buffers(self):
+        return ("m", "v") if self.bits == 32 else ("m", "m_scale", "r", "r_scale")
+
+    def state(self):
+        """{"step": steps taken, and the buffers of the states}: copies, for load_state."""
+        return {"step": self.steps if self.step_dev is None else int(self.step_dev.item()), **{k: getattr(self, k).clone() for k in self._buffers()}}
+
+    def load_state(self, state):
+        for k in self._buffers():
+            mine = getattr(self, k)
+            _need(k in state and state[k].shape == mine.shape and state[k].dtype == mine.dtype, f"load_state: {k} has to be {mine.dtype} {list(mine.shape)}")
+        for k in self._buffers():
+            getattr(self, k).view(torch.uint8).copy_(state[k].view(torch.uint8))
+        self.steps = int(state["step"])
+        if self.step_dev is not None:
+            self.step_dev.fill_(self.steps)
+
+    def zero_grad(self):
+        for p in self.params:
+            p.grad = None
+
+    def step(self, grads=None):
+        """One step with `grads` (one per tensor, of one type; None: p.grad).  A tensor whose gradient is None is left as it is."""
+        L = _lib.load_library()
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        count = len(self.params)
+        _need(len(grads) == count, f"{len(grads)} gradients for {count} tensors")
+        kind, gp, pp = None, (C.c_void_p * count)(), (C.c_void_p * count)()
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            _need(p.numel() == self._numel[i] and p.is_contiguous(), f"params[{i}] has changed its shape")
+            pp[i] = p.data_ptr()
+            if g is None:
+                continue
+            if g.device != self.device:
+                raise ValueError(f"grads[{i}] is on {g.device}, the tensors on {self.device}")
+            kind = kind or g.dtype
+            if g.dtype != kind or kind not in _CODE:
+                raise ValueError(f"grads[{i}] is {g.dtype}: one of float32, bfloat16, float16 for all")
+            if g.shape != p.shape:
+                raise ValueError(f"grads[{i}] is {list(g.shape)}, the tensor {list(p.shape)}")
+            if not g.is_contiguous():
+                g = grads[i] = g.contiguous()
+            gp[i] = g.data_ptr()
+        if self.step_dev is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW.step in a graph: capturable=True is needed (a replay has to count its step on the device)")
+        else:
+            self.step_dev.add_(1)
+        t = self.steps + 1
+        o = _lib.AdamWOptions(lr=self.lr, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, weight_decay=self.weight_decay, param_dtype=_CODE[self.params[0].dtype],
+                              grad_dtype=_CODE[kind or torch.float32], bits=self.bits, seed=self.seed & 0xFFFFFFFF, step=t, step_dev=_ptr(self.step_dev))
+        second, ms, rs = (self.v, None, None) if self.bits == 32 else (self.r, self.m_scale, self.r_scale)
+        _lib_call(L.agz_adamw_step(self.device.index, _stream(self.device), C.byref(o), count, pp, gp, self._numel, self.m.data_ptr(), second.data_ptr(), _ptr(ms), _ptr(rs)), L)
+        torch.autograd.graph.increment_version(self.params)
+        self.steps = t
+
+
+__all__ = ["log_probs", "LogProbs", "quantize_fp8", "matmul_fp8", "linear_fp8", "Fp8Matrix", "Fp8Weight", "AdamW", "TOP_MAX"]

@@ -251,6 +251,95 @@ int  agz_get_search_form(agz_engine *h, char *tree_kernel, char *nn_kernel, int 
 int  agz_set_profiling(agz_engine *h, int mode);       /* HIP events per launch: bit 0 tree kernel, bit 1 network kernel;
                                                           bit 2: instrument (events and agz_get_counters) every 4th search only */
 
+/* ---- operators on tensors in DEVICE memory: what a network learns with -----------------------------------------------------------------
+ * log probabilities of moves and their gradient, products in 8 bits and AdamW (alphagpu_amd.ops is their Python form, alphagpu_amd.learn
+ * calls them).  The reference learns in Flux (train.jl:12-15 the losses, :50 ADAM + WeightDecay, DenseNet.jl:161-198 the network).
+ * All of them: `device` is the HIP ordinal that owns the pointers, the work is queued on `stream` (a hipStream_t of that device, NULL: its
+ * default stream) and the call returns; the calling thread's current device is left as it was.  Nothing is allocated, copied to the host or
+ * kept between calls, so the calls can be captured into a graph; a workspace may be used again by later work on the same stream and is shared
+ * with nothing else (two graphs that may run at the same time need two).  Calls on different streams or threads are independent.
+ * Arguments are checked before anything is queued: AGZ_ERR_ARG and a text in agz_ops_last_error() (of this thread).  The results depend on
+ * the arguments alone (no atomics, no order of arrival). */
+enum agz_dtype { AGZ_F32 = 0, AGZ_BF16 = 1, AGZ_F16 = 2 };
+const char *agz_ops_last_error(void);
+
+/* Log probabilities of given moves, entropy and best alternatives of n rows of logits over a actions (softmax! of mcts_gpu.jl:417 and the
+ * policy term of train.jl:12-15).  S_i = the allowed entries of row i: mask_ij != 0 (no mask: all) and x_ij > -inf.
+ *   logp_j = x_j - log sum_S e^x;  move_logp = logp of the given move: 0 where move < 0 or >= a (no move given), -inf for a move outside S
+ *   entropy = -sum_S p logp;  target_logp = sum_j t_j logp_j over the t_j != 0
+ *   top_*: the `top` largest entries of S, largest first, equal ones by index; behind the last of them move -1 and logp -inf.
+ * A row with no allowed entry: entropy 0, move_logp -inf (0 without a move), target_logp 0 without targets and -inf with, no alternatives,
+ * gradient 0.  A row with a NaN or +inf in S: NaN everywhere and no alternatives. */
+typedef struct {
+    int64_t n, a;               /* rows, actions (1 <= a < 2^31) */
+    const void *logits;         /* [n][a], dtype, row stride ld (elements; any, also 0) */
+    int64_t ld;
+    int32_t dtype;              /* agz_dtype */
+    int32_t top;                /* alternatives per row: 0 .. AGZ_TOP_MAX */
+    const uint8_t *mask;        /* [n][a] bytes, row stride ld_mask (0: one row for all); NULL: all allowed */
+    int64_t ld_mask;
+    const int64_t *moves;       /* [n]; NULL: none given */
+    const float *target;        /* [n][a], row stride ld_target; NULL: none */
+    int64_t ld_target;
+    float *move_logp;           /* [n]; NULL: not wanted (so for the outputs below) */
+    float *entropy;             /* [n] */
+    float *target_logp;         /* [n] */
+    float *top_logp;            /* [n][top] */
+    int32_t *top_move;          /* [n][top] */
+    float *stats;               /* [n][4]: largest logit, log of the sum above it, entropy, sum of targets: what the backward pass reads; required */
+    void *workspace;            /* agz_logprob_workspace bytes (16-byte aligned); NULL where that is 0 */
+    int64_t workspace_bytes;
+} agz_logprob_args;
+#define AGZ_TOP_MAX 32
+int64_t agz_logprob_workspace(int64_t n, int64_t a, int32_t top);     /* bytes; < 0: bad arguments */
+int  agz_logprob_forward(int device, void *stream, const agz_logprob_args *args);
+/* dlogits_j = sum_k c_k (delta_jk - p_j) - g_entropy p_j (logp_j + entropy) in S, 0 outside it, c the given cotangents at their entries:
+ * g_move [n] at the move, g_target [n] times target, g_top [n][top] at top_move (a NULL cotangent counts as zeros).  Reads logits, mask, moves, target,
+ * top_move and stats of `args`; dlogits [n][a] in the logits' type, row stride ldd >= a, not overlapping the logits. */
+int  agz_logprob_backward(int device, void *stream, const agz_logprob_args *args, const float *g_move, const float *g_entropy,
+                          const float *g_target, const float *g_top, void *dlogits, int64_t ldd);
+
+/* Matrices in 8 bits: e4m3 values [rows][pitch], pitch = cols rounded up to 128 (the columns behind `cols` are 0), and one scale 2^(byte - 127)
+ * (e8m0) per row and 128 columns: bytes [rows][scale_pitch], scale_pitch = (cols / 128 rounded up) rounded up to 4.  The scale of a block is
+ * the smallest power of two (from 2^-127 on) with |x| <= 448 scale for its finite entries (1 for a block of zeros); values are rounded to the nearest, ties to even; NaN and
+ * infinities become NaN.  A power of two: the matrix unit applies such scales itself, and the scaling rounds nothing. */
+int64_t agz_fp8_pitch(int64_t cols);
+int64_t agz_fp8_scale_pitch(int64_t cols);
+/* x [rows][cols] (dtype, row stride ld) -> q, s in blocks of block_rows (1 or 128) x 128, and / or qt, st: the transposed matrix [cols][rows] with its blocks along
+ * the rows of x (block_rows = 1: 128 rows of one column; 128: the same blocks and values as q).  gate [rows][cols] of the same type and stride (NULL: none): entries where
+ * !(gate > 0) count as 0 (the gradient behind a relu whose result is `gate`).  colsum [cols] (NULL: not wanted; needs qt, and
+ * colsum_ws with agz_fp8_colsum_ws(rows, cols) bytes): the sums of the (gated) columns in 32 bits. */
+int64_t agz_fp8_colsum_ws(int64_t rows, int64_t cols);
+int  agz_fp8_quantize(int device, void *stream, const void *x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void *gate, int block_rows,
+                      void *q, void *s, void *qt, void *st, float *colsum, void *colsum_ws, int64_t colsum_ws_bytes);
+/* out [m][n] (out_dtype, row stride ldo) = relu?( A B^T + bias ): A [m][k], B [n][k] in 8 bits as above, bias [n] of type bias_dtype or NULL;
+ * sums in 32 bits, rounded once (a 16-bit result without relu comes from the matrix unit's products of 8 bits, which it adds in groups of eight
+ * cut off at 2^-13 of the group's largest; results in 32 bits and behind a relu keep 24 bits throughout).  Workspace: agz_fp8_matmul_workspace bytes (16-byte aligned). */
+int64_t agz_fp8_matmul_workspace(int64_t m, int64_t n, int64_t k);
+int  agz_fp8_matmul(int device, void *stream, int64_t m, int64_t n, int64_t k, const void *qa, const void *sa, const void *qb, const void *sb,
+                    const void *bias, int bias_dtype, int relu, void *out, int out_dtype, int64_t ldo, void *workspace, int64_t workspace_bytes);
+
+/* One AdamW step over `count` tensors (decoupled decay; train.jl:50 is ADAM with WeightDecay):
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * in 32 bits, p rounded once to its type.  The states of all tensors lie in common buffers: tensor i begins at element 128 x sum over the
+ * tensors before it of ceil(numel / 128) (agz_adamw_state_elements: their length).  bits = 32: m, v are floats.  bits = 8: m and r = sqrt(v) are
+ * held in e4m3 with one power-of-two scale (e8m0 byte, as in agz_fp8_quantize) per 128 elements and rounded up or down at random in
+ * proportion (unbiased: to the nearest, v could no longer shrink, its steps of 1 - b2 are below half a rounding step); r is 0 only where v is.
+ * The random bits are a hash of (seed, t, tensor index + tensor_base, element): equal arguments give equal results.
+ * A tensor whose gradient is NULL is left as it is, its states too.  Tensors must not overlap. */
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay;
+    int32_t param_dtype, grad_dtype;   /* agz_dtype */
+    int32_t bits;                      /* 32 or 8 */
+    uint32_t seed;
+    int32_t tensor_base;
+    int64_t step;                      /* t of this step, from 1 on; ignored where step_dev is given */
+    const int64_t *step_dev;           /* t in device memory, read when the step runs (graph replays); NULL: `step` */
+} agz_adamw_options;
+int64_t agz_adamw_state_elements(int count, const int64_t *numel);
+int  agz_adamw_step(int device, void *stream, const agz_adamw_options *opt, int count, void *const *params, const void *const *grads, const int64_t *numel,
+                    void *m, void *v, void *m_scale, void *v_scale);
+
 /*
  * Environment switches read by agz_create (all optional; results never depend on them, the tests use them to reach every
  * kernel build at small sizes):

@@ -1,0 +1,302 @@
+"""alphagpu_amd.ops.AdamW against a plain implementation in 64 bits, states in 32 and 8 bits, refusals and graphs."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from alphagpu_amd import lib, ops
+
+E32 = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+HYPER = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+
+
+def step64(p, g, m, v, t, lr, betas, eps, weight_decay):
+    """One step in 64 bits -> (p, m, v) and the errors that 32 bits may add."""
+    b1, b2 = betas
+    p, g, m, v = (x.double() for x in (p, g, m, v))
+    m1, v1 = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    den = (v1 / (1 - b2 ** t)).sqrt() + eps
+    up = lr * (m1 / (1 - b1 ** t)) / den
+    p1 = p * (1 - lr * weight_decay) - up
+    tm = E32 * (2 * (b1 * m).abs() + 2 * ((1 - b1) * g).abs() + m1.abs()) + 2.0 ** -140         # constants and products rounded
+    tv = E32 * (2 * b2 * v + 4 * (1 - b2) * g * g + v1) + 2.0 ** -140
+    rel_v = torch.where(v1 > 0, tv / v1.clamp_min(1e-300), 0.0)
+    tp = E32 * (3 * p.abs() + p1.abs()) + up.abs() * (rel_v + 12 * E32) + lr / (1 - b1 ** t) * tm / den
+    return (p1, m1, v1), (tp, tm, tv)
+
+
+def mix(h):
+    h = (h * 0x9E3779B1) & 0xFFFFFFFF
+    h ^= h >> 16
+    h = (h * 0xB504F335) & 0xFFFFFFFF
+    return h ^ (h >> 16)
+
+
+def tensors(shapes, dtype, gdtype, seed):
+    r = torch.Generator().manual_seed(seed)
+    ps = [torch.randn(*s, generator=r).to(dtype) for s in shapes]
+    gs = [(torch.randn(*s, generator=r) * torch.exp(2 * torch.randn(*s, generator=r))).to(gdtype) for s in shapes]
+    return ps, gs
+
+
+SETS = {"one": [(1,)], "odd": [(3,), (127,), (128,), (129,), (1,), (255,), (640, 3), (81, 128)], "empty": [(5,), (0,), (0, 7), (200,), (0,)],
+        "many": [(i % 7 + 1, i % 5 + 1) for i in range(250)], "large": [(1000, 1003), (17,), (2048, 512)]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gdtype", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("which", list(SETS))
+def test_32_bits_against_64(which, dtype, gdtype):
+    ps, gs = tensors(SETS[which], dtype, gdtype, 1)
+    dev = [p.cuda() for p in ps]
+    opt = ops.AdamW(dev, **HYPER)
+    assert opt.offsets == [sum(-(-q.numel() // 128) * 128 for q in ps[:i]) for i in range(len(ps))]
+    for t in (1, 2, 3):
+        before = [p.cpu().clone() for p in dev], opt.m.cpu().clone(), opt.v.cpu().clone()
+        _, gs = tensors(SETS[which], dtype, gdtype, 10 + t)
+        opt.step([g.cuda() for g in gs])
+        for i, (p, g, at) in enumerate(zip(before[0], gs, opt.offsets)):
+            n = p.numel()
+            held = slice(at, at + n)
+            (p1, m1, v1), (tp, tm, tv) = step64(p.reshape(-1), g.reshape(-1), before[1][held], before[2][held], t, **HYPER)
+            got = dev[i].cpu().reshape(-1).double()
+            assert ((got - p1).abs() <= tp * (1 + HALF[dtype]) + HALF[dtype] * p1.abs() + 2.0 ** -25 * (dtype == torch.float16)).all(), (t, i)
+            assert ((opt.m.cpu()[held].double() - m1).abs() <= tm).all() and ((opt.v.cpu()[held].double() - v1).abs() <= tv).all(), (t, i)
+            rest = slice(at + n, at + -(-n // 128) * 128)
+            assert not opt.m[rest].any() and not opt.v[rest].any()
+
+
+def held_as(codes, scale):
+    return (codes.float().view(-1, 128) * scale.float()[:, None]).view(-1).cpu()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("which", list(SETS))
+def test_8_bits_against_64(which, dtype, gdtype):
+    """The step itself as in 32 bits from the states that are held; then m and r = sqrt(v) are one of the two neighbours in 8 bits, the one that the hash says
+    (unless the place between them is within the error of the step of the border), in the smallest scale that holds the block."""
+    ps, gs = tensors(SETS[which], dtype, gdtype, 2)
+    dev = [p.cuda() for p in ps]
+    opt = ops.AdamW(dev, bits=8, seed=77, **HYPER)
+    for t in (1, 2, 3):
+        p0, m0, r0 = [p.cpu().clone() for p in dev], held_as(opt.m, opt.m_scale), held_as(opt.r, opt.r_scale)
+        _, gs = tensors(SETS[which], dtype, gdtype, 20 + t)
+        opt.step([g.cuda() for g in gs])
+        q = {"m": (opt.m.cpu().float(), opt.m_scale.view(torch.uint8).cpu().int() - 127), "r": (opt.r.cpu().float(), opt.r_scale.view(torch.uint8).cpu().int() - 127)}
+        for i, (p, g, at) in enumerate(zip(p0, gs, opt.offsets)):
+            n = p.numel()
+            if n == 0:
+                continue
+            s = slice(at, at + n)
+            (p1, m1, v1), (tp, tm, tv) = step64(p.reshape(-1), g.reshape(-1), m0[s], r0[s].double().square(), t, **HYPER)
+            got = dev[i].cpu().reshape(-1).double()
+            tv = tv + 2 * E32 * v1                                    # (r squared is rounded too)
+            tp = tp + 2 * E32 * p1.abs() + 4 * E32 * (p1 - p.reshape(-1).double()).abs()
+            assert ((got - p1).abs() <= tp * (1 + HALF[dtype]) + HALF[dtype] * p1.abs()).all(), (t, i)
+            key = mix(mix(mix((77 + 0x3C6EF372) & 0xFFFFFFFF) ^ t) + i & 0xFFFFFFFF)
+            h = mix(torch.arange(n) ^ key)
+            full = -(-n // 128) * 128
+            for name, x, tol, u, floor in (("m", m1, tm, h & 0xFFFF, False), ("r", v1.sqrt(), 0.5 * tv / v1.sqrt().clamp_min(1e-30) + 2 * E32 * v1.sqrt(), h >> 16, True)):
+                codes, e = q[name]
+                codes, e = codes[at:at + full], e[at // 128:(at + full) // 128]
+                pad = lambda z: torch.nn.functional.pad(z, (0, full - n)).view(-1, 128)  # noqa: E731
+                X, T = pad(x.abs()), pad(tol)
+                big = X.amax(1)
+                scale = torch.ldexp(torch.ones_like(big), e)
+                slack = T.amax(1) + E32 * big
+                assert (big <= 448 * scale + slack).all() and ((big >= 224 * scale - slack) | (e == -127) | (big <= slack)).all(), (t, i, name)
+                y, c, ty = X / scale[:, None], codes.view(-1, 128).double(), T / scale[:, None]
+                assert (c.abs() <= 448).all() and (torch.sign(c) * torch.sign(pad(x)) >= 0).all()
+                c = c.abs()
+                gap = torch.exp2(torch.floor(torch.log2(y.clamp_min(2.0 ** -6))) - 3)
+                place = y / gap
+                up = torch.floor(place + pad(u.double()) / 65536)
+                want = up * gap
+                if floor:
+                    want = torch.where(y > 0, want.clamp_min(2.0 ** -9), want)
+                near = (place + pad(u.double()) / 65536 - torch.round(place + pad(u.double()) / 65536)).abs() <= ty / gap + 2.0 ** -15
+                assert ((c == want) | (near & ((c - want).abs() <= 2 * gap))).all(), (t, i, name)
+                assert near.double().mean() < 0.05 or n < 500
+            assert not opt.m.view(torch.uint8)[at + n:at + full].any() and not opt.r.view(torch.uint8)[at + n:at + full].any()
+
+
+@pytest.mark.gpu
+def test_8_bits_round_without_a_bias():
+    """v under a constant gradient goes to g^2 also with steps far below half a rounding step (b2 = 0.999: each moves v by 0.1 % of the way, a step of 8 bits is
+    6 to 12 % of r).  2^17 elements with equal gradients: the mean of r has a standard error of at most 2^-3 / sqrt(2^17) = 0.0004 of r per step; rounding to
+    the nearest would leave r where it is.  From r0 = 2 g, 600 steps: v = g^2 (1 + 3 * 0.999^600) in the mean of the exact recurrence; rounding adds the variance of
+    r to the mean of v each step, at most (gap / 2)^2 with gap <= r / 8, carried on: v grows by at most a factor (1 + 1/256) per step, so only the direction
+    and the order are asked for: r falls by at least half of what the exact recurrence says."""
+    n = 1 << 17
+    p = torch.zeros(n, device="cuda")
+    opt = ops.AdamW([p], lr=0.0, betas=(0.9, 0.999), bits=8, weight_decay=0.0)
+    g = torch.full((n,), 0.75, device="cuda")
+    opt.r.view(torch.uint8).copy_(torch.full((n,), 1.5).to(torch.float8_e4m3fn).view(torch.uint8))
+    means = []
+    for _ in range(600):
+        opt.step([g])
+        means.append(None)
+    m, r = held_as(opt.m, opt.m_scale), held_as(opt.r, opt.r_scale)
+    exact = 0.75 * math.sqrt(1 + 3 * 0.999 ** 600)
+    assert r.mean().item() < 1.5 - 0.5 * (1.5 - exact), r.mean()
+    # m under b1 = 0.9 keeps to g: each step's rounding has mean 0 and a size of at most gap = 2^-4 (between 0.5 and 1)
+    assert abs(m.mean().item() - 0.75) < 6 * 2.0 ** -4 / math.sqrt(n * 0.19) + 0.75 * 2.0 ** -16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_zeros_tiny_and_non_finite_gradients(bits):
+    n = 512
+    p = torch.ones(n, device="cuda")
+    opt = ops.AdamW([p], bits=bits, **{**HYPER, "weight_decay": 0.0})
+    g = torch.zeros(n)
+    opt.step([g.cuda()])
+    assert (p == 1).all()
+    g[0], g[1], g[2], g[3] = math.nan, math.inf, 1e-30, 1.0
+    g[200] = 1e-25                                                # a block of which one element is tiny
+    opt.step([g.cuda()])
+    got = p.cpu()
+    assert torch.isnan(got[0]) and not torch.isfinite(got[1]) and (got[4:128] == 1).all() and torch.isfinite(got[2:]).all() and got[3] < 1
+    opt.step([torch.zeros(n, device="cuda")])
+    assert torch.isfinite(p.cpu()[2:]).all()
+    if bits == 8:                                                 # in one block with a much larger one, v is small but not 0: the step stays bounded
+        q = torch.zeros(128, device="cuda")
+        opt = ops.AdamW([q], bits=8, **{**HYPER, "weight_decay": 0.0})
+        g = torch.full((128,), 1e-6)
+        g[0] = 1e3
+        for t in range(1, 21):
+            # a small element is held as 0 or one unit 2^-9 of its block's scale: m <= b1 u_m + (1 - b1) g, and from the second step on r >= sqrt(b2) u_r, the floor
+            # (both from the scales that are held before the step); a step is lr m / (1 - b1^t) / (r / sqrt(1 - b2^t))
+            um, ur = (2.0 ** -9 * s[0].float().item() for s in (opt.m_scale, opt.r_scale))
+            before = q[1:].clone()
+            opt.step([g.cuda()])
+            m, r = (0.9 * um + 1e-7, math.sqrt(0.99) * ur) if t > 1 else (1e-7, 0.1 * 1e-6)
+            most = HYPER["lr"] * m / (1 - 0.9 ** t) / (r / math.sqrt(1 - 0.99 ** t))
+            assert (q[1:] - before).abs().max().item() <= most * 1.001 + 1e-9
+        assert (opt.r.float() > 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_missing_gradients_views_and_p_grad(bits):
+    """A tensor without a gradient stays as it is; gradients that are not contiguous; parameters that are parts of one buffer, not aligned to 16 bytes; p.grad."""
+    flat = torch.randn(1000, device="cuda")
+    shapes = [(0, 300), (301, 501), (501, 1000)]
+    ps = [flat[a:b] for a, b in shapes]
+    gs = [torch.randn(b - a, device="cuda") for a, b in shapes]
+    whole = [p.clone() for p in ps]
+    one, two = ops.AdamW(ps, bits=bits, **HYPER), ops.AdamW(whole, bits=bits, **HYPER)
+    gap = flat[300].clone()
+    one.step([gs[0], None, gs[2]])
+    assert torch.equal(ps[1], whole[1]) and not one.m[384:640].view(torch.uint8).any() and torch.equal(flat[300], gap)
+    two.step([gs[0], None, gs[2]])
+    wide = torch.randn(499, 2, device="cuda")
+    one.step([gs[0], gs[1], wide[:, 1]])
+    two.step([gs[0], gs[1], wide[:, 1].contiguous()])
+    for p, g in zip(whole, gs):
+        p.grad = g
+    two.step()
+    one.step(gs)
+    assert all(torch.equal(p, q) for p, q in zip(ps, whole))
+    assert all(torch.equal(getattr(one, k).view(torch.uint8), getattr(two, k).view(torch.uint8)) for k in one._buffers())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_graph_and_another_stream(bits):
+    """load_state goes on where state() was taken; a captured step counts on in its replays and equals eager steps bit for bit; a stream of its own."""
+    def fresh(capturable):
+        ps, _ = tensors(SETS["odd"], torch.float32, torch.float32, 3)
+        ps = [p.cuda() for p in ps]
+        return ps, ops.AdamW(ps, bits=bits, seed=5, capturable=capturable, **HYPER)
+
+    grads = [[g.cuda() for g in tensors(SETS["odd"], torch.float32, torch.float32, 30 + k)[1]] for k in range(6)]
+    ps, opt = fresh(False)
+    for g in grads:
+        opt.step(g)
+    qs, opt2 = fresh(False)
+    for g in grads[:3]:
+        opt2.step(g)
+    kept, at = opt2.state(), [q.clone() for q in qs]
+    opt3 = ops.AdamW(at, bits=bits, seed=5, **HYPER)
+    opt3.load_state(kept)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for g in grads[3:]:
+            opt3.step(g)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(ps, at))
+    ws, opt4 = fresh(True)
+    held = [g.clone() for g in grads[0]]
+    opt4.step(held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt4.step(held)
+    for k in range(1, 6):
+        for h, g in zip(held, grads[k]):
+            h.copy_(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        [w.sum().item() for w in ws]
+    assert opt4.state()["step"] == 6 and all(torch.equal(p, w) for p, w in zip(ps, ws))
+    with pytest.raises(RuntimeError, match="capturable"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step(grads[0])
+
+
+@pytest.mark.gpu
+def test_a_step_is_seen_by_autograd():
+    p = torch.randn(10, device="cuda", requires_grad=True)
+    y = (p * p).sum()
+    ops.AdamW([p], **HYPER).step([torch.ones(10, device="cuda")])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    p = torch.randn(40, 4, device="cuda")
+    g = torch.randn(40, 4, device="cuda")
+    for bad, match in ((lambda: ops.AdamW([]), "none"), (lambda: ops.AdamW([p], bits=16), "bits"), (lambda: ops.AdamW([p], lr=-1), "lr"), (lambda: ops.AdamW([p], betas=(0.9, 1.0)), "betas"),
+                       (lambda: ops.AdamW([p.double()]), "float32"), (lambda: ops.AdamW([p, p]), "overlap"), (lambda: ops.AdamW([p[:20], p[10:]]), "overlap"),
+                       (lambda: ops.AdamW([p, p.clone().half()]), "one AdamW"), (lambda: ops.AdamW([p.t()]), "contiguous"), (lambda: ops.AdamW([p]).step([g, g]), "gradients"),
+                       (lambda: ops.AdamW([p]).step([g[:3]]), "tensor"), (lambda: ops.AdamW([p]).step([g.double()]), "float32"), (lambda: ops.AdamW([p]).step([g.cpu()]), "cpu"),
+                       (lambda: ops.AdamW([p, p.clone()]).step([g, g.half()]), "for all"), (lambda: ops.AdamW([p]).load_state({"step": 1, "m": torch.zeros(1)}), "load_state")):
+        with pytest.raises(ValueError, match=match):
+            bad()
+
+
+def test_refusals_without_a_gpu():
+    with pytest.raises(ValueError, match="GPU"):
+        ops.AdamW([torch.randn(3)])
+    L = lib.load_library()
+    buf = (C.c_char * 4096)()
+    at = (C.addressof(buf) + 63) // 64 * 64
+    good = dict(lr=0.1, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, param_dtype=0, grad_dtype=0, bits=32, seed=0, tensor_base=0, step=1, step_dev=None)
+
+    def refused(match, count=1, p=at, g=at, n=4, m=at, v=at, ms=None, rs=None, **kw):
+        o = lib.AdamWOptions(**{**good, **kw})
+        rc = L.agz_adamw_step(0, None, C.byref(o), count, (C.c_void_p * 1)(p), (C.c_void_p * 1)(g), (C.c_int64 * 1)(n), m, v, ms, rs)
+        assert rc == -1 and match in L.agz_ops_last_error().decode(), L.agz_ops_last_error()
+
+    refused("null", count=-1)
+    refused("null", m=None)
+    refused("dtype", param_dtype=3)
+    refused("dtype", grad_dtype=-1)
+    refused("bits", bits=16)
+    refused("scales", bits=8)
+    refused("step", step=0)
+    refused("betas", beta1=1.0)
+    refused("betas", beta2=math.nan)
+    refused("lr", lr=-1.0)
+    refused("tensor", n=-1)
+    refused("16 bytes", m=at + 4)
+    refused("is null", p=None)
+    refused("aligned", g=at + 2)
+    assert L.agz_adamw_step(0, None, None, 0, None, None, None, None, None, None, None) == -1
+    assert L.agz_adamw_state_elements(3, (C.c_int64 * 3)(1, 0, 129)) == 384 and L.agz_adamw_state_elements(1, (C.c_int64 * 1)(-1)) == -1
