@@ -116,15 +116,11 @@ struct MatPar {
     int64_t m, n, k, pitch, spitch;
     const void* bias; int bias_dtype, relu;
     void* out; int out_dtype; int64_t ldo;
+    int slices; float* part;                    // slices of the k axis; above one: their results, [slices][m][n]
 };
 
 __device__ __forceinline__ float load_as(const void* p, int dtype, int64_t i) {
     return dtype == AGZ_F32 ? ((const float*)p)[i] : dtype == AGZ_BF16 ? to_f(((const bf16*)p)[i]) : to_f(((const f16*)p)[i]);
-}
-__device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float x) {
-    if (dtype == AGZ_F32) ((float*)p)[i] = x;
-    else if (dtype == AGZ_BF16) ((bf16*)p)[i] = from_f<bf16>(x);
-    else ((f16*)p)[i] = from_f<f16>(x);
 }
 __device__ __forceinline__ i32x8 load32(const uint8_t* p) {
     const i32x4 a = *(const i32x4*)p, b = *(const i32x4*)(p + 16);
@@ -163,47 +159,206 @@ __device__ __forceinline__ f32x4 mma_wide(const Wide& a, const Wide& b, f32x4 c)
     return c;
 }
 
-// the simple form: a wave per 64 x 64 of the result, operands straight from memory, a workgroup of 2 x 2 waves
-template <bool WIDE> __global__ __launch_bounds__(256) void k_matmul_fp8(MatPar p) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
-    const int64_t m0 = (int64_t)blockIdx.x * 128 + (w >> 1) * 64, n0 = (int64_t)blockIdx.y * 128 + (w & 1) * 64;
-    if (m0 >= p.m || n0 >= p.n) return;
-    const uint8_t *a[4], *b[4];
-    const int *sa[4], *sb[4];
-    for (int i = 0; i < 4; ++i) {
-        int64_t r = m0 + i * 16 + l16; r = r < p.m ? r : p.m - 1;
-        int64_t c = n0 + i * 16 + l16; c = c < p.n ? c : p.n - 1;
-        a[i] = p.qa + r * p.pitch + g * 32; sa[i] = (const int*)(p.sa + r * p.spitch);
-        b[i] = p.qb + c * p.pitch + g * 32; sb[i] = (const int*)(p.sb + c * p.spitch);
+// ---------------------------------------------------------------------------------------------------------------------------------------
+// Tiles of BM x BN, the k axis in steps of one block of 128: both operands' rows of a step (128 bytes each) go from memory straight into LDS
+// (global_load_lds, 16 bytes a lane), two steps deep, one barrier per step.  The 16-byte piece c of row r lies at piece c ^ (r & 7), so that the
+// eight lanes that a ds_read_b128 serves at a time, eight rows of one piece, meet all banks once (the permutation is on the memory side: the DMA
+// writes lanes in order).  WM x WN waves, each BM / WM x BN / WN in tiles of 16 x 16; B is the first operand, so that a lane ends with four
+// neighbouring columns of one row.  Rows and columns outside are read from the last one and not stored.  Scales: a word holds a row's bytes of four steps,
+// read one word ahead.
+// ---------------------------------------------------------------------------------------------------------------------------------------
+typedef __attribute__((address_space(1))) const void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
+
+template <typename O> __device__ __forceinline__ void store4(O* to, f32x4 v, int valid) {
+    if (valid >= 4) {
+        Span<O, 4> s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.e[e] = from_f<O>(v[e]);
+        *(Span<O, 4>*)to = s;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e) if (e < valid) to[e] = from_f<O>(v[e]);
     }
-    f32x4 acc[4][4] = {};
+}
+__device__ __forceinline__ void store_row4(const MatPar& p, int64_t r, int64_t c, f32x4 v) {
+    const int valid = (int)(p.n - c < 4 ? p.n - c : 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (p.bias && e < valid) v[e] += load_as(p.bias, p.bias_dtype, c + e);
+        if (p.relu) v[e] = v[e] < 0.0f ? 0.0f : v[e];        // (NaN stays NaN)
+    }
+    const int64_t at = r * p.ldo + c;
+    if (p.out_dtype == AGZ_F32) store4((float*)p.out + at, v, valid);
+    else if (p.out_dtype == AGZ_BF16) store4((bf16*)p.out + at, v, valid);
+    else store4((f16*)p.out + at, v, valid);
+}
+
+template <int BM, int BN, int WM, int WN, bool WIDE>
+__global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
+    constexpr int NT = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][(BM + BN) * FB];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    // workgroups of one XCD (every eighth id) take neighbouring tiles: eight rows of tiles by all columns, so that their L2 holds the operands they share
+    const uint32_t tm = (uint32_t)((p.m + BM - 1) / BM), tn = (uint32_t)((p.n + BN - 1) / BN), tiles = tm * tn;
+    uint32_t id = blockIdx.x % tiles;
+    const uint32_t slice = blockIdx.x / tiles;
+    {
+        const uint32_t per = tiles / 8, rest = tiles % 8, x = id % 8, o = id / 8;
+        id = x * per + (x < rest ? x : rest) + o;
+    }
+    const uint32_t band = id / (8 * tn), rows = tm - band * 8 < 8 ? tm - band * 8 : 8, in = id - band * 8 * tn;
+    const int64_t m0 = (int64_t)(band * 8 + in % rows) * BM, n0 = (int64_t)(in / rows) * BN;
+    const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
     const int kb = (int)((p.k + FB - 1) / FB);
-    for (int k = 0; k < kb; ++k) {
-        i32x8 av[4], bv[4];
-        int as[4], bs[4];
-        for (int i = 0; i < 4; ++i) {
-            av[i] = load32(a[i] + (int64_t)k * FB); bv[i] = load32(b[i] + (int64_t)k * FB);
-            as[i] = sa[i][k >> 2] >> 8 * (k & 3); bs[i] = sb[i][k >> 2] >> 8 * (k & 3);
+    const int k0 = (int)((int64_t)kb * slice / p.slices), k1 = (int)((int64_t)kb * (slice + 1) / p.slices);
+
+    // this thread's pieces of a step: piece tid + i NT of the tile's (BM + BN) * 8, whole waves in A or in B
+    constexpr int PA = BM * 8 / NT, PB = BN * 8 / NT;
+    static_assert(PA * NT == BM * 8 && PB * NT == BN * 8, "whole pieces");
+    const uint8_t* src[PA + PB];
+#pragma unroll
+    for (int i = 0; i < PA + PB; ++i) {
+        const int piece = tid + (i < PA ? i : i - PA) * NT, r = piece >> 3, c = (piece & 7) ^ (r & 7);
+        int64_t row = (i < PA ? m0 : n0) + r;
+        const int64_t last = (i < PA ? p.m : p.n) - 1;
+        row = row < last ? row : last;
+        src[i] = (i < PA ? p.qa : p.qb) + row * p.pitch + c * 16;
+    }
+    const int* sa[FM];
+    const int* sb[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) { int64_t r = m0 + wm + i * 16 + l16; r = r < p.m ? r : p.m - 1; sa[i] = (const int*)(p.sa + r * p.spitch); }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) { int64_t r = n0 + wn + j * 16 + l16; r = r < p.n ? r : p.n - 1; sb[j] = (const int*)(p.sb + r * p.spitch); }
+
+    auto fetch = [&](int k, int buf) {
+#pragma unroll
+        for (int i = 0; i < PA + PB; ++i)
+            __builtin_amdgcn_global_load_lds((gvoid*)(src[i] + (int64_t)k * FB), (lvoid*)(lds[buf] + (i < PA ? i : i - PA) * NT * 16 + (i < PA ? 0 : BM * FB) + w * 1024), 16, 0, 0);
+    };
+    f32x4 acc[FM][FN] = {};
+    uint32_t as[FM], bs[FN];
+    if (k0 < k1) {
+        fetch(k0, 0);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) as[i] = (uint32_t)sa[i][k0 >> 2] >> 8 * (k0 & 3);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) bs[j] = (uint32_t)sb[j][k0 >> 2] >> 8 * (k0 & 3);
+    }
+    const int p0 = (g ^ (l16 & 7)) * 16, p1 = p0 ^ 64;
+    for (int k = k0; k < k1; ++k) {
+        const int buf = (k - k0) & 1;
+        __syncthreads();                                         // step k is in LDS, and everybody is done with the buffer of step k - 1
+        uint32_t an[FM], bn[FN];
+        const bool next = ((k + 1) & 3) == 0 && k + 1 < k1;
+        if (k + 1 < k1) fetch(k + 1, buf ^ 1);
+        if (next) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) an[i] = (uint32_t)sa[i][(k + 1) >> 2];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) bn[j] = (uint32_t)sb[j][(k + 1) >> 2];
         }
+        const uint8_t* la = lds[buf] + (wm + l16) * FB;
+        const uint8_t* lb = lds[buf] + BM * FB + (wn + l16) * FB;
+        auto frag = [&](const uint8_t* base, int i) {
+            const i32x4 x = *(const i32x4*)(base + i * 16 * FB + p0), y = *(const i32x4*)(base + i * 16 * FB + p1);
+            return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        };
         if constexpr (WIDE) {
-            Wide bw[4];
-            for (int j = 0; j < 4; ++j) bw[j] = widen(bv[j], bs[j] & 0xFF);
-            for (int i = 0; i < 4; ++i) { const Wide aw = widen(av[i], as[i] & 0xFF); for (int j = 0; j < 4; ++j) acc[i][j] = mma_wide(aw, bw[j], acc[i][j]); }
+            Wide bw[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) bw[j] = widen(frag(lb, j), bs[j] & 0xFF);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const Wide aw = widen(frag(la, i), as[i] & 0xFF);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma_wide(bw[j], aw, acc[i][j]);
+            }
         } else {
-            for (int i = 0; i < 4; ++i) for (int j = 0; j < 4; ++j) acc[i][j] = mma<0>(av[i], bv[j], acc[i][j], as[i], bs[j]);
+            i32x8 bv[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) bv[j] = frag(lb, j);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const i32x8 av = frag(la, i);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma<0>(bv[j], av, acc[i][j], (int)bs[j], (int)as[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) as[i] = next ? an[i] : as[i] >> 8;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) bs[j] = next ? bn[j] : bs[j] >> 8;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t r = m0 + wm + i * 16 + l16;
+        if (r >= p.m) continue;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int64_t c = n0 + wn + j * 16 + g * 4;
+            if (c >= p.n) continue;
+            if (p.slices > 1) store4(p.part + ((int64_t)slice * p.m + r) * p.n + c, acc[i][j], (int)(p.n - c < 4 ? p.n - c : 4));
+            else store_row4(p, r, c, acc[i][j]);
         }
     }
-    for (int i = 0; i < 4; ++i) for (int j = 0; j < 4; ++j) {
-        const int64_t c = n0 + j * 16 + l16;
-        if (c >= p.n) continue;
-        const float bias = p.bias ? load_as(p.bias, p.bias_dtype, c) : 0.0f;
-        for (int e = 0; e < 4; ++e) {
-            const int64_t r = m0 + i * 16 + g * 4 + e;
-            if (r >= p.m) continue;
-            float y = acc[i][j][e] + bias;
-            if (p.relu) y = y < 0.0f ? 0.0f : y;             // (NaN stays NaN)
-            store_as(p.out, p.out_dtype, r * p.ldo + c, y);
+}
+
+// the slices of the k axis added up, in order
+__global__ __launch_bounds__(256) void k_matmul_join(MatPar p) {
+    const int64_t quads = (p.n + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / quads, c = (i - r * quads) * 4;
+    if (r >= p.m) return;
+    const int valid = (int)(p.n - c < 4 ? p.n - c : 4);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* at = p.part + r * p.n + c;
+    for (int s = 0; s < p.slices; ++s, at += p.m * p.n) {
+        if (valid == 4) {
+            const Span<float, 4> t = *(const Span<float, 4>*)at;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += t.e[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e) if (e < valid) v[e] += at[e];
         }
+    }
+    store_row4(p, r, c, v);
+}
+
+// Few rows (up to 16): the weights are read once, straight into the matrix unit's registers, and that is all the time there is.  A wave takes 16
+// columns and every fourth (FEW_WAVES) group of steps; the waves of a workgroup add up through LDS.
+constexpr int FEW_WAVES = 4, FEW_DEEP = 4;
+template <bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) void k_matmul_fp8_few(MatPar p) {
+    __shared__ f32x4 sum[FEW_WAVES][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    int64_t r = l16 < p.m ? l16 : p.m - 1, c = n0 + l16 < p.n ? n0 + l16 : p.n - 1;
+    const uint8_t *a = p.qa + r * p.pitch + g * 32, *b = p.qb + c * p.pitch + g * 32;
+    const int *sa = (const int*)(p.sa + r * p.spitch), *sb = (const int*)(p.sb + c * p.spitch);
+    const int kb = (int)((p.k + FB - 1) / FB), whole = kb / FEW_DEEP;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto one = [&](i32x8 av, i32x8 bv, int as, int bs) {
+        if constexpr (WIDE) acc = mma_wide(widen(bv, bs & 0xFF), widen(av, as & 0xFF), acc);
+        else acc = mma<0>(bv, av, acc, bs, as);
+    };
+    for (int q = w; q < whole; q += FEW_WAVES) {                 // FEW_DEEP = 4 steps: one word of scales
+        i32x8 av[FEW_DEEP], bv[FEW_DEEP];
+#pragma unroll
+        for (int k = 0; k < FEW_DEEP; ++k) bv[k] = load32(b + (int64_t)(q * FEW_DEEP + k) * FB);
+#pragma unroll
+        for (int k = 0; k < FEW_DEEP; ++k) av[k] = load32(a + (int64_t)(q * FEW_DEEP + k) * FB);
+        const int as = sa[q], bs = sb[q];
+#pragma unroll
+        for (int k = 0; k < FEW_DEEP; ++k) one(av[k], bv[k], as >> 8 * k, bs >> 8 * k);
+    }
+    if (w == (whole & (FEW_WAVES - 1)))
+        for (int k = whole * FEW_DEEP; k < kb; ++k) one(load32(a + (int64_t)k * FB), load32(b + (int64_t)k * FB), sa[k >> 2] >> 8 * (k & 3), sb[k >> 2] >> 8 * (k & 3));
+    sum[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && l16 < p.m && n0 + g * 4 < p.n) {
+#pragma unroll
+        for (int k = 1; k < FEW_WAVES; ++k) acc += sum[k][lane];
+        store_row4(p, l16, n0 + g * 4, acc);
     }
 }
 
@@ -213,6 +368,22 @@ template <bool WIDE> __global__ __launch_bounds__(256) void k_matmul_fp8(MatPar 
 using namespace agz::ops;
 
 static bool too_large(int64_t a) { return a > (1ll << 31) - 256; }
+
+// How a product runs: `few` rows, or tiles of 256 or 128 a side and slices of the k axis.  A tile of 256 reads half as much per operation and needs a whole CU; where
+// there are fewer of them than CUs, tiles of 128 (two a CU), and where these leave CUs idle too, the k axis is cut so that there are
+// about two workgroups a CU, of at least four steps each.
+namespace {
+constexpr int CUS = 256;
+struct Plan { bool few; int tile, slices; };
+Plan plan(int64_t m, int64_t n, int64_t k) {
+    if (m <= 16) return {true, 16, 1};
+    const int64_t big = cdiv(m, 256) * cdiv(n, 256), small = cdiv(m, 128) * cdiv(n, 128), steps = cdiv(k, FB);
+    if (big >= CUS) return {false, 256, 1};
+    int64_t slices = small < CUS ? 2 * CUS / small : 1;
+    if (slices > steps / 4) slices = steps / 4;
+    return {false, 128, (int)(slices < 1 ? 1 : slices)};
+}
+}
 
 extern "C" {
 
@@ -256,7 +427,9 @@ int agz_fp8_quantize(int device, void* stream, const void* x, int dtype, int64_t
 
 int64_t agz_fp8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
     if (m < 0 || n < 0 || k < 0 || too_large(m) || too_large(n) || too_large(k)) return -1;
-    return 0;
+    if (m == 0 || n == 0) return 0;
+    const Plan w = plan(m, n, k);
+    return w.slices > 1 ? w.slices * m * n * 4 : 0;
 }
 
 int agz_fp8_matmul(int device, void* stream, int64_t m, int64_t n, int64_t k, const void* qa, const void* sa, const void* qb, const void* sb,
@@ -271,9 +444,18 @@ int agz_fp8_matmul(int device, void* stream, int64_t m, int64_t n, int64_t k, co
     if (!out || ldo < n || !aligned(out, esize(out_dtype)) || (bias && !aligned(bias, esize(bias_dtype)))) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: out with a row stride of at least %lld, aligned to its type", (long long)n);
     if (k > 0 && (!qa || !sa || !qb || !sb || !aligned(qa, 16) || !aligned(qb, 16) || !aligned(sa, 4) || !aligned(sb, 4)))
         return fail(AGZ_ERR_ARG, "agz_fp8_matmul: values aligned to 16 bytes and scales to 4");
-    MatPar p{(const uint8_t*)qa, (const uint8_t*)sa, (const uint8_t*)qb, (const uint8_t*)sb, m, n, k, up(k, FB), up(cdiv(k, FB), 4), bias, bias_dtype, relu, out, out_dtype, ldo};
-    if (cdiv(n, 128) > 65535) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: more than 65535 x 128 columns");
-    return launch(out_dtype == AGZ_F32 || relu ? k_matmul_fp8<true> : k_matmul_fp8<false>, dim3((uint32_t)cdiv(m, 128), (uint32_t)cdiv(n, 128)), dim3(256), 0, stream, p);
+    MatPar p{(const uint8_t*)qa, (const uint8_t*)sa, (const uint8_t*)qb, (const uint8_t*)sb, m, n, k, up(k, FB), up(cdiv(k, FB), 4), bias, bias_dtype, relu, out, out_dtype, ldo, 1, nullptr};
+    const Plan w = plan(m, n, k);
+    const bool wide = out_dtype == AGZ_F32 || relu;
+    if (w.few) return launch(wide ? k_matmul_fp8_few<true> : k_matmul_fp8_few<false>, dim3((uint32_t)cdiv(n, 16)), dim3(FEW_WAVES * 64), 0, stream, p);
+    const int64_t groups = cdiv(m, w.tile) * cdiv(n, w.tile) * w.slices;
+    if (groups > 0x7fffffffll) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: more than 2^31 tiles");
+    p.slices = w.slices;
+    p.part = (float*)ws;
+    const int rc = w.tile == 256 ? launch(wide ? k_matmul_fp8<256, 256, 2, 4, true> : k_matmul_fp8<256, 256, 2, 4, false>, dim3((uint32_t)groups), dim3(512), 0, stream, p)
+                                 : launch(wide ? k_matmul_fp8<128, 128, 2, 2, true> : k_matmul_fp8<128, 128, 2, 2, false>, dim3((uint32_t)groups), dim3(256), 0, stream, p);
+    if (rc != AGZ_OK || w.slices == 1) return rc;
+    return launch(k_matmul_join, dim3((uint32_t)cdiv(m * cdiv(n, 4), 256)), dim3(256), 0, stream, p);
 }
 
 }  // extern "C"

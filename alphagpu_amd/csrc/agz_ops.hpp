@@ -60,8 +60,31 @@ template <> __device__ __forceinline__ float from_f(float x) { return x; }
 template <> __device__ __forceinline__ bf16 from_f(float x) { __bf16 b = (__bf16)x; bf16 r; __builtin_memcpy(&r, &b, 2); return r; }
 template <> __device__ __forceinline__ f16 from_f(float x) { return (f16)x; }
 
-__device__ __forceinline__ float wave_max(float x) { for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o)); return x; }
-__device__ __forceinline__ float wave_sum(float x) { for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o); return x; }
+// reductions over G neighbouring lanes, the result in all of them: DPP inside a row of 16 lanes, register swaps between rows (no LDS)
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false); }
+template <int G, typename F> __device__ __forceinline__ uint32_t lanes_reduce(uint32_t x, F&& f) {
+    if constexpr (G >= 2) x = f(x, dpp<0xB1>(x));            // quad_perm 1 0 3 2
+    if constexpr (G >= 4) x = f(x, dpp<0x4E>(x));            // quad_perm 2 3 0 1
+    if constexpr (G >= 8) x = f(x, dpp<0x141>(x));           // row_half_mirror
+    if constexpr (G >= 16) x = f(x, dpp<0x140>(x));          // row_mirror
+    if constexpr (G >= 32) { const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false); x = f(r[0], r[1]); }
+    if constexpr (G >= 64) { const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false); x = f(r[0], r[1]); }
+    return x;
+}
+template <int G> __device__ __forceinline__ float lanes_max(float x) {
+    return __uint_as_float(lanes_reduce<G>(__float_as_uint(x), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+template <int G> __device__ __forceinline__ float lanes_sum(float x) {
+    return __uint_as_float(lanes_reduce<G>(__float_as_uint(x), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+template <int G> __device__ __forceinline__ uint32_t lanes_min_u(uint32_t x) {
+    return lanes_reduce<G>(x, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+__device__ __forceinline__ float wave_max(float x) { return lanes_max<64>(x); }
+__device__ __forceinline__ float wave_sum(float x) { return lanes_sum<64>(x); }
+
+// N neighbouring elements at any address that suits one element (the memory unit takes such addresses)
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Span { T e[N]; };
 
 // the byte of the smallest power-of-two scale 2^(byte - 127) with amax <= 448 * scale (amax finite, >= 0; 448 = 1.75 * 2^8: the exponent less
 // eight, one more where the mantissa is above 1.75); 127, a scale of one, for a block of zeros.  Subnormal amax: byte 0, 2^-127.
