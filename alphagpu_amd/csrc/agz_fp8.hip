@@ -7,14 +7,6 @@ namespace ops {
 
 constexpr int FB = 128;                        // a block: 128 along the contracted axis
 
-__device__ __forceinline__ float finite_abs(float x) { x = fabsf(x); return x < INFINITY ? x : 0.0f; }
-// two values times inv (a power of two), rounded to e4m3; NaN and infinities: NaN
-__device__ __forceinline__ uint32_t enc2(float a, float b, float inv) {
-    a = fabsf(a) < INFINITY ? a * inv : NAN;
-    b = fabsf(b) < INFINITY ? b * inv : NAN;
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xFFFFu;
-}
-
 struct QuantPar {
     const void *x, *gate;
     int64_t rows, cols, ld;
@@ -23,88 +15,188 @@ struct QuantPar {
     float* part;                                // column sums of a tile of rows: [row tiles][cols]
 };
 
-// One workgroup per tile of 128 x 128; wave w holds rows 32 w .. 32 w + 31, lane l the columns 2 l, 2 l + 1, all in registers: a row's 128
-// columns are one wave, 32 rows of a column one lane.
+// eight values times inv (a power of two: exact), rounded to e4m3 to the nearest; the conversion turns NaN and infinities into NaN
+__device__ __forceinline__ uint2 enc8(const float* v, float inv) {
+    int lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, hi, true);
+    return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+// values of the 4 groups of 16 lanes combined (lane l with l ^ 16 and l ^ 32)
+template <typename F> __device__ __forceinline__ float groups_reduce(float x, F&& f) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// One workgroup per tile of 128 x 128, all of it in registers: wave w, lane l hold rows 32 w + 8 (l / 16) + 0..7 of columns 8 (l % 16) + 0..7, read and
+// written eight at a time both ways (8 x 8 values: the transpose is a matter of which eight are packed).  A row's largest is a reduction over
+// 16 lanes, a column's one over 4 lanes and, through LDS, the 4 waves.  fmaxf passes NaN over; a largest of infinity means that the block has one, and its largest
+// finite entry is looked for again.
 template <typename T, int BR, bool ROW, bool COL>
 __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
-    __shared__ float red[4][FB];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t r0 = (int64_t)blockIdx.y * FB + w * 32, c0 = (int64_t)blockIdx.x * FB, c = c0 + lane * 2;
-    float v[32][2];
+    __shared__ __attribute__((aligned(16))) float red[4][FB];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15;
+    const int64_t r0 = (int64_t)blockIdx.y * FB + w * 32 + (lane >> 4) * 8, c0 = (int64_t)blockIdx.x * FB, c = c0 + l16 * 8;
+    float v[8][8];
+    {
+        const int n = (int)(c >= p.cols ? 0 : (p.cols - c < 8 ? p.cols - c : 8));
+        Span<T, 8> x[8], y[8];
 #pragma unroll
-    for (int k = 0; k < 32; ++k)
+        for (int k = 0; k < 8; ++k)
+            if (r0 + k < p.rows) {
+                const T* at = (const T*)p.x + (r0 + k) * p.ld + c;
+                const T* gt = (const T*)p.gate + (r0 + k) * p.ld + c;
+                if (n == 8) {
+                    x[k] = *(const Span<T, 8>*)at;
+                    if (p.gate) y[k] = *(const Span<T, 8>*)gt;
+                } else
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const bool in = r0 + k < p.rows && c + e < p.cols;
-            const int64_t at = (r0 + k) * p.ld + c + e;
-            v[k][e] = in ? to_f(((const T*)p.x)[at]) : 0.0f;
-            if (in && p.gate && !(to_f(((const T*)p.gate)[at]) > 0.0f)) v[k][e] = 0.0f;
-        }
+                    for (int e = 0; e < 7; ++e) if (e < n) { x[k].e[e] = at[e]; if (p.gate) y[k].e[e] = gt[e]; }
+            }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[k][e] = r0 + k < p.rows && e < n ? to_f(x[k].e[e]) : 0.0f;
+                if (p.gate && r0 + k < p.rows && e < n && !(to_f(y[k].e[e]) > 0.0f)) v[k][e] = 0.0f;
+            }
+    }
+    auto max2 = [](float a, float b) { return fmaxf(a, b); };
+    auto finite = [](float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; };
     int tile_byte = 0;
     if (BR == FB) {
         float m = 0.0f;
-        for (int k = 0; k < 32; ++k) m = fmaxf(m, fmaxf(finite_abs(v[k][0]), finite_abs(v[k][1])));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[k][e]));
+        if (__any(m == INFINITY)) {
+            m = 0.0f;
+            for (int k = 0; k < 8; ++k) for (int e = 0; e < 8; ++e) m = fmaxf(m, finite(v[k][e]));
+        }
         m = wave_max(m);
         if (lane == 0) red[w][0] = m;
         __syncthreads();
         tile_byte = scale_byte(fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])));
     }
     if (ROW) {
-        for (int k = 0; k < 32; ++k) {
-            if (r0 + k >= p.rows) break;
-            const int b = BR == FB ? tile_byte : scale_byte(wave_max(fmaxf(finite_abs(v[k][0]), finite_abs(v[k][1]))));
-            *(uint16_t*)(p.q + (r0 + k) * p.pitch + c) = (uint16_t)enc2(v[k][0], v[k][1], inv_scale_of(b));
-            if (lane == 0) p.s[(r0 + k) * p.spitch + blockIdx.x] = (uint8_t)b;
-            if (blockIdx.x == gridDim.x - 1 && lane > 0 && blockIdx.x + lane < p.spitch) p.s[(r0 + k) * p.spitch + blockIdx.x + lane] = 127;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            int b = tile_byte;
+            if (BR == 1) {
+                float m = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[k][e]));
+                if (__any(m == INFINITY)) {
+                    m = 0.0f;
+                    for (int e = 0; e < 8; ++e) m = fmaxf(m, finite(v[k][e]));
+                }
+                b = scale_byte(lanes_max<16>(m));
+            }
+            if (r0 + k < p.rows) {
+                *(uint2*)(p.q + (r0 + k) * p.pitch + c) = enc8(v[k], inv_scale_of(b));
+                if (l16 == 0) p.s[(r0 + k) * p.spitch + blockIdx.x] = (uint8_t)b;
+                if (blockIdx.x == gridDim.x - 1 && l16 > 0 && blockIdx.x + l16 < p.spitch) p.s[(r0 + k) * p.spitch + blockIdx.x + l16] = 127;
+            }
         }
     }
     if (COL) {
-        int b[2] = {tile_byte, tile_byte};
+        float inv[8];
         if (BR == 1) {
-            for (int e = 0; e < 2; ++e) {
-                float m = 0.0f;
-                for (int k = 0; k < 32; ++k) m = fmaxf(m, finite_abs(v[k][e]));
-                red[w][lane * 2 + e] = m;
+            float m[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m[e] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) m[e] = fmaxf(m[e], fabsf(v[k][e]));
+                if (__any(m[e] == INFINITY)) {
+                    m[e] = 0.0f;
+                    for (int k = 0; k < 8; ++k) m[e] = fmaxf(m[e], finite(v[k][e]));
+                }
+                m[e] = groups_reduce(m[e], max2);
+            }
+            if (lane < 16) {
+                *(float4*)&red[w][l16 * 8] = make_float4(m[0], m[1], m[2], m[3]);
+                *(float4*)&red[w][l16 * 8 + 4] = make_float4(m[4], m[5], m[6], m[7]);
             }
             __syncthreads();
-            for (int e = 0; e < 2; ++e) {
-                const int l = lane * 2 + e;
-                b[e] = scale_byte(fmaxf(fmaxf(red[0][l], red[1][l]), fmaxf(red[2][l], red[3][l])));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4 t = *(const float4*)&red[0][l16 * 8 + 4 * h];
+#pragma unroll
+                for (int o = 1; o < 4; ++o) {
+                    const float4 u = *(const float4*)&red[o][l16 * 8 + 4 * h];
+                    t = make_float4(fmaxf(t.x, u.x), fmaxf(t.y, u.y), fmaxf(t.z, u.z), fmaxf(t.w, u.w));
+                }
+                m[4 * h] = t.x; m[4 * h + 1] = t.y; m[4 * h + 2] = t.z; m[4 * h + 3] = t.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int b = scale_byte(m[e]);
+                inv[e] = inv_scale_of(b);
+                if (threadIdx.x < 16 && c + e < p.cols) {
+                    uint8_t* st = p.st + (c + e) * p.tspitch + blockIdx.y;
+                    st[0] = (uint8_t)b;
+                    if (blockIdx.y == gridDim.y - 1) for (int k = 1; blockIdx.y + k < p.tspitch; ++k) st[k] = 127;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                inv[e] = inv_scale_of(tile_byte);
+                if (threadIdx.x < 16 && c + e < p.cols) {
+                    uint8_t* st = p.st + (c + e) * p.tspitch + blockIdx.y;
+                    st[0] = (uint8_t)tile_byte;
+                    if (blockIdx.y == gridDim.y - 1) for (int k = 1; blockIdx.y + k < p.tspitch; ++k) st[k] = 127;
+                }
             }
         }
-        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
             if (c + e >= p.cols) continue;
-            const float inv = inv_scale_of(b[e]);
-            uint32_t o[8];
-            for (int k = 0; k < 8; ++k) o[k] = enc2(v[4 * k][e], v[4 * k + 1][e], inv) | enc2(v[4 * k + 2][e], v[4 * k + 3][e], inv) << 16;
-            uint4* to = (uint4*)(p.qt + (c + e) * p.tpitch + r0);
-            to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            to[1] = make_uint4(o[4], o[5], o[6], o[7]);
-            if (w == 0) {
-                p.st[(c + e) * p.tspitch + blockIdx.y] = (uint8_t)b[e];
-                if (blockIdx.y == gridDim.y - 1) for (int k = 1; blockIdx.y + k < p.tspitch; ++k) p.st[(c + e) * p.tspitch + blockIdx.y + k] = 127;
-            }
+            const float t[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
+            *(uint2*)(p.qt + (c + e) * p.tpitch + r0) = enc8(t, inv[e]);
         }
         if (p.part) {
-            __syncthreads();
-            for (int e = 0; e < 2; ++e) {
-                float sum = 0.0f;
-                for (int k = 0; k < 32; ++k) sum += v[k][e];
-                red[w][lane * 2 + e] = sum;
+            float sum[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum[e] = ((v[0][e] + v[1][e]) + (v[2][e] + v[3][e])) + ((v[4][e] + v[5][e]) + (v[6][e] + v[7][e]));
+                sum[e] = groups_reduce(sum[e], [](float a, float b) { return a + b; });
             }
             __syncthreads();
-            if (threadIdx.x < FB && c0 + threadIdx.x < p.cols)
-                p.part[(int64_t)blockIdx.y * p.cols + c0 + threadIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+            if (lane < 16) {
+                *(float4*)&red[w][l16 * 8] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                *(float4*)&red[w][l16 * 8 + 4] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+            }
+            __syncthreads();
+            const int t = threadIdx.x;
+            if (t < FB && c0 + t < p.cols) p.part[(int64_t)blockIdx.y * p.cols + c0 + t] = (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
         }
     }
 }
 
-__global__ __launch_bounds__(256) void k_colsum(const float* part, int64_t tiles, int64_t cols, float* out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+// the tiles' column sums added up in a fixed order: 64 columns and 16 shares of the tiles per workgroup
+__global__ __launch_bounds__(1024) void k_colsum(const float* part, int64_t tiles, int64_t cols, float* out) {
+    __shared__ float red[16][64];
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + x;
     float s = 0.0f;
-    for (int64_t i = 0; i < tiles; ++i) s += part[i * cols + c];
-    out[c] = s;
+    if (c < cols) {
+#pragma unroll 8
+        for (int64_t i = y; i < tiles; i += 16) s += part[i * cols + c];
+    }
+    red[y][x] = s;
+    __syncthreads();
+    if (y == 0 && c < cols) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += red[k][x];
+        out[c] = s;
+    }
 }
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
@@ -421,7 +513,7 @@ int agz_fp8_quantize(int device, void* stream, const void* x, int dtype, int64_t
         });
         if (rc != AGZ_OK) return rc;
     }
-    if (colsum) return launch(k_colsum, dim3((uint32_t)cdiv(cols, 256)), dim3(256), 0, stream, (const float*)ws, cdiv(rows, FB), cols, colsum);
+    if (colsum) return launch(k_colsum, dim3((uint32_t)cdiv(cols, 64)), dim3(1024), 0, stream, (const float*)ws, cdiv(rows, FB), cols, colsum);
     return AGZ_OK;
 }
 
