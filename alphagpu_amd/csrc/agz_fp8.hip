@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
 }
 
 // the tiles' column sums added up in a fixed order: 64 columns and 16 shares of the tiles per workgroup
-__global__ __launch_bounds__(1024) void k_colsum(const float* part, int64_t tiles, int64_t cols, float* out) {
+__global__ __launch_bounds__(1024) void k_colsum(const float* part, int64_t tiles, int64_t cols, void* out, int out_dtype) {
     __shared__ float red[16][64];
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
     const int64_t c = (int64_t)blockIdx.x * 64 + x;
@@ -195,7 +195,9 @@ __global__ __launch_bounds__(1024) void k_colsum(const float* part, int64_t tile
     if (y == 0 && c < cols) {
 #pragma unroll
         for (int k = 1; k < 16; ++k) s += red[k][x];
-        out[c] = s;
+        if (out_dtype == AGZ_F32) ((float*)out)[c] = s;
+        else if (out_dtype == AGZ_BF16) ((bf16*)out)[c] = from_f<bf16>(s);
+        else ((f16*)out)[c] = from_f<f16>(s);
     }
 }
 
@@ -477,6 +479,81 @@ Plan plan(int64_t m, int64_t n, int64_t k) {
 }
 }
 
+// the work of the entry points below, on the current device, arguments checked
+namespace {
+struct Mat8 { uint8_t *q, *s; };                 // a matrix in 8 bits
+int quantize(void* stream, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* gate, int block_rows, Mat8 a, Mat8 t, void* colsum, int colsum_dtype, float* part) {
+    if (cols == 0) return AGZ_OK;
+    if (rows > 0) {
+        const QuantPar p{x, gate, rows, cols, ld, a.q, a.s, t.q, t.s, up(cols, FB), up(cdiv(cols, FB), 4), up(rows, FB), up(cdiv(rows, FB), 4), colsum ? part : nullptr};
+        const dim3 grid((uint32_t)cdiv(cols, FB), (uint32_t)cdiv(rows, FB));
+        const int rc = by_dtype(dtype, [&](auto T) {
+            using X = decltype(T);
+            if (block_rows == 1) {
+                if (a.q && t.q) return launch(k_quantize<X, 1, true, true>, grid, dim3(256), 0, stream, p);
+                if (a.q) return launch(k_quantize<X, 1, true, false>, grid, dim3(256), 0, stream, p);
+                return launch(k_quantize<X, 1, false, true>, grid, dim3(256), 0, stream, p);
+            }
+            if (a.q && t.q) return launch(k_quantize<X, FB, true, true>, grid, dim3(256), 0, stream, p);
+            if (a.q) return launch(k_quantize<X, FB, true, false>, grid, dim3(256), 0, stream, p);
+            return launch(k_quantize<X, FB, false, true>, grid, dim3(256), 0, stream, p);
+        });
+        if (rc != AGZ_OK) return rc;
+    }
+    if (!colsum) return AGZ_OK;
+    return launch(k_colsum, dim3((uint32_t)cdiv(cols, 64)), dim3(1024), 0, stream, (const float*)part, cdiv(rows, FB), cols, colsum, colsum_dtype);
+}
+
+int product(void* stream, int64_t m, int64_t n, int64_t k, Mat8 a, Mat8 b, const void* bias, int bias_dtype, int relu, void* out, int out_dtype, int64_t ldo, void* ws) {
+    if (m == 0 || n == 0) return AGZ_OK;
+    const Plan w = plan(m, n, k);
+    const MatPar p{a.q, a.s, b.q, b.s, m, n, k, up(k, FB), up(cdiv(k, FB), 4), bias, bias_dtype, relu, out, out_dtype, ldo, w.slices, (float*)ws};
+    const bool wide = out_dtype == AGZ_F32 || relu;
+    if (w.few) return launch(wide ? k_matmul_fp8_few<true> : k_matmul_fp8_few<false>, dim3((uint32_t)cdiv(n, 16)), dim3(FEW_WAVES * 64), 0, stream, p);
+    const int64_t groups = cdiv(m, w.tile) * cdiv(n, w.tile) * w.slices;
+    if (groups > 0x7fffffffll) return fail(AGZ_ERR_ARG, "a product of more than 2^31 tiles");
+    const int rc = w.tile == 256 ? launch(wide ? k_matmul_fp8<256, 256, 2, 4, true> : k_matmul_fp8<256, 256, 2, 4, false>, dim3((uint32_t)groups), dim3(512), 0, stream, p)
+                                 : launch(wide ? k_matmul_fp8<128, 128, 2, 2, true> : k_matmul_fp8<128, 128, 2, 2, false>, dim3((uint32_t)groups), dim3(256), 0, stream, p);
+    if (rc != AGZ_OK || w.slices == 1) return rc;
+    return launch(k_matmul_join, dim3((uint32_t)cdiv(m * cdiv(n, 4), 256)), dim3(256), 0, stream, p);
+}
+
+// matrices in 8 bits one behind the other in a buffer (every part at a multiple of 256 bytes); without a buffer it only counts
+struct Carve {
+    uint8_t* base; int64_t at = 0;
+    uint8_t* take(int64_t bytes) { uint8_t* p = base ? base + at : nullptr; at += up(bytes, 256); return p; }
+    Mat8 matrix(int64_t rows, int64_t cols) { Mat8 m; m.q = take(rows * up(cols, FB)); m.s = take(rows * up(cdiv(cols, FB), 4)); return m; }
+};
+bool good_sizes(int64_t m, int64_t n, int64_t k) { return m >= 0 && n >= 0 && k >= 0 && !too_large(m) && !too_large(n) && !too_large(k) && cdiv(m, FB) <= 65535 && cdiv(n, FB) <= 65535; }
+struct Forward { Mat8 a, b; void* ws; };
+Forward forward_ws(Carve& c, int64_t m, int64_t n, int64_t k) { return {c.matrix(m, k), c.matrix(n, k), c.take(agz_fp8_matmul_workspace(m, n, k))}; }
+struct Saved { Mat8 at, bt; };
+Saved saved_of(Carve& c, int64_t m, int64_t n, int64_t k, bool need_dx, bool need_dw) {
+    Saved s{};
+    if (need_dw) s.at = c.matrix(k, m);
+    if (need_dx) s.bt = c.matrix(k, n);
+    return s;
+}
+struct Backward { Mat8 d, t; void *ws; float* part; };
+Backward backward_ws(Carve& c, int64_t m, int64_t n, int64_t k, bool need_dx, bool need_dw, bool need_db) {
+    Backward w{};
+    if (need_dx) w.d = c.matrix(m, n);
+    if (need_dw || need_db) w.t = c.matrix(n, m);
+    if (need_db) w.part = (float*)c.take(agz_fp8_colsum_ws(m, n));
+    const int64_t x = need_dx ? agz_fp8_matmul_workspace(m, k, n) : 0, y = need_dw ? agz_fp8_matmul_workspace(n, k, m) : 0;
+    w.ws = c.take(x > y ? x : y);                // (one after the other on the stream)
+    return w;
+}
+int check_linear(const char* who, const agz_linear_fp8_args* q) {
+    if (!q) return fail(AGZ_ERR_ARG, "%s: no arguments", who);
+    if (!good_sizes(q->m, q->n, q->k)) return fail(AGZ_ERR_ARG, "%s: %lld x %lld x %lld", who, (long long)q->m, (long long)q->n, (long long)q->k);
+    if (!good_dtype(q->dtype) || !good_dtype(q->w_dtype) || (q->bias && !good_dtype(q->bias_dtype))) return fail(AGZ_ERR_ARG, "%s: unknown dtype", who);
+    if (q->ldx < 0 || q->ldw < 0) return fail(AGZ_ERR_ARG, "%s: a negative stride", who);
+    if (!aligned(q->x, esize(q->dtype)) || !aligned(q->w, esize(q->w_dtype)) || (q->bias && !aligned(q->bias, esize(q->bias_dtype)))) return fail(AGZ_ERR_ARG, "%s: a pointer is not aligned to its type", who);
+    return AGZ_OK;
+}
+}  // namespace
+
 extern "C" {
 
 int64_t agz_fp8_pitch(int64_t cols) { return cols < 0 ? -1 : up(cols, FB); }
@@ -494,27 +571,10 @@ int agz_fp8_quantize(int device, void* stream, const void* x, int dtype, int64_t
     OnDevice on(device);
     if (on.rc != AGZ_OK) return on.rc;
     if (cols == 0 || (rows == 0 && !colsum)) return AGZ_OK;
-    if (rows > 0) {
-        if (!x || !aligned(x, esize(dtype)) || !aligned(gate, esize(dtype)) || !aligned(q, 16) || !aligned(s, 4) || !aligned(qt, 16) || !aligned(st, 4))
-            return fail(AGZ_ERR_ARG, "agz_fp8_quantize: x missing, or a pointer that is not aligned (q, qt: to 16 bytes, scales: to 4)");
-        QuantPar p{x, gate, rows, cols, ld, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st, up(cols, FB), up(cdiv(cols, FB), 4), up(rows, FB), up(cdiv(rows, FB), 4), colsum ? (float*)ws : nullptr};
-        const dim3 grid((uint32_t)cdiv(cols, FB), (uint32_t)cdiv(rows, FB));
-        if (grid.y > 65535u) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: more than 65535 x 128 rows");
-        const int rc = by_dtype(dtype, [&](auto T) {
-            using X = decltype(T);
-            if (block_rows == 1) {
-                if (q && qt) return launch(k_quantize<X, 1, true, true>, grid, dim3(256), 0, stream, p);
-                if (q) return launch(k_quantize<X, 1, true, false>, grid, dim3(256), 0, stream, p);
-                return launch(k_quantize<X, 1, false, true>, grid, dim3(256), 0, stream, p);
-            }
-            if (q && qt) return launch(k_quantize<X, FB, true, true>, grid, dim3(256), 0, stream, p);
-            if (q) return launch(k_quantize<X, FB, true, false>, grid, dim3(256), 0, stream, p);
-            return launch(k_quantize<X, FB, false, true>, grid, dim3(256), 0, stream, p);
-        });
-        if (rc != AGZ_OK) return rc;
-    }
-    if (colsum) return launch(k_colsum, dim3((uint32_t)cdiv(cols, 64)), dim3(1024), 0, stream, (const float*)ws, cdiv(rows, FB), cols, colsum);
-    return AGZ_OK;
+    if (rows > 0 && (!x || !aligned(x, esize(dtype)) || !aligned(gate, esize(dtype)) || !aligned(q, 16) || !aligned(s, 4) || !aligned(qt, 16) || !aligned(st, 4)))
+        return fail(AGZ_ERR_ARG, "agz_fp8_quantize: x missing, or a pointer that is not aligned (q, qt: to 16 bytes, scales: to 4)");
+    if (cdiv(rows, FB) > 65535) return fail(AGZ_ERR_ARG, "agz_fp8_quantize: more than 65535 x 128 rows");
+    return quantize(stream, x, dtype, rows, cols, ld, gate, block_rows, {(uint8_t*)q, (uint8_t*)s}, {(uint8_t*)qt, (uint8_t*)st}, colsum, AGZ_F32, (float*)ws);
 }
 
 int64_t agz_fp8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
@@ -536,18 +596,61 @@ int agz_fp8_matmul(int device, void* stream, int64_t m, int64_t n, int64_t k, co
     if (!out || ldo < n || !aligned(out, esize(out_dtype)) || (bias && !aligned(bias, esize(bias_dtype)))) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: out with a row stride of at least %lld, aligned to its type", (long long)n);
     if (k > 0 && (!qa || !sa || !qb || !sb || !aligned(qa, 16) || !aligned(qb, 16) || !aligned(sa, 4) || !aligned(sb, 4)))
         return fail(AGZ_ERR_ARG, "agz_fp8_matmul: values aligned to 16 bytes and scales to 4");
-    MatPar p{(const uint8_t*)qa, (const uint8_t*)sa, (const uint8_t*)qb, (const uint8_t*)sb, m, n, k, up(k, FB), up(cdiv(k, FB), 4), bias, bias_dtype, relu, out, out_dtype, ldo, 1, nullptr};
-    const Plan w = plan(m, n, k);
-    const bool wide = out_dtype == AGZ_F32 || relu;
-    if (w.few) return launch(wide ? k_matmul_fp8_few<true> : k_matmul_fp8_few<false>, dim3((uint32_t)cdiv(n, 16)), dim3(FEW_WAVES * 64), 0, stream, p);
-    const int64_t groups = cdiv(m, w.tile) * cdiv(n, w.tile) * w.slices;
-    if (groups > 0x7fffffffll) return fail(AGZ_ERR_ARG, "agz_fp8_matmul: more than 2^31 tiles");
-    p.slices = w.slices;
-    p.part = (float*)ws;
-    const int rc = w.tile == 256 ? launch(wide ? k_matmul_fp8<256, 256, 2, 4, true> : k_matmul_fp8<256, 256, 2, 4, false>, dim3((uint32_t)groups), dim3(512), 0, stream, p)
-                                 : launch(wide ? k_matmul_fp8<128, 128, 2, 2, true> : k_matmul_fp8<128, 128, 2, 2, false>, dim3((uint32_t)groups), dim3(256), 0, stream, p);
-    if (rc != AGZ_OK || w.slices == 1) return rc;
-    return launch(k_matmul_join, dim3((uint32_t)cdiv(m * cdiv(n, 4), 256)), dim3(256), 0, stream, p);
+    return product(stream, m, n, k, {(uint8_t*)qa, (uint8_t*)sa}, {(uint8_t*)qb, (uint8_t*)sb}, bias, bias_dtype, relu, out, out_dtype, ldo, ws);
+}
+
+int64_t agz_linear_fp8_workspace(int64_t m, int64_t n, int64_t k) {
+    if (!good_sizes(m, n, k)) return -1;
+    Carve c{nullptr};
+    forward_ws(c, m, n, k);
+    return c.at;
+}
+int64_t agz_linear_fp8_saved(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw) {
+    if (!good_sizes(m, n, k)) return -1;
+    Carve c{nullptr};
+    saved_of(c, m, n, k, need_dx, need_dw);
+    return c.at;
+}
+int64_t agz_linear_fp8_backward_workspace(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, int need_db) {
+    if (!good_sizes(m, n, k)) return -1;
+    Carve c{nullptr};
+    backward_ws(c, m, n, k, need_dx, need_dw, need_db);
+    return c.at;
+}
+
+int agz_linear_fp8_forward(int device, void* stream, const agz_linear_fp8_args* q, void* y, void* saved, int need_dx, int need_dw, void* ws, int64_t ws_bytes) {
+    if (int rc = check_linear("agz_linear_fp8_forward", q)) return rc;
+    const int64_t need = agz_linear_fp8_workspace(q->m, q->n, q->k);
+    if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 256))) return fail(AGZ_ERR_ARG, "agz_linear_fp8_forward: a workspace of %lld bytes, 256-byte aligned", (long long)need);
+    if ((need_dx || need_dw) && (!aligned(saved, 256) || (!saved && agz_linear_fp8_saved(q->m, q->n, q->k, need_dx, need_dw) > 0))) return fail(AGZ_ERR_ARG, "agz_linear_fp8_forward: saved, 256-byte aligned");
+    if ((q->m > 0 && q->n > 0 && (!y || !aligned(y, esize(q->dtype)))) || (q->m > 0 && q->k > 0 && !q->x) || (q->n > 0 && q->k > 0 && !q->w)) return fail(AGZ_ERR_ARG, "agz_linear_fp8_forward: x, w and y are required");
+    OnDevice on(device);
+    if (on.rc != AGZ_OK) return on.rc;
+    Carve c{(uint8_t*)ws}, d{(uint8_t*)saved};
+    const Forward f = forward_ws(c, q->m, q->n, q->k);
+    const Saved s = saved_of(d, q->m, q->n, q->k, need_dx, need_dw);
+    if (int rc = quantize(stream, q->x, q->dtype, q->m, q->k, q->ldx, nullptr, 1, f.a, s.at, nullptr, 0, nullptr)) return rc;
+    if (int rc = quantize(stream, q->w, q->w_dtype, q->n, q->k, q->ldw, nullptr, FB, f.b, s.bt, nullptr, 0, nullptr)) return rc;
+    return product(stream, q->m, q->n, q->k, f.a, f.b, q->bias, q->bias_dtype, q->relu, y, q->dtype, q->n, f.ws);
+}
+
+int agz_linear_fp8_backward(int device, void* stream, const agz_linear_fp8_args* q, const void* dy, const void* y, const void* saved, int saved_dx, int saved_dw, void* dx, void* dw, void* db, void* ws, int64_t ws_bytes) {
+    if (int rc = check_linear("agz_linear_fp8_backward", q)) return rc;
+    const int64_t m = q->m, n = q->n, k = q->k, need = agz_linear_fp8_backward_workspace(m, n, k, !!dx, !!dw, !!db);
+    if ((dx && !saved_dx) || (dw && !saved_dw)) return fail(AGZ_ERR_ARG, "agz_linear_fp8_backward: the forward call did not save what this needs");
+    if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 256))) return fail(AGZ_ERR_ARG, "agz_linear_fp8_backward: a workspace of %lld bytes, 256-byte aligned", (long long)need);
+    if (!aligned(saved, 256) || (!saved && agz_linear_fp8_saved(m, n, k, saved_dx, saved_dw) > 0)) return fail(AGZ_ERR_ARG, "agz_linear_fp8_backward: saved, 256-byte aligned");
+    if (m > 0 && n > 0 && (!dy || (q->relu && !y) || !aligned(dy, esize(q->dtype)) || !aligned(y, esize(q->dtype)))) return fail(AGZ_ERR_ARG, "agz_linear_fp8_backward: dy, and y behind a relu, are required");
+    if (!aligned(dx, esize(q->dtype)) || !aligned(dw, esize(q->w_dtype)) || (db && (!good_dtype(q->bias_dtype) || !aligned(db, esize(q->bias_dtype))))) return fail(AGZ_ERR_ARG, "agz_linear_fp8_backward: a pointer is not aligned to its type");
+    OnDevice on(device);
+    if (on.rc != AGZ_OK) return on.rc;
+    Carve c{(uint8_t*)ws}, d{(uint8_t*)saved};
+    const Backward b = backward_ws(c, m, n, k, dx, dw, db);
+    const Saved s = saved_of(d, m, n, k, saved_dx, saved_dw);
+    if (dx || dw || db) if (int rc = quantize(stream, dy, q->dtype, m, n, n, q->relu ? y : nullptr, 1, b.d, b.t, db, q->bias_dtype, b.part)) return rc;
+    if (dx) if (int rc = product(stream, m, k, n, b.d, s.bt, nullptr, 0, 0, dx, q->dtype, k, b.ws)) return rc;
+    if (dw) return product(stream, n, k, m, b.t, s.at, nullptr, 0, 0, dw, q->w_dtype, k, b.ws);
+    return AGZ_OK;
 }
 
 }  // extern "C"

@@ -44,6 +44,11 @@ class LogProbArgs(C.Structure):                     # agz_logprob_args
                 ("top_move", C.c_void_p), ("stats", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+class LinearFp8Args(C.Structure):                   # agz_linear_fp8_args
+    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+                ("bias", C.c_void_p), ("dtype", C.c_int32), ("w_dtype", C.c_int32), ("bias_dtype", C.c_int32), ("relu", C.c_int32)]
+
+
 class AdamWOptions(C.Structure):                    # agz_adamw_options
     _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
                 ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("seed", C.c_uint32), ("tensor_base", C.c_int32),
@@ -129,16 +134,21 @@ def load_library():
         L.agz_ops_last_error.argtypes = []
         L.agz_ops_last_error.restype = C.c_char_p
         L.agz_logprob_workspace.argtypes = [i64, i64, C.c_int32]
-        L.agz_logprob_forward.argtypes = [i32, vp, C.POINTER(LogProbArgs)]
-        L.agz_logprob_backward.argtypes = [i32, vp, C.POINTER(LogProbArgs), vp, vp, vp, vp, vp, i64]
+        L.agz_logprob_forward.argtypes = [i32, vp, vp]
+        L.agz_logprob_backward.argtypes = [i32, vp, vp, vp, vp, vp, vp, vp, i64]
         L.agz_fp8_pitch.argtypes = L.agz_fp8_scale_pitch.argtypes = [i64]
         L.agz_fp8_colsum_ws.argtypes = [i64, i64]
         L.agz_fp8_quantize.argtypes = [i32, vp, vp, i32, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp, vp, i64]
         L.agz_fp8_matmul_workspace.argtypes = [i64, i64, i64]
         L.agz_fp8_matmul.argtypes = [i32, vp, i64, i64, i64, vp, vp, vp, vp, vp, i32, i32, vp, i32, i64, vp, i64]
+        L.agz_linear_fp8_workspace.argtypes = [i64] * 3
+        L.agz_linear_fp8_saved.argtypes = [i64] * 3 + [i32] * 2
+        L.agz_linear_fp8_backward_workspace.argtypes = [i64] * 3 + [i32] * 3
+        L.agz_linear_fp8_forward.argtypes = [i32, vp, vp, vp, vp, i32, i32, vp, i64]
+        L.agz_linear_fp8_backward.argtypes = [i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64]
         L.agz_adamw_state_elements.argtypes = [i32, vp]
-        L.agz_adamw_step.argtypes = [i32, vp, C.POINTER(AdamWOptions), i32, vp, vp, vp, vp, vp, vp, vp]
-        for n in ("logprob_workspace", "fp8_pitch", "fp8_scale_pitch", "fp8_colsum_ws", "fp8_matmul_workspace", "adamw_state_elements"):
+        L.agz_adamw_step.argtypes = [i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+        for n in ("logprob_workspace", "fp8_pitch", "fp8_scale_pitch", "fp8_colsum_ws", "fp8_matmul_workspace", "linear_fp8_workspace", "linear_fp8_saved", "linear_fp8_backward_workspace", "adamw_state_elements"):
             getattr(L, "agz_" + n).restype = i64
     _LIB = L
     return L

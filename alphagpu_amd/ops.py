@@ -9,9 +9,11 @@ stream of their device, nothing waits for it, and it can be captured into a grap
 queued, errors of the library AgzError.  There is no CPU path.
 """
 import ctypes as C
+import struct
 from collections import namedtuple
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream     # the current stream's handle without a Stream object around it
 
 from . import lib as _lib
 
@@ -31,7 +33,7 @@ def _need(ok, text):
 
 
 def _on_gpu(t, name, device=None):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: a tensor on a GPU is needed (there is no CPU path)")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the others on {device}")
@@ -51,10 +53,6 @@ def _rows(t, name):
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -65,66 +63,69 @@ def _ptr(t):
 LogProbs = namedtuple("LogProbs", "move entropy target top top_move")
 
 
-def _log_probs_args(logits, moves, mask, target, top):
-    dev = logits.device
-    n, a = logits.shape
-    q = _lib.LogProbArgs(n=n, a=a, logits=logits.data_ptr(), ld=_rows(logits, "logits"), dtype=_CODE[logits.dtype], top=top)
-    if mask is not None:
-        q.mask, q.ld_mask = mask.data_ptr(), (mask.stride(0) if mask.shape[0] > 1 else 0)
-    if moves is not None:
-        q.moves = moves.data_ptr()
-    if target is not None:
-        q.target, q.ld_target = target.data_ptr(), _rows(target, "target")
-    return q, dev, n, a
+# agz_logprob_args as bytes (a ctypes.Structure takes several times as long to fill)
+_LP = struct.Struct("=qqqqii13q")
+assert _LP.size == C.sizeof(_lib.LogProbArgs)
 
 
 def _log_probs_forward(logits, moves, mask, target, top):
+    """Checked arguments -> (what the backward pass needs besides the tensors, move, entropy, target, top, top_move)."""
     L = _lib.load_library()
-    q, dev, n, a = _log_probs_args(logits, moves, mask, target, top)
-    # the outputs share one allocation: [stats 4][move][entropy][target][top_logp top][top_move top] x n
-    width = 6 + (target is not None) + 2 * top
-    need = L.agz_logprob_workspace(n, a, top)
-    flat = torch.empty(width * n, dtype=torch.float32, device=dev)
-    at = 4 * n
-    stats, parts = flat[:at], []
-    for want, w in ((moves is not None, 1), (True, 1), (target is not None, 1), (top > 0, top), (top > 0, top)):
-        parts.append(flat[at:at + w * n].view(*((n,) if w == 1 and len(parts) < 3 else (n, w))) if want else None)
-        at += w * n if want else 0
-    move, entropy, tl, tops, top_move = parts
+    n, a = logits.shape
+    i = logits.get_device()
+    f32 = {"dtype": torch.float32, "device": logits.device}
+    stats, entropy = torch.empty(n, 4, **f32), torch.empty(n, **f32)
+    move = None if moves is None else torch.empty(n, **f32)
+    expected = None if target is None else torch.empty(n, **f32)
+    tops = top_move = ws = None
     if top:
-        top_move = top_move.view(torch.int32)
-    q.stats, q.move_logp, q.entropy, q.target_logp, q.top_logp, q.top_move = map(_ptr, (stats, move, entropy, tl, tops, top_move))
+        tops, top_move = torch.empty(n, top, **f32), torch.empty(n, top, dtype=torch.int32, device=logits.device)
+    need = L.agz_logprob_workspace(n, a, top) if a > 1024 else 0      # (rows that fit a wave's registers need none)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        q.workspace, q.workspace_bytes = ws.data_ptr(), need
-    _lib_call(L.agz_logprob_forward(dev.index, _stream(dev), C.byref(q)), L)
-    return stats, move, entropy, tl, tops, top_move
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    head = (n, a, logits.data_ptr(), _rows(logits, "logits"), _CODE[logits.dtype], top,
+            0 if mask is None else mask.data_ptr(), 0 if mask is None or mask.shape[0] == 1 else mask.stride(0), 0 if moves is None else moves.data_ptr(),
+            0 if target is None else target.data_ptr(), 0 if target is None else _rows(target, "target"))
+    q = _LP.pack(*head, 0 if move is None else move.data_ptr(), entropy.data_ptr(), 0 if expected is None else expected.data_ptr(),
+                 tops.data_ptr() if top else 0, top_move.data_ptr() if top else 0, stats.data_ptr(), ws.data_ptr() if need else 0, need)
+    rc = L.agz_logprob_forward(i, _raw_stream(i), q)
+    if rc:
+        _lib_call(rc, L)
+    return (head, stats), move, entropy, expected, tops, top_move
+
+
+def _log_probs_backward(ctx, g_move, g_entropy, g_target, g_top, _):
+    if g_move is None and g_entropy is None and g_target is None and g_top is None:
+        return None, None, None, None, None
+    logits, _, _, _, top_move, stats = ctx.saved_tensors
+    L = _lib.load_library()
+    head = ctx.head
+    q = _LP.pack(*head, 0, 0, 0, 0, 0 if top_move is None else top_move.data_ptr(), stats.data_ptr(), 0, 0)
+    g = [None if x is None else x.contiguous() for x in (g_move, g_entropy, g_target, g_top)]     # (held here until the call is queued)
+    dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    i = logits.get_device()
+    rc = L.agz_logprob_backward(i, _raw_stream(i), q, *map(_ptr, g), dx.data_ptr(), head[1])
+    if rc:
+        _lib_call(rc, L)
+    return dx, None, None, None, None
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, moves, mask, target, top):
-        stats, *out = _log_probs_forward(logits, moves, mask, target, top)
+        (ctx.head, stats), *out = _log_probs_forward(logits, moves, mask, target, top)
         ctx.set_materialize_grads(False)
-        ctx.top = top
         ctx.save_for_backward(logits, moves, mask, target, out[4], stats)
-        if out[4] is not None:
+        if top:
             ctx.mark_non_differentiable(out[4])
         return tuple(out)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_move, g_entropy, g_target, g_top, _):
-        logits, moves, mask, target, top_move, stats = ctx.saved_tensors
-        if g_move is None and g_entropy is None and g_target is None and g_top is None:
-            return None, None, None, None, None
-        L = _lib.load_library()
-        q, dev, n, a = _log_probs_args(logits, moves, mask, target, ctx.top)
-        q.stats, q.top_move = stats.data_ptr(), _ptr(top_move)
-        g = [None if x is None else x.contiguous() for x in (g_move, g_entropy, g_target, g_top)]
-        dx = torch.empty((n, a), dtype=logits.dtype, device=dev)
-        _lib_call(L.agz_logprob_backward(dev.index, _stream(dev), C.byref(q), *map(_ptr, g), dx.data_ptr(), max(a, 1)), L)
-        return dx, None, None, None, None
+    def backward(ctx, *g):
+        # a backward pass that is recorded itself (create_graph): its own gradient is refused where it is asked for
+        return (_LogProbs._once if torch.is_grad_enabled() else _log_probs_backward)(ctx, *g)
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_log_probs_backward))
 
 
 def log_probs(logits, moves=None, mask=None, target=None, top=0):
@@ -145,22 +146,27 @@ def log_probs(logits, moves=None, mask=None, target=None, top=0):
     n, a = logits.shape
     dev = logits.device
     _need(a >= 1, "logits: no actions")
-    _need(isinstance(top, int) and 0 <= top <= min(TOP_MAX, a), f"top: 0 to {TOP_MAX} and at most the number of actions, not {top!r}")
+    if not (isinstance(top, int) and 0 <= top <= min(TOP_MAX, a)):
+        raise ValueError(f"top: 0 to {TOP_MAX} and at most the number of actions, not {top!r}")
     if moves is not None:
         _on_gpu(moves, "moves", dev)
-        _need(moves.shape == (n,) and moves.dtype in (torch.int64, torch.int32), f"moves: int64 or int32 [{n}], not {moves.dtype} {list(moves.shape)}")
+        if moves.shape != (n,) or moves.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"moves: int64 or int32 [{n}], not {moves.dtype} {list(moves.shape)}")
         if moves.dtype != torch.int64 or not moves.is_contiguous():
             moves = moves.long().contiguous()
     if mask is not None:
         _on_gpu(mask, "mask", dev)
-        _need(mask.dtype in (torch.bool, torch.uint8), f"mask: bool or uint8, not {mask.dtype}")
+        if mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"mask: bool or uint8, not {mask.dtype}")
         if mask.dim() == 1:
             mask = mask[None]
-        _need(mask.dim() == 2 and mask.shape[0] in (1, n) and mask.shape[1] == a, f"mask: [{n}, {a}], [1, {a}] or [{a}], not {list(mask.shape)}")
+        if mask.shape != (n, a) and mask.shape != (1, a):
+            raise ValueError(f"mask: [{n}, {a}], [1, {a}] or [{a}], not {list(mask.shape)}")
         _rows(mask, "mask")
     if target is not None:
         _on_gpu(target, "target", dev)
-        _need(target.dtype == torch.float32 and target.shape == (n, a), f"target: float32 [{n}, {a}], not {target.dtype} {list(target.shape)}")
+        if target.dtype != torch.float32 or target.shape != (n, a):
+            raise ValueError(f"target: float32 [{n}, {a}], not {target.dtype} {list(target.shape)}")
         _need(not target.requires_grad, "target: a constant is needed (detach() it)")
         _rows(target, "target")
     if logits.requires_grad and torch.is_grad_enabled():
@@ -207,7 +213,7 @@ def _quantize(x, block_rows, straight, transposed, gate=None, colsum=False):
         sums = torch.empty(c, dtype=torch.float32, device=dev)
         need = L.agz_fp8_colsum_ws(r, c)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    _lib_call(L.agz_fp8_quantize(dev.index, _stream(dev), x.data_ptr(), _CODE[x.dtype], r, c, ld, _ptr(gate), block_rows,
+    _lib_call(L.agz_fp8_quantize(dev.index, _raw_stream(dev.index), x.data_ptr(), _CODE[x.dtype], r, c, ld, _ptr(gate), block_rows,
                                  a and a.q.data_ptr() or None, a and a.scale.data_ptr() or None, t and t.q.data_ptr() or None, t and t.scale.data_ptr() or None,
                                  _ptr(sums), _ptr(ws), need), L)
     return a, t, sums
@@ -231,7 +237,7 @@ def _product(a, b, bias, relu, dtype):
     out = torch.empty((a.rows, b.rows), dtype=dtype, device=dev)
     need = L.agz_fp8_matmul_workspace(a.rows, b.rows, a.cols)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _lib_call(L.agz_fp8_matmul(dev.index, _stream(dev), a.rows, b.rows, a.cols, a.q.data_ptr(), a.scale.data_ptr(), b.q.data_ptr(), b.scale.data_ptr(),
+    _lib_call(L.agz_fp8_matmul(dev.index, _raw_stream(dev.index), a.rows, b.rows, a.cols, a.q.data_ptr(), a.scale.data_ptr(), b.q.data_ptr(), b.scale.data_ptr(),
                                _ptr(bias), 0 if bias is None else _CODE[bias.dtype], int(relu), out.data_ptr(), _CODE[dtype], max(b.rows, 1), _ptr(ws), need), L)
     return out
 
@@ -240,7 +246,8 @@ def _check_bias(bias, n, dev):
     if bias is not None:
         _on_gpu(bias, "bias", dev)
         _float_type(bias, "bias")
-        _need(bias.shape == (n,) and (n < 2 or bias.stride(0) == 1), f"bias: [{n}], contiguous, not {list(bias.shape)}")
+        if bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
+            raise ValueError(f"bias: [{n}], contiguous, not {list(bias.shape)}")
 
 
 def matmul_fp8(a, b, bias=None, relu=False, dtype=torch.bfloat16):
@@ -262,29 +269,64 @@ class Fp8Weight:
         self.matrix = quantize_fp8(w, block_rows=128)
 
 
+_LIN = struct.Struct("=qqqqqqqqiiii")               # agz_linear_fp8_args
+assert _LIN.size == C.sizeof(_lib.LinearFp8Args)
+
+
+def _linear_args(x, w, bias, relu):
+    m, k = x.shape
+    return _LIN.pack(m, w.shape[0], k, x.data_ptr(), _rows(x, "x"), w.data_ptr(), _rows(w, "w"), 0 if bias is None else bias.data_ptr(),
+                     _CODE[x.dtype], _CODE[w.dtype], 0 if bias is None else _CODE[bias.dtype], relu)
+
+
+def _linear_forward(x, w, bias, relu, need_x, need_w):
+    L = _lib.load_library()
+    (m, k), n, dev, i = x.shape, w.shape[0], x.device, x.get_device()
+    y = torch.empty(m, n, dtype=x.dtype, device=dev)
+    need = L.agz_linear_fp8_workspace(m, n, k)
+    if need < 0:
+        raise ValueError(f"linear_fp8: {m} x {n} x {k} is too large")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    saved = torch.empty(L.agz_linear_fp8_saved(m, n, k, need_x, need_w), dtype=torch.uint8, device=dev) if need_x or need_w else None
+    q = _linear_args(x, w, bias, relu)
+    rc = L.agz_linear_fp8_forward(i, _raw_stream(i), q, y.data_ptr(), _ptr(saved), need_x, need_w, ws.data_ptr(), need)
+    if rc:
+        _lib_call(rc, L)
+    return y, saved, q
+
+
+def _linear_backward(ctx, dy):
+    saved, y = ctx.saved_tensors
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    L = _lib.load_library()
+    m, n, k = ctx.sizes
+    dev, i = dy.device, dy.get_device()
+    dy = dy.contiguous()
+    dx = torch.empty(m, k, dtype=dy.dtype, device=dev) if need_x else None
+    dw = torch.empty(n, k, dtype=ctx.types[0], device=dev) if need_w else None
+    db = torch.empty(n, dtype=ctx.types[1], device=dev) if need_b else None
+    need = L.agz_linear_fp8_backward_workspace(m, n, k, need_x, need_w, need_b)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    rc = L.agz_linear_fp8_backward(i, _raw_stream(i), ctx.args, dy.data_ptr(), _ptr(y), _ptr(saved), ctx.kept[0], ctx.kept[1], _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), need)
+    if rc:
+        _lib_call(rc, L)
+    return dx, dw, db, None
+
+
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, relu):
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        a, at, _ = _quantize(x, 1, True, need_w)
-        b, bt, _ = _quantize(w, 128, True, need_x)
-        y = _product(a, b, bias, relu, x.dtype)
-        ctx.relu, ctx.types, ctx.shape = relu, (x.dtype, w.dtype, None if bias is None else bias.dtype), (x.shape[0], w.shape[0], w.shape[1])
-        ctx.save_for_backward(*(at and (at.q, at.scale) or (None, None)), *(bt and (bt.q, bt.scale) or (None, None)), y if relu else None)
+        ctx.kept = need_x, need_w = ctx.needs_input_grad[:2]
+        y, saved, ctx.args = _linear_forward(x, w, bias, relu, need_x, need_w)
+        ctx.sizes, ctx.types = (x.shape[0], *w.shape), (w.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(saved, y if relu else None)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        atq, ats, btq, bts, y = ctx.saved_tensors
-        m, n, k = ctx.shape
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dy = dy.contiguous()
-        d, dt, sums = _quantize(dy, 1, need_x, need_w or need_b, gate=y, colsum=need_b)
-        dx = _product(d, Fp8Matrix.of(btq, bts, k, n), None, False, ctx.types[0]) if need_x else None
-        dw = _product(dt, Fp8Matrix.of(atq, ats, k, m), None, False, ctx.types[1]) if need_w else None
-        db = sums.to(ctx.types[2]) if need_b else None
-        return dx, dw, db, None
+        return (_LinearFp8._once if torch.is_grad_enabled() else _linear_backward)(ctx, dy)
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_linear_backward))
 
 
 def linear_fp8(x, w, bias=None, relu=False):
@@ -304,23 +346,29 @@ def linear_fp8(x, w, bias=None, relu=False):
         _float_type(w, "w")
         _rows(w, "w")
         n, k = w.shape
-    _need(x.shape[-1] == k, f"x has {x.shape[-1]} columns, w {k}")
+    if x.shape[-1] != k:
+        raise ValueError(f"x has {x.shape[-1]} columns, w {k}")
     _check_bias(bias, n, dev)
     two = x if x.dim() == 2 else x.reshape(-1, k)
     _rows(two, "x")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not ready and w.requires_grad)):
         _need(not ready, "w: gradients need the weights themselves, not Fp8Weight")
         y = _LinearFp8.apply(two, w, bias, bool(relu))
-    else:
+    elif ready:
         a, _, _ = _quantize(two, 1, True, False)
-        b = w.matrix if ready else _quantize(w, 128, True, False)[0]
-        y = _product(a, b, bias, relu, x.dtype)
+        y = _product(a, w.matrix, bias, relu, x.dtype)
+    else:
+        y = _linear_forward(two, w, bias, bool(relu), False, False)[0]
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # AdamW
 # ---------------------------------------------------------------------------------------------------------------------------------------
+_ADAMW = struct.Struct("=dddddiiiIi4xqq")           # agz_adamw_options
+assert _ADAMW.size == C.sizeof(_lib.AdamWOptions)
+
+
 class AdamW:
     """AdamW (decoupled weight decay) over many tensors in one launch, in place:
 
@@ -396,7 +444,7 @@ class AdamW:
             pp[i] = p.data_ptr()
             if g is None:
                 continue
-            if g.device != self.device:
+            if g.get_device() != self.device.index:
                 raise ValueError(f"grads[{i}] is on {g.device}, the tensors on {self.device}")
             kind = kind or g.dtype
             if g.dtype != kind or kind not in _CODE:
@@ -412,10 +460,10 @@ class AdamW:
         else:
             self.step_dev.add_(1)
         t = self.steps + 1
-        o = _lib.AdamWOptions(lr=self.lr, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, weight_decay=self.weight_decay, param_dtype=_CODE[self.params[0].dtype],
-                              grad_dtype=_CODE[kind or torch.float32], bits=self.bits, seed=self.seed & 0xFFFFFFFF, step=t, step_dev=_ptr(self.step_dev))
+        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[self.params[0].dtype], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t,
+                        0 if self.step_dev is None else self.step_dev.data_ptr())
         second, ms, rs = (self.v, None, None) if self.bits == 32 else (self.r, self.m_scale, self.r_scale)
-        _lib_call(L.agz_adamw_step(self.device.index, _stream(self.device), C.byref(o), count, pp, gp, self._numel, self.m.data_ptr(), second.data_ptr(), _ptr(ms), _ptr(rs)), L)
+        _lib_call(L.agz_adamw_step(self.device.index, _raw_stream(self.device.index), o, count, pp, gp, self._numel, self.m.data_ptr(), second.data_ptr(), _ptr(ms), _ptr(rs)), L)
         torch.autograd.graph.increment_version(self.params)
         self.steps = t
 

@@ -319,6 +319,25 @@ int64_t agz_fp8_matmul_workspace(int64_t m, int64_t n, int64_t k);
 int  agz_fp8_matmul(int device, void *stream, int64_t m, int64_t n, int64_t k, const void *qa, const void *sa, const void *qb, const void *sb,
                     const void *bias, int bias_dtype, int relu, void *out, int out_dtype, int64_t ldo, void *workspace, int64_t workspace_bytes);
 
+/* A layer y = relu?(x w^T + bias) and its gradients in one call each: x [m][k] (dtype, row stride ldx), w [n][k] (w_dtype, ldw), bias [n] or NULL; y, dy [m][n]
+ * and dx [m][k] of type dtype, dw [n][k] of type w_dtype, db [n] of type bias_dtype, all without gaps.  x and dy are held in blocks of 1 x 128 along what is
+ * summed over, w in blocks of 128 x 128.  The forward call leaves in `saved` (agz_linear_fp8_saved bytes) what the backward call needs for dx (need_dx) and dw
+ * (need_dw): the transposes in 8 bits; the backward call gets the same flags as saved_dx, saved_dw, and computes those of dx, dw, db that are not NULL.
+ * (m, n up to 65535 x 128.)  saved and the workspaces: 256-byte aligned. */
+typedef struct {
+    int64_t m, n, k;
+    const void *x; int64_t ldx;
+    const void *w; int64_t ldw;
+    const void *bias;
+    int32_t dtype, w_dtype, bias_dtype, relu;
+} agz_linear_fp8_args;
+int64_t agz_linear_fp8_workspace(int64_t m, int64_t n, int64_t k);
+int64_t agz_linear_fp8_saved(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw);
+int64_t agz_linear_fp8_backward_workspace(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, int need_db);
+int  agz_linear_fp8_forward(int device, void *stream, const agz_linear_fp8_args *args, void *y, void *saved, int need_dx, int need_dw, void *workspace, int64_t workspace_bytes);
+int  agz_linear_fp8_backward(int device, void *stream, const agz_linear_fp8_args *args, const void *dy, const void *y, const void *saved, int saved_dx, int saved_dw,
+                             void *dx, void *dw, void *db, void *workspace, int64_t workspace_bytes);
+
 /* One AdamW step over `count` tensors (decoupled decay; train.jl:50 is ADAM with WeightDecay):
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * in 32 bits, p rounded once to its type.  The states of all tensors lie in common buffers: tensor i begins at element 128 x sum over the
