@@ -44,17 +44,70 @@ __device__ __forceinline__ float aw_round(float y, uint32_t u) {
     return __uint_as_float(t) - low;
 }
 
-// the simple form: one wave per block of 128 elements, two elements per lane
+// A workgroup takes AW_CHUNK neighbouring elements of one tensor, a lane AW_TURNS times four of them: every access is 16 (8, 4) bytes a lane and whole lines a
+// wave, and all of a lane's loads are under way before the first is used.  A block of 128 is half a wave: its largest is a reduction over 32 lanes.
+constexpr int AW_TURNS = 2, AW_CHUNK = 256 * 4 * AW_TURNS, AW_BLOCKS = AW_CHUNK / AW_BLOCK;
+
+template <typename T> __device__ __forceinline__ void load4(float* to, const T* from, int64_t i, int64_t n) {
+    if (i + 4 <= n) {
+        const Span<T, 4> v = *(const Span<T, 4>*)(from + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = to_f(v.e[e]);
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = i + e < n ? to_f(from[i + e]) : 0.0f;
+}
+// what is held for four elements in 8 bits: rounded as aw_round says; NaN for what is not finite (a block's scale counts its finite entries)
+template <bool FLOOR> __device__ __forceinline__ uint32_t aw_hold(const float* x, const uint32_t* u, uint8_t* scale, bool first) {
+    float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    if (__any(m == INFINITY)) {
+        m = 0.0f;
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+    }
+    const int b = scale_byte(lanes_max<32>(m));
+    if (first) *scale = (uint8_t)b;
+    const float inv = inv_scale_of(b);
+    float q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float y = fabsf(x[e]) * inv;
+        q[e] = aw_round(y, u[e]);
+        if (FLOOR) q[e] = y > 0.0f ? fmaxf(q[e], 0.001953125f) : q[e];
+        else q[e] = copysignf(q[e], x[e]);
+        if (!(y < INFINITY)) q[e] = NAN;
+    }
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+}
+
 template <typename P, typename G, int BITS>
 __global__ __launch_bounds__(256) void k_adamw(AwTable tab, AwPar a, void* mp, void* vp, uint8_t* ms, uint8_t* vs) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t chunk = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int tid = threadIdx.x;
     int lo = 0, hi = a.count;
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (tab.t[mid].chunk0 <= chunk) lo = mid; else hi = mid; }
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (tab.t[mid].chunk0 <= blockIdx.x) lo = mid; else hi = mid; }
     const AwTensor t = tab.t[lo];
-    const int64_t n = (int64_t)((uint64_t)t.n_hi << 32 | t.n_lo);
-    const int64_t blk = chunk - t.chunk0;
-    if (blk * AW_BLOCK >= n) return;
+    const int64_t n = (int64_t)((uint64_t)t.n_hi << 32 | t.n_lo), chunk = blockIdx.x - t.chunk0;
+    const int64_t full = (n + AW_BLOCK - 1) / AW_BLOCK * AW_BLOCK;          // the states go to the end of the last block
+    const int64_t i0 = chunk * AW_CHUNK + tid * 4, s0 = (int64_t)t.block0 * AW_BLOCK;
+    float p[AW_TURNS][4], g[AW_TURNS][4], m[AW_TURNS][4], v[AW_TURNS][4];
+    uint32_t mq[AW_TURNS], vq[AW_TURNS];
+    uint8_t mb[AW_TURNS], vb[AW_TURNS];
+#pragma unroll
+    for (int k = 0; k < AW_TURNS; ++k) {
+        const int64_t i = i0 + k * 1024;
+        if (i >= full) continue;
+        if (BITS == 32) {
+            *(float4*)m[k] = *(const float4*)((const float*)mp + s0 + i);
+            *(float4*)v[k] = *(const float4*)((const float*)vp + s0 + i);
+        } else {
+            mq[k] = *(const uint32_t*)((const uint8_t*)mp + s0 + i);
+            vq[k] = *(const uint32_t*)((const uint8_t*)vp + s0 + i);
+            mb[k] = ms[(s0 + i) / AW_BLOCK];
+            vb[k] = vs[(s0 + i) / AW_BLOCK];
+        }
+        load4(g[k], (const G*)t.g, i, n);
+        load4(p[k], (const P*)t.p, i, n);
+    }
     int64_t step = a.step;
     float step_size = a.step_size, inv_root = a.inv_root;
     if (a.step_dev) {
@@ -63,47 +116,48 @@ __global__ __launch_bounds__(256) void k_adamw(AwTable tab, AwPar a, void* mp, v
         inv_root = (float)(1.0 / sqrt(1.0 - aw_pow(a.b2d, step)));
     }
     const uint32_t key = aw_key(a.seed, (uint32_t)step, a.tensor0 + lo);
-    const int64_t state0 = ((int64_t)t.block0 + blk) * AW_BLOCK;
-    float m[2], r[2], v[2];
-    float m_scale = 1.0f, r_scale = 1.0f;
-    if (BITS == 8) { m_scale = scale_of(ms[t.block0 + blk]); r_scale = scale_of(vs[t.block0 + blk]); }
-    for (int k = 0; k < 2; ++k) {
-        const int64_t i = blk * AW_BLOCK + lane * 2 + k, si = state0 + lane * 2 + k;
-        const bool in = i < n;
-        const float g = in ? to_f(((const G*)t.g)[i]) : 0.0f;
-        if (BITS == 32) { m[k] = ((const float*)mp)[si]; v[k] = ((const float*)vp)[si]; }
-        else {
-            m[k] = __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)mp)[si], 0) * m_scale;
-            const float rr = __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)vp)[si], 0) * r_scale;
-            v[k] = rr * rr;
+#pragma unroll
+    for (int k = 0; k < AW_TURNS; ++k) {
+        const int64_t i = i0 + k * 1024;
+        if (i >= full) continue;                               // (a whole half wave: blocks begin at multiples of 32 lanes)
+        if (BITS == 8) {
+            const float fm = scale_of(mb[k]), fv = scale_of(vb[k]);
+            const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mq[k], false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mq[k], true);
+            const auto v01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vq[k], false), v23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vq[k], true);
+            m[k][0] = m01[0] * fm; m[k][1] = m01[1] * fm; m[k][2] = m23[0] * fm; m[k][3] = m23[1] * fm;
+            v[k][0] = v01[0] * fv; v[k][1] = v01[1] * fv; v[k][2] = v23[0] * fv; v[k][3] = v23[1] * fv;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][e] *= v[k][e];
         }
-        m[k] = m[k] * a.b1 + g * a.c1;
-        v[k] = v[k] * a.b2 + (g * g) * a.c2;
-        r[k] = sqrtf(v[k]);
-        if (in) {
-            P* p = (P*)t.p + i;
-            *p = from_f<P>(to_f(*p) * a.keep - (m[k] * step_size) / (r[k] * inv_root + a.eps));
+        float r[4];
+        uint32_t um[4], ur[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            m[k][e] = m[k][e] * a.b1 + g[k][e] * a.c1;
+            v[k][e] = v[k][e] * a.b2 + (g[k][e] * g[k][e]) * a.c2;
+            r[e] = sqrtf(v[k][e]);
+            p[k][e] = p[k][e] * a.keep - (m[k][e] * step_size) / (r[e] * inv_root + a.eps);
+            if (BITS == 8) {
+                const uint32_t h = aw_mix((uint32_t)(i + e) ^ (key + (uint32_t)(i >> 32) * 0x9E3779B1u));
+                um[e] = h & 0xFFFFu; ur[e] = h >> 16;
+            }
         }
-        if (BITS == 32) { ((float*)mp)[si] = m[k]; ((float*)vp)[si] = v[k]; }
-    }
-    if (BITS == 8) {
-        float am = 0.0f, ar = 0.0f;
-        for (int k = 0; k < 2; ++k) { am = fmaxf(am, fabsf(m[k]) < INFINITY ? fabsf(m[k]) : 0.0f); ar = fmaxf(ar, r[k] < INFINITY ? r[k] : 0.0f); }
-        const int bm = scale_byte(wave_max(am)), br = scale_byte(wave_max(ar));
-        const float im = inv_scale_of(bm), ir = inv_scale_of(br);
-        for (int k = 0; k < 2; ++k) {
-            const int64_t i = blk * AW_BLOCK + lane * 2 + k, si = state0 + lane * 2 + k;
-            const uint32_t h = aw_mix((uint32_t)i ^ (key + (uint32_t)(i >> 32) * 0x9E3779B1u));
-            const float ym = fabsf(m[k]) * im, yr = r[k] * ir;
-            float qm = ym < INFINITY ? copysignf(aw_round(ym, h & 0xFFFFu), m[k]) : NAN;
-            float qr = yr < INFINITY ? aw_round(yr, h >> 16) : NAN;
-            if (yr > 0.0f) qr = fmaxf(qr, 0.001953125f);
-            if (!(yr < INFINITY)) qr = NAN;
-            const int w = __builtin_amdgcn_cvt_pk_fp8_f32(qm, qr, 0, false);
-            ((uint8_t*)mp)[si] = (uint8_t)(w & 0xFF);
-            ((uint8_t*)vp)[si] = (uint8_t)(w >> 8 & 0xFF);
+        if (i + 4 <= n) {
+            Span<P, 4> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.e[e] = from_f<P>(p[k][e]);
+            *(Span<P, 4>*)((P*)t.p + i) = o;
+        } else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (i + e < n) ((P*)t.p)[i + e] = from_f<P>(p[k][e]);
+        if (BITS == 32) {
+            *(float4*)((float*)mp + s0 + i) = make_float4(m[k][0], m[k][1], m[k][2], m[k][3]);
+            *(float4*)((float*)vp + s0 + i) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+        } else {
+            const bool first = (tid & 31) == 0;
+            *(uint32_t*)((uint8_t*)mp + s0 + i) = aw_hold<false>(m[k], um, ms + (s0 + i) / AW_BLOCK, first);
+            *(uint32_t*)((uint8_t*)vp + s0 + i) = aw_hold<true>(r, ur, vs + (s0 + i) / AW_BLOCK, first);
         }
-        if (lane == 0) { ms[t.block0 + blk] = (uint8_t)bm; vs[t.block0 + blk] = (uint8_t)br; }
     }
 }
 
@@ -169,7 +223,7 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
             if (blocks > (1ll << 29)) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d has more than 2^36 elements", i);
             if (k > 0 && (state_block - base) + blocks > (1ll << 30)) break;
             tab.t[k++] = AwTensor{params[i], grads[i], (uint32_t)numel[i], (uint32_t)(numel[i] >> 32), chunks, (uint32_t)(state_block - base)};
-            chunks += grads[i] ? (uint32_t)blocks : 0;
+            chunks += grads[i] ? (uint32_t)cdiv(blocks, AW_BLOCKS) : 0;
             state_block += blocks;
         }
         if (chunks == 0) continue;
@@ -181,8 +235,8 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
         uint8_t* ms = o->bits == 8 ? (uint8_t*)m_scale + base : nullptr;
         uint8_t* vs = o->bits == 8 ? (uint8_t*)v_scale + base : nullptr;
         const int rc = by_dtype(o->param_dtype, [&](auto P) { return by_dtype(o->grad_dtype, [&](auto G) {
-            return o->bits == 8 ? launch(k_adamw<decltype(P), decltype(G), 8>, dim3((chunks + 3) / 4), dim3(256), 0, stream, tab, a, mp, vp, ms, vs)
-                                : launch(k_adamw<decltype(P), decltype(G), 32>, dim3((chunks + 3) / 4), dim3(256), 0, stream, tab, a, mp, vp, ms, vs);
+            return o->bits == 8 ? launch(k_adamw<decltype(P), decltype(G), 8>, dim3(chunks), dim3(256), 0, stream, tab, a, mp, vp, ms, vs)
+                                : launch(k_adamw<decltype(P), decltype(G), 32>, dim3(chunks), dim3(256), 0, stream, tab, a, mp, vp, ms, vs);
         }); });
         if (rc != AGZ_OK) return rc;
     }
