@@ -275,24 +275,79 @@ template <typename O> __device__ __forceinline__ void store4(O* to, f32x4 v, int
         for (int e = 0; e < 3; ++e) if (e < valid) to[e] = from_f<O>(v[e]);
     }
 }
+__device__ __forceinline__ f32x4 bias4(const MatPar& p, int64_t c) {
+    f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (p.bias && c + e < p.n) b[e] = load_as(p.bias, p.bias_dtype, c + e);
+    return b;
+}
+__device__ __forceinline__ f32x4 finish4(const MatPar& p, f32x4 v, f32x4 b) {
+    v += b;
+    if (p.relu)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.0f ? 0.0f : v[e];        // (NaN stays NaN)
+    return v;
+}
 __device__ __forceinline__ void store_row4(const MatPar& p, int64_t r, int64_t c, f32x4 v) {
     const int valid = (int)(p.n - c < 4 ? p.n - c : 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (p.bias && e < valid) v[e] += load_as(p.bias, p.bias_dtype, c + e);
-        if (p.relu) v[e] = v[e] < 0.0f ? 0.0f : v[e];        // (NaN stays NaN)
-    }
+    v = finish4(p, v, bias4(p, c));
     const int64_t at = r * p.ldo + c;
     if (p.out_dtype == AGZ_F32) store4((float*)p.out + at, v, valid);
     else if (p.out_dtype == AGZ_BF16) store4((bf16*)p.out + at, v, valid);
     else store4((f16*)p.out + at, v, valid);
 }
 
+template <int BM, int BN, int WM, int WN> struct Tile {
+    static constexpr int NT = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16, PA = BM * 8 / NT, PB = BN * 8 / NT;
+    static constexpr int STEP = (BM + BN) * FB, ROW = BN * 2 + 16, OUT = BM * ROW;         // bytes of a step, of a row and of all rows of a 16-bit result
+    static constexpr int LDS = 2 * STEP > OUT ? 2 * STEP : OUT;
+    static_assert(PA * NT == BM * 8 && PB * NT == BN * 8, "whole pieces");
+};
+
+// a tile's results: through LDS (rows padded by 16 bytes, so that the 16 rows that a store covers meet different banks), then whole rows to memory;
+// a result in 32 bits in two halves, by rows of waves
+template <typename O, typename TL, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void store_tile(uint8_t* lds, const f32x4 (&acc)[TL::FM][TL::FN], O* out, int64_t ld, int64_t m, int64_t n, int64_t m0, int64_t n0) {
+    constexpr int HALVES = sizeof(O) == 4 ? 2 : 1, RB = BM / HALVES, ROW = BN * sizeof(O) + 16, EV = 16 / sizeof(O), CHUNKS = BN / EV;
+    static_assert(WM % HALVES == 0 && RB * ROW <= TL::LDS, "a half of the tile fits");
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+        __syncthreads();
+        if (wm / RB == h) {
+#pragma unroll
+            for (int i = 0; i < TL::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < TL::FN; ++j) {
+                    Span<O, 4> s;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s.e[e] = from_f<O>(acc[i][j][e]);
+                    __builtin_memcpy(__builtin_assume_aligned(lds + (wm - h * RB + i * 16 + l16) * ROW + (wn + j * 16 + g * 4) * (int)sizeof(O), 8), &s, sizeof s);
+                }
+        }
+        __syncthreads();
+        for (int x = tid; x < RB * CHUNKS; x += TL::NT) {
+            const int r = x / CHUNKS, c = x % CHUNKS * EV;
+            const int64_t row = m0 + h * RB + r, col = n0 + c;
+            if (row >= m || col >= n) continue;
+            Span<O, EV> s;
+            __builtin_memcpy(&s, __builtin_assume_aligned(lds + r * ROW + c * (int)sizeof(O), 16), 16);
+            O* to = out + row * ld + col;
+            if (col + EV <= n) *(Span<O, EV>*)to = s;
+            else
+#pragma unroll
+                for (int e = 0; e < EV - 1; ++e) if (col + e < n) to[e] = s.e[e];
+        }
+    }
+}
+
 template <int BM, int BN, int WM, int WN, bool WIDE>
 __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
-    constexpr int NT = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][(BM + BN) * FB];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    using TL = Tile<BM, BN, WM, WN>;
+    constexpr int NT = TL::NT, FM = TL::FM, FN = TL::FN, PA = TL::PA, PB = TL::PB;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[TL::LDS];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
     // workgroups of one XCD (every eighth id) take neighbouring tiles: eight rows of tiles by all columns, so that their L2 holds the operands they share
     const uint32_t tm = (uint32_t)((p.m + BM - 1) / BM), tn = (uint32_t)((p.n + BN - 1) / BN), tiles = tm * tn;
     uint32_t id = blockIdx.x % tiles;
@@ -307,38 +362,30 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
     const int kb = (int)((p.k + FB - 1) / FB);
     const int k0 = (int)((int64_t)kb * slice / p.slices), k1 = (int)((int64_t)kb * (slice + 1) / p.slices);
 
-    // this thread's pieces of a step: piece tid + i NT of the tile's (BM + BN) * 8, whole waves in A or in B
-    constexpr int PA = BM * 8 / NT, PB = BN * 8 / NT;
-    static_assert(PA * NT == BM * 8 && PB * NT == BN * 8, "whole pieces");
-    const uint8_t* src[PA + PB];
+    // this thread's pieces of a step: piece tid + i NT of the tile's (BM + BN) * 8, whole waves in A or in B; offsets from the tile's first row
+    const uint32_t lastm = (uint32_t)(p.m - 1 - m0 < BM ? p.m - 1 - m0 : BM - 1), lastn = (uint32_t)(p.n - 1 - n0 < BN ? p.n - 1 - n0 : BN - 1);
+    const uint32_t pitch = (uint32_t)p.pitch, spitch = (uint32_t)p.spitch;
+    const uint8_t *qa = p.qa + m0 * p.pitch, *qb = p.qb + n0 * p.pitch, *sa = p.sa + m0 * p.spitch, *sb = p.sb + n0 * p.spitch;
+    uint32_t src[PA + PB];
 #pragma unroll
     for (int i = 0; i < PA + PB; ++i) {
-        const int piece = tid + (i < PA ? i : i - PA) * NT, r = piece >> 3, c = (piece & 7) ^ (r & 7);
-        int64_t row = (i < PA ? m0 : n0) + r;
-        const int64_t last = (i < PA ? p.m : p.n) - 1;
-        row = row < last ? row : last;
-        src[i] = (i < PA ? p.qa : p.qb) + row * p.pitch + c * 16;
+        const uint32_t piece = tid + (i < PA ? i : i - PA) * NT, r = piece >> 3, c = (piece & 7) ^ (r & 7), last = i < PA ? lastm : lastn;
+        src[i] = (r < last ? r : last) * pitch + c * 16;
     }
-    const int* sa[FM];
-    const int* sb[FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) { int64_t r = m0 + wm + i * 16 + l16; r = r < p.m ? r : p.m - 1; sa[i] = (const int*)(p.sa + r * p.spitch); }
-#pragma unroll
-    for (int j = 0; j < FN; ++j) { int64_t r = n0 + wn + j * 16 + l16; r = r < p.n ? r : p.n - 1; sb[j] = (const int*)(p.sb + r * p.spitch); }
-
     auto fetch = [&](int k, int buf) {
 #pragma unroll
         for (int i = 0; i < PA + PB; ++i)
-            __builtin_amdgcn_global_load_lds((gvoid*)(src[i] + (int64_t)k * FB), (lvoid*)(lds[buf] + (i < PA ? i : i - PA) * NT * 16 + (i < PA ? 0 : BM * FB) + w * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gvoid*)((i < PA ? qa : qb) + (int64_t)k * FB + src[i]), (lvoid*)(lds + buf * TL::STEP + (i < PA ? i : i - PA) * NT * 16 + (i < PA ? 0 : BM * FB) + w * 1024), 16, 0, 0);
     };
+    auto scale = [&](const uint8_t* s, uint32_t r, uint32_t last, int word) { return *(const uint32_t*)(s + word * 4 + (r < last ? r : last) * spitch); };
     f32x4 acc[FM][FN] = {};
     uint32_t as[FM], bs[FN];
     if (k0 < k1) {
         fetch(k0, 0);
 #pragma unroll
-        for (int i = 0; i < FM; ++i) as[i] = (uint32_t)sa[i][k0 >> 2] >> 8 * (k0 & 3);
+        for (int i = 0; i < FM; ++i) as[i] = scale(sa, wm + i * 16 + l16, lastm, k0 >> 2) >> 8 * (k0 & 3);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) bs[j] = (uint32_t)sb[j][k0 >> 2] >> 8 * (k0 & 3);
+        for (int j = 0; j < FN; ++j) bs[j] = scale(sb, wn + j * 16 + l16, lastn, k0 >> 2) >> 8 * (k0 & 3);
     }
     const int p0 = (g ^ (l16 & 7)) * 16, p1 = p0 ^ 64;
     for (int k = k0; k < k1; ++k) {
@@ -349,12 +396,12 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
         if (k + 1 < k1) fetch(k + 1, buf ^ 1);
         if (next) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i) an[i] = (uint32_t)sa[i][(k + 1) >> 2];
+            for (int i = 0; i < FM; ++i) an[i] = scale(sa, wm + i * 16 + l16, lastm, (k + 1) >> 2);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) bn[j] = (uint32_t)sb[j][(k + 1) >> 2];
+            for (int j = 0; j < FN; ++j) bn[j] = scale(sb, wn + j * 16 + l16, lastn, (k + 1) >> 2);
         }
-        const uint8_t* la = lds[buf] + (wm + l16) * FB;
-        const uint8_t* lb = lds[buf] + BM * FB + (wn + l16) * FB;
+        const uint8_t* la = lds + buf * TL::STEP + (wm + l16) * FB;
+        const uint8_t* lb = lds + buf * TL::STEP + BM * FB + (wn + l16) * FB;
         auto frag = [&](const uint8_t* base, int i) {
             const i32x4 x = *(const i32x4*)(base + i * 16 * FB + p0), y = *(const i32x4*)(base + i * 16 * FB + p1);
             return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -363,21 +410,24 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
             Wide bw[FN];
 #pragma unroll
             for (int j = 0; j < FN; ++j) bw[j] = widen(frag(lb, j), bs[j] & 0xFF);
+            i32x8 av = frag(la, 0);
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const Wide aw = widen(frag(la, i), as[i] & 0xFF);
+                const Wide aw = widen(av, as[i] & 0xFF);
+                if (i + 1 < FM) av = frag(la, i + 1);
 #pragma unroll
                 for (int j = 0; j < FN; ++j) acc[i][j] = mma_wide(bw[j], aw, acc[i][j]);
             }
         } else {
-            i32x8 bv[FN];
+            i32x8 bv[FN], av[2];
 #pragma unroll
             for (int j = 0; j < FN; ++j) bv[j] = frag(lb, j);
+            av[0] = frag(la, 0);
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const i32x8 av = frag(la, i);
+                if (i + 1 < FM) av[(i + 1) & 1] = frag(la, i + 1);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma<0>(bv[j], av, acc[i][j], (int)bs[j], (int)as[i]);
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma<0>(bv[j], av[i & 1], acc[i][j], (int)bs[j], (int)as[i]);
             }
         }
 #pragma unroll
@@ -385,18 +435,19 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) bs[j] = next ? bn[j] : bs[j] >> 8;
     }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t r = m0 + wm + i * 16 + l16;
-        if (r >= p.m) continue;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int64_t c = n0 + wn + j * 16 + g * 4;
-            if (c >= p.n) continue;
-            if (p.slices > 1) store4(p.part + ((int64_t)slice * p.m + r) * p.n + c, acc[i][j], (int)(p.n - c < 4 ? p.n - c : 4));
-            else store_row4(p, r, c, acc[i][j]);
-        }
+    if (p.slices > 1) {
+        store_tile<float, TL, BM, BN, WM, WN>(lds, acc, p.part + (int64_t)slice * p.m * p.n, p.n, p.m, p.n, m0, n0);
+        return;
     }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const f32x4 b = bias4(p, n0 + wn + j * 16 + g * 4);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[i][j] = finish4(p, acc[i][j], b);
+    }
+    if (p.out_dtype == AGZ_F32) { if constexpr (WIDE) store_tile<float, TL, BM, BN, WM, WN>(lds, acc, (float*)p.out, p.ldo, p.m, p.n, m0, n0); }
+    else if (p.out_dtype == AGZ_BF16) store_tile<bf16, TL, BM, BN, WM, WN>(lds, acc, (bf16*)p.out, p.ldo, p.m, p.n, m0, n0);
+    else store_tile<f16, TL, BM, BN, WM, WN>(lds, acc, (f16*)p.out, p.ldo, p.m, p.n, m0, n0);
 }
 
 // the slices of the k axis added up, in order
@@ -462,6 +513,7 @@ template <bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) void k_matmul_
 using namespace agz::ops;
 
 static bool too_large(int64_t a) { return a > (1ll << 31) - 256; }
+static bool too_deep(int64_t k) { return k > (1ll << 24) - FB; }       // 255 rows of a tile and their pitch in 32 bits
 
 // How a product runs: `few` rows, or tiles of 256 or 128 a side and slices of the k axis.  A tile of 256 reads half as much per operation and needs a whole CU; where
 // there are fewer of them than CUs, tiles of 128 (two a CU), and where these leave CUs idle too, the k axis is cut so that there are
@@ -524,7 +576,7 @@ struct Carve {
     uint8_t* take(int64_t bytes) { uint8_t* p = base ? base + at : nullptr; at += up(bytes, 256); return p; }
     Mat8 matrix(int64_t rows, int64_t cols) { Mat8 m; m.q = take(rows * up(cols, FB)); m.s = take(rows * up(cdiv(cols, FB), 4)); return m; }
 };
-bool good_sizes(int64_t m, int64_t n, int64_t k) { return m >= 0 && n >= 0 && k >= 0 && !too_large(m) && !too_large(n) && !too_large(k) && cdiv(m, FB) <= 65535 && cdiv(n, FB) <= 65535; }
+bool good_sizes(int64_t m, int64_t n, int64_t k) { return m >= 0 && n >= 0 && k >= 0 && !too_large(m) && !too_large(n) && !too_deep(k) && cdiv(m, FB) <= 65535 && cdiv(n, FB) <= 65535; }
 struct Forward { Mat8 a, b; void* ws; };
 Forward forward_ws(Carve& c, int64_t m, int64_t n, int64_t k) { return {c.matrix(m, k), c.matrix(n, k), c.take(agz_fp8_matmul_workspace(m, n, k))}; }
 struct Saved { Mat8 at, bt; };
@@ -578,7 +630,7 @@ int agz_fp8_quantize(int device, void* stream, const void* x, int dtype, int64_t
 }
 
 int64_t agz_fp8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
-    if (m < 0 || n < 0 || k < 0 || too_large(m) || too_large(n) || too_large(k)) return -1;
+    if (m < 0 || n < 0 || k < 0 || too_large(m) || too_large(n) || too_deep(k)) return -1;
     if (m == 0 || n == 0) return 0;
     const Plan w = plan(m, n, k);
     return w.slices > 1 ? w.slices * m * n * 4 : 0;
