@@ -258,8 +258,8 @@ __device__ __forceinline__ f32x4 mma_wide(const Wide& a, const Wide& b, f32x4 c)
 // (global_load_lds, 16 bytes a lane), two steps deep, one barrier per step.  The 16-byte piece c of row r lies at piece c ^ (r & 7), so that the
 // eight lanes that a ds_read_b128 serves at a time, eight rows of one piece, meet all banks once (the permutation is on the memory side: the DMA
 // writes lanes in order).  WM x WN waves, each BM / WM x BN / WN in tiles of 16 x 16; B is the first operand, so that a lane ends with four
-// neighbouring columns of one row.  Rows and columns outside are read from the last one and not stored.  Scales: a word holds a row's bytes of four steps,
-// read one word ahead.
+// neighbouring columns of one row.  Rows and columns outside are read from the last one and not stored.  Scales: a word holds a row's bytes of four steps; the words
+// go through LDS too (a load to registers inside the loop would have to be waited for, and with it the next step's loads).
 // ---------------------------------------------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(1))) const void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
@@ -300,8 +300,8 @@ __device__ __forceinline__ void store_row4(const MatPar& p, int64_t r, int64_t c
 template <int BM, int BN, int WM, int WN> struct Tile {
     static constexpr int NT = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16, PA = BM * 8 / NT, PB = BN * 8 / NT;
     static constexpr int STEP = (BM + BN) * FB, ROW = BN * 2 + 16, OUT = BM * ROW;         // bytes of a step, of a row and of all rows of a 16-bit result
-    static constexpr int LDS = 2 * STEP > OUT ? 2 * STEP : OUT;
-    static_assert(PA * NT == BM * 8 && PB * NT == BN * 8, "whole pieces");
+    static constexpr int IN = 2 * STEP + 2 * (BM + BN) * 4, LDS = IN > OUT ? IN : OUT;     // two steps and two groups of scale words
+    static_assert((BM + BN) % NT == 0 && BM % 64 == 0 && PA * NT == BM * 8 && PB * NT == BN * 8, "whole pieces");
 };
 
 // a tile's results: through LDS (rows padded by 16 bytes, so that the 16 rows that a store covers meet different banks), then whole rows to memory;
@@ -377,35 +377,42 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
         for (int i = 0; i < PA + PB; ++i)
             __builtin_amdgcn_global_load_lds((gvoid*)((i < PA ? qa : qb) + (int64_t)k * FB + src[i]), (lvoid*)(lds + buf * TL::STEP + (i < PA ? i : i - PA) * NT * 16 + (i < PA ? 0 : BM * FB) + w * 1024), 16, 0, 0);
     };
-    auto scale = [&](const uint8_t* s, uint32_t r, uint32_t last, int word) { return *(const uint32_t*)(s + word * 4 + (r < last ? r : last) * spitch); };
+    // scale words of a group of four steps: one per row of the tile, BM + BN of them, into the buffer of the group's parity
+    auto fetch_scales = [&](int word) {
+#pragma unroll
+        for (int i = 0; i < (BM + BN) / NT; ++i) {
+            const uint32_t x = tid + i * NT, r = x < BM ? x : x - BM, last = x < BM ? lastm : lastn;
+            __builtin_amdgcn_global_load_lds((gvoid*)((x < BM ? sa : sb) + (r < last ? r : last) * spitch + word * 4), (lvoid*)(lds + 2 * TL::STEP + (word & 1) * (BM + BN) * 4 + i * NT * 4 + w * 256), 4, 0, 0);
+        }
+    };
     f32x4 acc[FM][FN] = {};
     uint32_t as[FM], bs[FN];
     if (k0 < k1) {
+        fetch_scales(k0 >> 2);
         fetch(k0, 0);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) as[i] = scale(sa, wm + i * 16 + l16, lastm, k0 >> 2) >> 8 * (k0 & 3);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) bs[j] = scale(sb, wn + j * 16 + l16, lastn, k0 >> 2) >> 8 * (k0 & 3);
     }
     const int p0 = (g ^ (l16 & 7)) * 16, p1 = p0 ^ 64;
     for (int k = k0; k < k1; ++k) {
         const int buf = (k - k0) & 1;
         __syncthreads();                                         // step k is in LDS, and everybody is done with the buffer of step k - 1
-        uint32_t an[FM], bn[FN];
-        const bool next = ((k + 1) & 3) == 0 && k + 1 < k1;
-        if (k + 1 < k1) fetch(k + 1, buf ^ 1);
-        if (next) {
-#pragma unroll
-            for (int i = 0; i < FM; ++i) an[i] = scale(sa, wm + i * 16 + l16, lastm, (k + 1) >> 2);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) bn[j] = scale(sb, wn + j * 16 + l16, lastn, (k + 1) >> 2);
+        if (k + 1 < k1) {
+            if (((k + 1) & 3) == 0) fetch_scales((k + 1) >> 2);
+            fetch(k + 1, buf ^ 1);
         }
         const uint8_t* la = lds + buf * TL::STEP + (wm + l16) * FB;
         const uint8_t* lb = lds + buf * TL::STEP + BM * FB + (wn + l16) * FB;
+        if (k == k0 || (k & 3) == 0) {
+            const uint32_t* words = (const uint32_t*)(lds + 2 * TL::STEP + ((k >> 2) & 1) * (BM + BN) * 4) + l16;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) as[i] = words[wm + i * 16] >> 8 * (k & 3);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) bs[j] = words[BM + wn + j * 16] >> 8 * (k & 3);
+        }
         auto frag = [&](const uint8_t* base, int i) {
             const i32x4 x = *(const i32x4*)(base + i * 16 * FB + p0), y = *(const i32x4*)(base + i * 16 * FB + p1);
             return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
         };
+        // (the scheduler would move a row's read behind the products of the row before it, into the same registers: the barriers keep it one row ahead)
         if constexpr (WIDE) {
             Wide bw[FN];
 #pragma unroll
@@ -415,25 +422,28 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
             for (int i = 0; i < FM; ++i) {
                 const Wide aw = widen(av, as[i] & 0xFF);
                 if (i + 1 < FM) av = frag(la, i + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int j = 0; j < FN; ++j) acc[i][j] = mma_wide(bw[j], aw, acc[i][j]);
             }
         } else {
             i32x8 bv[FN], av[2];
+            av[0] = frag(la, 0);
 #pragma unroll
             for (int j = 0; j < FN; ++j) bv[j] = frag(lb, j);
-            av[0] = frag(la, 0);
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 if (i + 1 < FM) av[(i + 1) & 1] = frag(la, i + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int j = 0; j < FN; ++j) acc[i][j] = mma<0>(bv[j], av[i & 1], acc[i][j], (int)bs[j], (int)as[i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
-        for (int i = 0; i < FM; ++i) as[i] = next ? an[i] : as[i] >> 8;
+        for (int i = 0; i < FM; ++i) as[i] >>= 8;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) bs[j] = next ? bn[j] : bs[j] >> 8;
+        for (int j = 0; j < FN; ++j) bs[j] >>= 8;
     }
     if (p.slices > 1) {
         store_tile<float, TL, BM, BN, WM, WN>(lds, acc, p.part + (int64_t)slice * p.m * p.n, p.n, p.m, p.n, m0, n0);
