@@ -41,29 +41,49 @@ __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
     __shared__ __attribute__((aligned(16))) float red[4][FB];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15;
     const int64_t r0 = (int64_t)blockIdx.y * FB + w * 32 + (lane >> 4) * 8, c0 = (int64_t)blockIdx.x * FB, c = c0 + l16 * 8;
+    // Straight-line loads, all under way at once: rows behind the last read the last one, and where the matrix ends inside a lane's eight columns the eight
+    // that end with it are read and moved down; what is outside counts as 0.
     float v[8][8];
+    const bool whole = c0 + FB <= p.cols && ((int64_t)blockIdx.y + 1) * FB <= p.rows;      // (of the workgroup)
     {
-        const int n = (int)(c >= p.cols ? 0 : (p.cols - c < 8 ? p.cols - c : 8));
+        const int64_t cl = c < p.cols - 8 ? c : p.cols - 8;
         Span<T, 8> x[8], y[8];
+        if (p.cols >= 8) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (r0 + k < p.rows) {
-                const T* at = (const T*)p.x + (r0 + k) * p.ld + c;
-                const T* gt = (const T*)p.gate + (r0 + k) * p.ld + c;
-                if (n == 8) {
-                    x[k] = *(const Span<T, 8>*)at;
-                    if (p.gate) y[k] = *(const Span<T, 8>*)gt;
-                } else
-#pragma unroll
-                    for (int e = 0; e < 7; ++e) if (e < n) { x[k].e[e] = at[e]; if (p.gate) y[k].e[e] = gt[e]; }
+            for (int k = 0; k < 8; ++k) {
+                const int64_t at = (r0 + k < p.rows ? r0 + k : p.rows - 1) * p.ld + cl;
+                x[k] = *(const Span<T, 8>*)((const T*)p.x + at);
+                if (p.gate) y[k] = *(const Span<T, 8>*)((const T*)p.gate + at);
             }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                for (int e = 0; e < (int)p.cols; ++e) {
+                    const int64_t at = (r0 + k < p.rows ? r0 + k : p.rows - 1) * p.ld + e;
+                    const T xe = ((const T*)p.x)[at], ye = p.gate ? ((const T*)p.gate)[at] : T{};
+#pragma unroll
+                    for (int o = 0; o < 8; ++o) if (o == e) { x[k].e[o] = xe; y[k].e[o] = ye; }
+                }
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[k][e] = r0 + k < p.rows && e < n ? to_f(x[k].e[e]) : 0.0f;
-                if (p.gate && r0 + k < p.rows && e < n && !(to_f(y[k].e[e]) > 0.0f)) v[k][e] = 0.0f;
+                v[k][e] = to_f(x[k].e[e]);
+                if (p.gate && !(to_f(y[k].e[e]) > 0.0f)) v[k][e] = 0.0f;
             }
+        if (!whole) {
+            const int down = p.cols >= 8 ? (int)(c - cl < 8 ? c - cl : 8) : 0, n = (int)(c >= p.cols ? 0 : (p.cols - c < 8 ? p.cols - c : 8));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                for (int s = 4; s; s >>= 1)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[k][e] = (down & s) ? (e + s < 8 ? v[k][e + s] : 0.0f) : v[k][e];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] = e < n && r0 + k < p.rows ? v[k][e] : 0.0f;
+            }
+        }
     }
     auto max2 = [](float a, float b) { return fmaxf(a, b); };
     auto finite = [](float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; };
@@ -467,16 +487,27 @@ __global__ __launch_bounds__(256) void k_matmul_join(MatPar p) {
     const int valid = (int)(p.n - c < 4 ? p.n - c : 4);
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     const float* at = p.part + r * p.n + c;
-    for (int s = 0; s < p.slices; ++s, at += p.m * p.n) {
-        if (valid == 4) {
-            const Span<float, 4> t = *(const Span<float, 4>*)at;
+    const int64_t next = p.m * p.n;
+    if (valid == 4) {
+        int s = 0;
+        for (; s + 8 <= p.slices; s += 8) {                      // eight loads under way
+            Span<float, 4> t[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) t[u] = *(const Span<float, 4>*)(at + (s + u) * next);
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += t[u].e[e];
+        }
+        for (; s < p.slices; ++s) {
+            const Span<float, 4> t = *(const Span<float, 4>*)(at + s * next);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += t.e[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 3; ++e) if (e < valid) v[e] += at[e];
         }
-    }
+    } else
+        for (int s = 0; s < p.slices; ++s)
+#pragma unroll
+            for (int e = 0; e < 3; ++e) if (e < valid) v[e] += at[s * next + e];
     store_row4(p, r, c, v);
 }
 
