@@ -1,6 +1,7 @@
 // agz_fp8.hip — matrices in 8 bits (e4m3 with one power-of-two scale per block of 128) and their product on the matrix units
 // (include/agz.h agz_fp8_quantize / agz_fp8_matmul): the layers of the network, forward and backward (DenseNet.jl:161-198, 294-304).
 #include "agz_ops.hpp"
+#include <type_traits>
 
 namespace agz {
 namespace ops {
@@ -36,9 +37,10 @@ template <typename F> __device__ __forceinline__ float groups_reduce(float x, F&
 // written eight at a time both ways (8 x 8 values: the transpose is a matter of which eight are packed).  A row's largest is a reduction over
 // 16 lanes, a column's one over 4 lanes and, through LDS, the 4 waves.  fmaxf passes NaN over; a largest of infinity means that the block has one, and its largest
 // finite entry is looked for again.
-template <typename T, int BR, bool ROW, bool COL>
+template <typename T, int BR, bool ROW, bool COL, bool GATE, bool NARROW>
 __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
     __shared__ __attribute__((aligned(16))) float red[4][FB];
+    __shared__ uint2 turn[COL ? FB : 1][16];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15;
     const int64_t r0 = (int64_t)blockIdx.y * FB + w * 32 + (lane >> 4) * 8, c0 = (int64_t)blockIdx.x * FB, c = c0 + l16 * 8;
     // Straight-line loads, all under way at once: rows behind the last read the last one, and where the matrix ends inside a lane's eight columns the eight
@@ -48,21 +50,21 @@ __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
     {
         const int64_t cl = c < p.cols - 8 ? c : p.cols - 8;
         Span<T, 8> x[8], y[8];
-        if (p.cols >= 8) {
+        if constexpr (!NARROW) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const int64_t at = (r0 + k < p.rows ? r0 + k : p.rows - 1) * p.ld + cl;
                 x[k] = *(const Span<T, 8>*)((const T*)p.x + at);
-                if (p.gate) y[k] = *(const Span<T, 8>*)((const T*)p.gate + at);
+                if (GATE) y[k] = *(const Span<T, 8>*)((const T*)p.gate + at);
             }
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                for (int e = 0; e < (int)p.cols; ++e) {
-                    const int64_t at = (r0 + k < p.rows ? r0 + k : p.rows - 1) * p.ld + e;
-                    const T xe = ((const T*)p.x)[at], ye = p.gate ? ((const T*)p.gate)[at] : T{};
 #pragma unroll
-                    for (int o = 0; o < 8; ++o) if (o == e) { x[k].e[o] = xe; y[k].e[o] = ye; }
+                for (int e = 0; e < 8; ++e) {
+                    const int64_t at = (r0 + k < p.rows ? r0 + k : p.rows - 1) * p.ld + (e < p.cols ? e : p.cols - 1);
+                    x[k].e[e] = ((const T*)p.x)[at];
+                    if (GATE) y[k].e[e] = ((const T*)p.gate)[at];
                 }
         }
 #pragma unroll
@@ -70,10 +72,10 @@ __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[k][e] = to_f(x[k].e[e]);
-                if (p.gate && !(to_f(y[k].e[e]) > 0.0f)) v[k][e] = 0.0f;
+                if (GATE && !(to_f(y[k].e[e]) > 0.0f)) v[k][e] = 0.0f;
             }
         if (!whole) {
-            const int down = p.cols >= 8 ? (int)(c - cl < 8 ? c - cl : 8) : 0, n = (int)(c >= p.cols ? 0 : (p.cols - c < 8 ? p.cols - c : 8));
+            const int down = !NARROW ? (int)(c - cl < 8 ? c - cl : 8) : 0, n = (int)(c >= p.cols ? 0 : (p.cols - c < 8 ? p.cols - c : 8));
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
 #pragma unroll
@@ -175,11 +177,19 @@ __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
                 }
             }
         }
+        // through LDS, so that a column's 128 bytes leave as one line: piece j (8 bytes) of column c lies at piece j + c / 8 of its 16, which spreads a store's
+        // 16 columns, eight apart, over all banks
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (c + e >= p.cols) continue;
             const float t[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
-            *(uint2*)(p.qt + (c + e) * p.tpitch + r0) = enc8(t, inv[e]);
+            turn[l16 * 8 + e][(w * 4 + (lane >> 4) + l16) & 15] = enc8(t, inv[e]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int col = k * 32 + (threadIdx.x >> 3), j = (threadIdx.x & 7) * 2 + (col >> 3);
+            const uint2 lo = turn[col][j & 15], hi = turn[col][(j + 1) & 15];
+            if (c0 + col < p.cols) *(uint4*)(p.qt + (c0 + col) * p.tpitch + (int64_t)blockIdx.y * FB + (threadIdx.x & 7) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
         if (p.part) {
             float sum[8];
@@ -582,14 +592,18 @@ int quantize(void* stream, const void* x, int dtype, int64_t rows, int64_t cols,
         const dim3 grid((uint32_t)cdiv(cols, FB), (uint32_t)cdiv(rows, FB));
         const int rc = by_dtype(dtype, [&](auto T) {
             using X = decltype(T);
-            if (block_rows == 1) {
-                if (a.q && t.q) return launch(k_quantize<X, 1, true, true>, grid, dim3(256), 0, stream, p);
-                if (a.q) return launch(k_quantize<X, 1, true, false>, grid, dim3(256), 0, stream, p);
-                return launch(k_quantize<X, 1, false, true>, grid, dim3(256), 0, stream, p);
-            }
-            if (a.q && t.q) return launch(k_quantize<X, FB, true, true>, grid, dim3(256), 0, stream, p);
-            if (a.q) return launch(k_quantize<X, FB, true, false>, grid, dim3(256), 0, stream, p);
-            return launch(k_quantize<X, FB, false, true>, grid, dim3(256), 0, stream, p);
+            auto go = [&](auto br, auto gated) {
+                if (cols < 8)
+                    return a.q && t.q ? launch(k_quantize<X, br(), true, true, gated(), true>, grid, dim3(256), 0, stream, p)
+                         : a.q ? launch(k_quantize<X, br(), true, false, gated(), true>, grid, dim3(256), 0, stream, p)
+                               : launch(k_quantize<X, br(), false, true, gated(), true>, grid, dim3(256), 0, stream, p);
+                if (a.q && t.q) return launch(k_quantize<X, br(), true, true, gated(), false>, grid, dim3(256), 0, stream, p);
+                if (a.q) return launch(k_quantize<X, br(), true, false, gated(), false>, grid, dim3(256), 0, stream, p);
+                return launch(k_quantize<X, br(), false, true, gated(), false>, grid, dim3(256), 0, stream, p);
+            };
+            using std::integral_constant;
+            if (block_rows == 1) return gate ? go(integral_constant<int, 1>{}, std::true_type{}) : go(integral_constant<int, 1>{}, std::false_type{});
+            return gate ? go(integral_constant<int, FB>{}, std::true_type{}) : go(integral_constant<int, FB>{}, std::false_type{});
         });
         if (rc != AGZ_OK) return rc;
     }
