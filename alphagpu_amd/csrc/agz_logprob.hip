@@ -94,6 +94,71 @@ __device__ __forceinline__ Sums row_sums(const Row<T, VEC, G, NV>& r, const floa
     return o;
 }
 
+// order of the alternatives as one unsigned number: larger logits first, then lower indices; 0 = none
+__device__ __forceinline__ uint64_t lp_key(float x, uint32_t j) {
+    uint32_t b = __float_as_uint(x + 0.0f);                  // (-0 -> +0: equal logits)
+    b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    return (uint64_t)b << 32 | (uint32_t)~j;
+}
+__device__ __forceinline__ float lp_key_value(uint64_t k) {
+    const uint32_t b = (uint32_t)(k >> 32);
+    return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
+}
+// the places of a list of different keys in LDS: emit(place, key) for the first `top`, emit(place, 0) for the places that nobody has
+template <typename E> __device__ __forceinline__ void wave_list_ranks(const uint64_t* list, int count, int top, E&& emit) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int lane = threadIdx.x & 63;
+    for (int q = lane; q < count; q += 64) {
+        const uint64_t mine = list[q];
+        int before = 0;
+#pragma unroll 8
+        for (int o = 0; o < count; ++o) before += list[o] > mine ? 1 : 0;
+        if (before < top) emit(before, mine);
+    }
+    for (int k = count + lane; k < top; k += 64) emit(k, (uint64_t)0);
+}
+
+// The `top` best entries of what a wave holds (NE per lane, -inf: not allowed), largest first: emit(rank, key) from the lane that finds it, emit(rank, 0) behind
+// the last.  Every lane's best: the top-th largest of these 64 is a lower bound of the top-th largest entry.  The entries from that bound on (at most top lanes'
+// shares) go into a list in LDS, and an entry's place is the number of entries before it: all comparisons are independent, where taking the best again and
+// again is a chain of `top` reductions (20 of a row of 131072: part launch 41.5 -> 7 us).
+constexpr int LIST = AGZ_TOP_MAX * 32;
+template <int NE, typename J, typename E> __device__ __forceinline__ void wave_top(const float (&x)[NE], J&& index, int top, uint64_t* list, E&& emit) {
+    static_assert(NE <= 32, "the list holds the shares of AGZ_TOP_MAX lanes");
+    const int lane = threadIdx.x & 63;
+    float v = -INFINITY;
+    uint32_t j = 0;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) if (x[k] > v) { v = x[k]; j = index(k); }
+    const uint64_t mine = v > -INFINITY ? lp_key(v, j) : 0;
+    const uint32_t hi = (uint32_t)(mine >> 32), lo = (uint32_t)mine;
+    int before = 0;
+#pragma unroll 8
+    for (int o = 0; o < 64; ++o) {
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, o) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, o);
+        before += other > mine ? 1 : 0;
+    }
+    const uint64_t at = __ballot(mine != 0 && before == top - 1);
+    uint64_t bound = 1;                                        // fewer than `top` lanes with an entry: every entry
+    if (at) {
+        const int o = __builtin_ctzll(at);
+        bound = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, o) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, o);
+    }
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+        const uint64_t key = x[k] > -INFINITY ? lp_key(x[k], index(k)) : 0;
+        const uint64_t in = __ballot(key >= bound);
+        if (in) {
+            if (key >= bound) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = key;
+            count += __popcll(in);
+        }
+    }
+    wave_list_ranks(list, count, top, emit);
+}
+
 // The next best entry of what G lanes hold, taken out of it: its value (-inf: none is left) and its index.  Equal entries by index: every lane offers the
 // first of its largest, the lowest index among the lanes whose offer is the largest wins.
 template <int N> struct Offer { float v; uint32_t j; int k; };
@@ -155,62 +220,123 @@ template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) 
     const Done f = finish(p, i, q, xm, given, l == 0);
     if (p.top > 0) {
         const float off = base_of(q.mx);
-        auto o = offer(r);
-        for (int k = 0; k < p.top; ++k) {
-            uint32_t j;
-            const float v = take_best(r, o, j);
-            if (l == 0) {
-                const bool some = v > -INFINITY && !f.bad;
-                if (p.top_move) p.top_move[i * p.top + k] = some ? (int32_t)j : -1;
-                if (p.top_logp) p.top_logp[i * p.top + k] = some ? v - off - f.ls : (f.bad ? NAN : -INFINITY);
+        auto put = [&](int k, bool some, float v, uint32_t j) {
+            some = some && !f.bad;
+            if (p.top_move) p.top_move[i * p.top + k] = some ? (int32_t)j : -1;
+            if (p.top_logp) p.top_logp[i * p.top + k] = some ? v - off - f.ls : (f.bad ? NAN : -INFINITY);
+        };
+        if constexpr (G == 64) {
+            __shared__ uint64_t list[4][LIST];
+            wave_top(r.x, [&](int k) { return (uint32_t)(r.at[k / VEC] + k % VEC); }, p.top, list[threadIdx.x >> 6], [&](int k, uint64_t key) { put(k, key != 0, lp_key_value(key), ~(uint32_t)key); });
+        } else {
+            auto o = offer(r);
+            for (int k = 0; k < p.top; ++k) {
+                uint32_t j;
+                const float v = take_best(r, o, j);
+                if (l == 0) put(k, v > -INFINITY, v, j);
             }
         }
     }
 }
 
-// Longer rows: one wave per part of PART elements leaves the part's sums and best alternatives (as keys) in the workspace, a second launch joins
-// the parts of a row.  Parts of one size whatever the number of rows: one row of 131072 is 64 waves, 4096 rows of 50001 are 102400.
-constexpr int PART = 2048;
+// Longer rows: one wave per part leaves the part's sums and best alternatives (as keys) in the workspace, a second launch joins the parts of a row.  A part
+// is one block of PART elements where alternatives are wanted or rows are few, up to MOST blocks where there are waves enough without: a lane then carries its
+// own maximum and sums from block to block (the sums rescaled where the maximum grows), the next block's loads under way behind them,
+// and the lanes are joined once.  (4096 rows of 50001 bf16: a block a wave 221 us.)
+constexpr int PART = 2048, MOST = 16, WAVES_ENOUGH = 8192;
 struct PartOut { Sums q; float pad[3]; };
 
-// order of the alternatives as one unsigned number: larger logits first, then lower indices; 0 = none
-__device__ __forceinline__ uint64_t lp_key(float x, uint32_t j) {
-    uint32_t b = __float_as_uint(x + 0.0f);                  // (-0 -> +0: equal logits)
-    b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    return (uint64_t)b << 32 | (uint32_t)~j;
-}
-__device__ __forceinline__ float lp_key_value(uint64_t k) {
-    const uint32_t b = (uint32_t)(k >> 32);
-    return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
-}
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t x) {
-    const uint32_t hi = lanes_reduce<64>((uint32_t)(x >> 32), [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-    const uint32_t lo = lanes_reduce<64>((uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-    return (uint64_t)hi << 32 | lo;
+// blocks of a part and parts of a row
+struct Parts { int32_t blocks, parts; };
+static Parts parts_of(int64_t n, int64_t a, int top) {
+    const int64_t all = cdiv(a, PART);
+    int64_t blocks = top > 0 ? 1 : n * all / WAVES_ENOUGH;
+    blocks = blocks < 1 ? 1 : (blocks > MOST ? MOST : blocks);
+    const int64_t parts = cdiv(all, blocks);
+    return {(int32_t)cdiv(all, parts), (int32_t)parts};
 }
 
-template <typename T, int VEC, int NV> __global__ __launch_bounds__(256) void k_logprob_part(LpPar p, int32_t parts, PartOut* part, uint64_t* keys) {
+// sums relative to `mx` brought to `to` >= mx
+__device__ __forceinline__ void rebase(Sums& q, float to) {
+    const float d = base_of(q.mx) - base_of(to), e = q.mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(d * LOG2E);
+    q.sd = e > 0.0f ? e * (q.sd + d * q.s) : 0.0f;             // (lowest values: d * s may be infinite, e is 0)
+    q.s *= e;
+    q.tx += q.ts == 0.0f ? 0.0f : d * q.ts;
+    q.mx = to;
+}
+
+template <typename T, int VEC, int NV, bool PLAIN> __global__ __launch_bounds__(256) void k_logprob_part(LpPar p, Parts s, PartOut* part, uint64_t* keys) {
     const int l = threadIdx.x & 63;
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t i = w / parts;
+    const int64_t i = w / s.parts;
     if (i >= p.n) return;
-    const int32_t first = (int32_t)(w - i * parts) * PART;
-    const int32_t end = p.a - first > PART ? first + PART : p.a;
+    const int64_t begin = (w - i * s.parts) * s.blocks * PART, stop = begin + (int64_t)s.blocks * PART < p.a ? begin + (int64_t)s.blocks * PART : p.a;
     const T* x = (const T*)p.x + i * p.ld;
-    Row<T, VEC, 64, NV> r;
-    r.load(x, p.mask ? p.mask + i * p.ld_mask : nullptr, first, end, l);
-    const Sums q = row_sums(r, p.target ? p.target + i * p.ld_target : nullptr, first, end, l);
-    if (l == 0) part[w].q = q;
-    if (p.top > 0) {
-        auto o = offer(r);
-        for (int k = 0; k < p.top; ++k) {
-            uint32_t j;
-            const float v = take_best(r, o, j);
-            if (l == 0) keys[w * p.top + k] = v > -INFINITY ? lp_key(v, j) : 0;
+    if constexpr (PLAIN) {                                     // no mask, no target, no alternatives
+        Span<T, VEC> v[NV], u[NV];
+        auto fetch = [&](Span<T, VEC> (&to)[NV], int64_t first) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int64_t own = first + VEC * (l + 64 * k);
+                to[k] = *(const Span<T, VEC>*)(x + (own < p.a - VEC ? own : p.a - VEC));
+            }
+        };
+        Sums q{-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f};
+        fetch(v, begin);
+        for (int64_t first = begin; first < stop; first += PART) {
+            if (first + PART < stop) fetch(u, first + PART);
+            float f[NV * VEC], mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < NV * VEC; ++k) f[k] = to_f(v[k / VEC].e[k % VEC]);
+            if (first + PART > p.a) {                          // the row's last block: entries outside it, and those that a span before it has, count as not there
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int64_t own = first + VEC * (l + 64 * k), at = own < p.a - VEC ? own : p.a - VEC;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) f[k * VEC + e] = own < p.a && at + e >= own ? f[k * VEC + e] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NV * VEC; ++k) mx = fmaxf(mx, f[k]);
+            if (mx > q.mx) rebase(q, mx);
+            const float base = base_of(q.mx);
+#pragma unroll
+            for (int k = 0; k < NV * VEC; ++k) {
+                const float d = f[k] - base, e = __builtin_amdgcn_exp2f(d * LOG2E);
+                q.s += e;
+                q.sd += e * fmaxf(d, -3.0e38f);
+            }
+#pragma unroll
+            for (int k = 0; k < NV; ++k) v[k] = u[k];
         }
+        const float mx = wave_max(q.mx);
+        rebase(q, mx);
+        q.s = wave_sum(q.s);
+        q.sd = wave_sum(q.sd);
+        if (l == 0) part[w].q = q;
+    } else {
+        Sums all{-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f};
+        for (int64_t first = begin; first < stop; first += PART) {
+            const int32_t end = (int32_t)(stop - first > PART ? first + PART : stop);
+            Row<T, VEC, 64, NV> r;
+            r.load(x, p.mask ? p.mask + i * p.ld_mask : nullptr, (int32_t)first, end, l);
+            Sums q = row_sums(r, p.target ? p.target + i * p.ld_target : nullptr, (int32_t)first, end, l);
+            if (s.blocks > 1) {
+                const float mx = fmaxf(all.mx, q.mx);
+                rebase(all, mx);
+                rebase(q, mx);
+                all.s += q.s; all.sd += q.sd; all.tx += q.tx; all.ts += q.ts;
+            } else all = q;
+            if (p.top > 0) {
+                __shared__ uint64_t list[4][LIST];
+                wave_top(r.x, [&](int k) { return (uint32_t)(r.at[k / VEC] + k % VEC); }, p.top, list[threadIdx.x >> 6], [&](int k, uint64_t key) { keys[w * p.top + k] = key; });
+            }
+        }
+        if (l == 0) part[w].q = all;
     }
 }
 
+constexpr int JOIN_LIST = 1024;
 template <typename T> __global__ __launch_bounds__(256) void k_logprob_join(LpPar p, int32_t parts, const PartOut* part, const uint64_t* keys) {
     const int l = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -219,35 +345,65 @@ template <typename T> __global__ __launch_bounds__(256) void k_logprob_join(LpPa
     bool given;
     const float xm = given_logit(p, x, p.mask ? p.mask + i * p.ld_mask : nullptr, i, given);
     part += i * parts;
-    float mx = -INFINITY;
-    for (int32_t k = l; k < parts; k += 64) mx = fmaxf(mx, part[k].q.mx);
-    mx = wave_max(mx);
-    Sums q{mx, 0.0f, 0.0f, 0.0f, 0.0f};
+    Sums q{-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f};
     for (int32_t k = l; k < parts; k += 64) {
-        const Sums t = part[k].q;
-        const float d = base_of(t.mx) - base_of(mx), e = t.s == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(d * LOG2E);   // (a part without entries: base 0)
-        q.s += t.s * e;
-        q.sd += e > 0.0f ? e * (t.sd + d * t.s) : 0.0f;      // (a part of lowest values: d * s may be infinite, e is 0)
-        q.tx += t.ts == 0.0f && t.tx == 0.0f ? 0.0f : t.tx + d * t.ts;
-        q.ts += t.ts;
+        Sums t = part[k].q;
+        const float mx = fmaxf(q.mx, t.mx);
+        rebase(q, mx);
+        rebase(t, mx);
+        q.s += t.s; q.sd += t.sd; q.tx += t.tx; q.ts += t.ts;
     }
+    const float mx = wave_max(q.mx);
+    rebase(q, mx);
     q.s = wave_sum(q.s); q.sd = wave_sum(q.sd); q.tx = wave_sum(q.tx); q.ts = wave_sum(q.ts);
     const Done f = finish(p, i, q, xm, given, l == 0);
-    if (p.top > 0) {
-        keys += i * parts * p.top;
-        const int64_t total = (int64_t)parts * p.top;
-        uint64_t last = ~0ull;
-        for (int k = 0; k < p.top; ++k) {
-            uint64_t best = 0;
-            if (last) for (int64_t c = l; c < total; c += 64) { const uint64_t v = keys[c]; if (v < last && v > best) best = v; }
-            best = wave_max_u64(best);
-            if (l == 0) {
-                const bool some = best && !f.bad;
-                if (p.top_move) p.top_move[i * p.top + k] = some ? (int32_t)~(uint32_t)best : -1;
-                if (p.top_logp) p.top_logp[i * p.top + k] = some ? lp_key_value(best) - base_of(mx) - f.ls : (f.bad ? NAN : -INFINITY);
-            }
-            last = best;
+    if (p.top == 0) return;
+    __shared__ uint64_t lists[4][JOIN_LIST];
+    uint64_t* list = lists[threadIdx.x >> 6];
+    keys += i * parts * p.top;
+    const int64_t total = (int64_t)parts * p.top;
+    auto emit = [&](int k, uint64_t key) {
+        const bool some = key != 0 && !f.bad;
+        if (p.top_move) p.top_move[i * p.top + k] = some ? (int32_t)~(uint32_t)key : -1;
+        if (p.top_logp) p.top_logp[i * p.top + k] = some ? lp_key_value(key) - base_of(mx) - f.ls : (f.bad ? NAN : -INFINITY);
+    };
+    // the bound as in wave_top, over the lanes' shares of the parts' keys; a share is short (total / 64), so that the list holds `top` of them up to 100 parts or so
+    uint64_t mine = 0;
+    for (int64_t c = l; c < total; c += 64) { const uint64_t v = keys[c]; mine = v > mine ? v : mine; }
+    const uint32_t hi = (uint32_t)(mine >> 32), lo = (uint32_t)mine;
+    int before = 0;
+#pragma unroll 8
+    for (int o = 0; o < 64; ++o) {
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, o) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, o);
+        before += other > mine ? 1 : 0;
+    }
+    const uint64_t at = __ballot(mine != 0 && before == p.top - 1);
+    uint64_t bound = 1;
+    if (at) {
+        const int o = __builtin_ctzll(at);
+        bound = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, o) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, o);
+    }
+    int count = 0;
+    for (int64_t c0 = 0; c0 < total; c0 += 64) {
+        const uint64_t key = c0 + l < total ? keys[c0 + l] : 0, in = __ballot(key >= bound);
+        if (in) {
+            const int to = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+            if (key >= bound && to < JOIN_LIST) list[to] = key;
+            count += __popcll(in);
         }
+    }
+    if (count <= JOIN_LIST) {
+        wave_list_ranks(list, count, p.top, emit);
+        return;
+    }
+    uint64_t last = ~0ull;                                     // (thousands of parts whose best ones fall to few lanes: one after the other)
+    for (int k = 0; k < p.top; ++k) {
+        uint64_t best = 0;
+        for (int64_t c = l; c < total; c += 64) { const uint64_t v = keys[c]; if (v < last && v > best) best = v; }
+        const uint32_t bh = lanes_reduce<64>((uint32_t)(best >> 32), [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        const uint32_t bl = lanes_reduce<64>((uint32_t)(best >> 32) == bh ? (uint32_t)best : 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        last = (uint64_t)bh << 32 | bl;
+        if (l == 0) emit(k, last);
     }
 }
 
@@ -260,7 +416,7 @@ __device__ __forceinline__ float grad_at(const GradRow& c, float v, float t, boo
     float g = c.gt * t - pr * (c.whole + c.gh * fmaxf(lp + c.h, -1.0e30f)) + (hot ? c.gm : 0.0f);     // (0 * -inf)
     return v == -INFINITY ? 0.0f : g;
 }
-template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) void k_logprob_grad(LpPar p, int32_t parts) {
+template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) void k_logprob_grad(LpPar p, int32_t parts) {   // parts: blocks of PART elements of a row
     const int l = threadIdx.x & (G - 1);
     const int64_t w = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, i = parts == 1 ? w : w / parts;
     if (i >= p.n) return;
@@ -352,7 +508,6 @@ template <typename T, typename F> static int by_length(int64_t a, F&& f) {
     return AGZ_LP(V, 64, PART / 64 / V);
 #undef AGZ_LP
 }
-static int64_t part_count(int64_t a) { return cdiv(a, PART); }
 static bool too_many(int64_t groups) { return cdiv(groups, 4) > 0x7fffffffll; }
 
 extern "C" {
@@ -360,7 +515,7 @@ extern "C" {
 int64_t agz_logprob_workspace(int64_t n, int64_t a, int32_t top) {
     if (n < 0 || a < 1 || a > (1ll << 30) || top < 0 || top > AGZ_TOP_MAX) return -1;
     if (a <= PART) return 0;
-    return n * part_count(a) * (int64_t)(sizeof(PartOut) + 8 * top);
+    return n * parts_of(n, a, top).parts * (int64_t)(sizeof(PartOut) + 8 * top);
 }
 
 int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
@@ -374,19 +529,20 @@ int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
     if (on.rc != AGZ_OK) return on.rc;
     if (q->n == 0) return AGZ_OK;
     const LpPar p = pack(q);
-    const int64_t parts = part_count(p.a);
-    if (too_many(p.n * parts)) return fail(AGZ_ERR_ARG, "agz_logprob_forward: too many rows");
+    const Parts w = parts_of(p.n, p.a, p.top);
+    if (too_many(p.n * w.parts)) return fail(AGZ_ERR_ARG, "agz_logprob_forward: too many rows");
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
-        if (parts == 1)
+        if (p.a <= PART)
             return by_length<T>(p.a, [&](auto vec, auto g, auto nv) {
                 return launch(k_logprob<T, vec(), g(), nv()>, dim3((uint32_t)cdiv(p.n, 256 / g())), dim3(256), 0, stream, p);
             });
         constexpr int V = 16 / sizeof(T);
         PartOut* part = (PartOut*)q->workspace;
-        uint64_t* keys = (uint64_t*)(part + p.n * parts);
-        if (int rc = launch(k_logprob_part<T, V, PART / 64 / V>, dim3((uint32_t)cdiv(p.n * parts, 4)), dim3(256), 0, stream, p, (int32_t)parts, part, keys)) return rc;
-        return launch(k_logprob_join<T>, dim3((uint32_t)cdiv(p.n, 4)), dim3(256), 0, stream, p, (int32_t)parts, part, keys);
+        uint64_t* keys = (uint64_t*)(part + p.n * w.parts);
+        const bool plain = !p.mask && !p.target && p.top == 0;
+        if (int rc = launch(plain ? k_logprob_part<T, V, PART / 64 / V, true> : k_logprob_part<T, V, PART / 64 / V, false>, dim3((uint32_t)cdiv(p.n * w.parts, 4)), dim3(256), 0, stream, p, w, part, keys)) return rc;
+        return launch(k_logprob_join<T>, dim3((uint32_t)cdiv(p.n, 4)), dim3(256), 0, stream, p, w.parts, part, keys);
     });
 }
 
@@ -403,7 +559,7 @@ int agz_logprob_backward(int device, void* stream, const agz_logprob_args* q, co
     if (q->n == 0) return AGZ_OK;
     LpPar p = pack(q);
     p.g_move = g_move; p.g_entropy = g_entropy; p.g_target = g_target; p.g_top = g_top; p.dx = dx; p.ldd = ldd;
-    const int64_t parts = part_count(p.a);
+    const int64_t parts = cdiv(p.a, PART);
     if (too_many(p.n * parts)) return fail(AGZ_ERR_ARG, "agz_logprob_backward: too many rows");
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
