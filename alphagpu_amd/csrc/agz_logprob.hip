@@ -206,19 +206,20 @@ template <typename T> __device__ __forceinline__ float given_logit(const LpPar& 
 }
 
 // A row per group of G lanes: rows of up to G NV VEC actions.  One pass: the row is read once and stays in registers.
-template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) void k_logprob(LpPar p) {
+// PLAIN: without mask, target and alternatives (fewer registers).
+template <typename T, int VEC, int G, int NV, bool PLAIN> __global__ __launch_bounds__(256) void k_logprob(LpPar p) {
     const int l = threadIdx.x & (G - 1);
     const int64_t i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (i >= p.n) return;
     const T* x = (const T*)p.x + i * p.ld;
-    const uint8_t* mask = p.mask ? p.mask + i * p.ld_mask : nullptr;
+    const uint8_t* mask = !PLAIN && p.mask ? p.mask + i * p.ld_mask : nullptr;
     bool given;
     const float xm = given_logit(p, x, mask, i, given);
     Row<T, VEC, G, NV> r;
     r.load(x, mask, 0, p.a, l);
-    const Sums q = row_sums(r, p.target ? p.target + i * p.ld_target : nullptr, 0, p.a, l);
+    const Sums q = row_sums(r, !PLAIN && p.target ? p.target + i * p.ld_target : nullptr, 0, p.a, l);
     const Done f = finish(p, i, q, xm, given, l == 0);
-    if (p.top > 0) {
+    if (!PLAIN && p.top > 0) {
         const float off = base_of(q.mx);
         auto put = [&](int k, bool some, float v, uint32_t j) {
             some = some && !f.bad;
@@ -410,13 +411,14 @@ template <typename T> __global__ __launch_bounds__(256) void k_logprob_join(LpPa
 // ---------------------------------------------------------------------------------------------------------------------------------------
 // the gradient: one pass that reads the row and writes the gradient; a row (or part) per group of G lanes as above
 // ---------------------------------------------------------------------------------------------------------------------------------------
-struct GradRow { float mx, ls, h, gh, gt, gm, whole; int32_t mv; };
+struct GradRow { float mx, ls, gh, gt, gm, whole; int32_t mv; };         // whole: the sum of the cotangents, and gh times the entropy
 __device__ __forceinline__ float grad_at(const GradRow& c, float v, float t, bool hot) {
     const float lp = v - c.mx - c.ls, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
-    float g = c.gt * t - pr * (c.whole + c.gh * fmaxf(lp + c.h, -1.0e30f)) + (hot ? c.gm : 0.0f);     // (0 * -inf)
+    float g = c.gt * t - pr * __builtin_fmaf(c.gh, fmaxf(lp, -1.0e30f), c.whole);      // (0 * -inf)
+    g = hot ? g + c.gm : g;
     return v == -INFINITY ? 0.0f : g;
 }
-template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) void k_logprob_grad(LpPar p, int32_t parts) {   // parts: blocks of PART elements of a row
+template <typename T, int VEC, int G, int NV, bool PLAIN> __global__ __launch_bounds__(256) void k_logprob_grad(LpPar p, int32_t parts) {   // parts: blocks of PART elements of a row
     const int l = threadIdx.x & (G - 1);
     const int64_t w = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, i = parts == 1 ? w : w / parts;
     if (i >= p.n) return;
@@ -424,8 +426,8 @@ template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) 
     const int32_t end = parts == 1 || p.a - first <= PART ? p.a : first + PART;
     const T* x = (const T*)p.x + i * p.ld;
     T* dx = (T*)p.dx + i * p.ldd;
-    const uint8_t* mask = p.mask ? p.mask + i * p.ld_mask : nullptr;
-    const float* target = p.target && p.g_target ? p.target + i * p.ld_target : nullptr;
+    const uint8_t* mask = !PLAIN && p.mask ? p.mask + i * p.ld_mask : nullptr;
+    const float* target = !PLAIN && p.g_target ? p.target + i * p.ld_target : nullptr;
     Row<T, VEC, G, NV> r;
     r.load(x, mask, first, end, l);
     Span<float, VEC> t[NV];
@@ -433,13 +435,14 @@ template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) 
 #pragma unroll
         for (int k = 0; k < NV; ++k) if (first + VEC * (l + G * k) < end) t[k] = *(const Span<float, VEC>*)(target + r.at[k]);
     const float4 st = *(const float4*)(p.stats + i * 4);
-    GradRow c{st.x, st.y, st.z, p.g_entropy ? p.g_entropy[i] : 0.0f, target ? p.g_target[i] : 0.0f, 0.0f, 0.0f, -1};
+    GradRow c{st.x, st.y, p.g_entropy ? p.g_entropy[i] : 0.0f, target ? p.g_target[i] : 0.0f, 0.0f, 0.0f, -1};
     if (p.moves && p.g_move) {
         const int64_t mv = p.moves[i];
         if (mv >= 0 && mv < p.a) { c.mv = (int32_t)mv; c.gm = p.g_move[i]; }
     }
     c.whole = c.gm + c.gt * st.w;
-    if (p.g_top) for (int k = 0; k < p.top; ++k) if (p.top_move[i * p.top + k] >= 0) c.whole += p.g_top[i * p.top + k];
+    if (!PLAIN && p.g_top) for (int k = 0; k < p.top; ++k) if (p.top_move[i * p.top + k] >= 0) c.whole += p.g_top[i * p.top + k];
+    c.whole += c.gh * st.z;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         if (first + VEC * (l + G * k) >= end) continue;
@@ -452,7 +455,7 @@ template <typename T, int VEC, int G, int NV> __global__ __launch_bounds__(256) 
 #pragma unroll
             for (int e = 0; e < VEC; ++e) if (r.at[k] + e >= own) dx[r.at[k] + e] = o.e[e];
     }
-    if (p.g_top) {                                             // the alternatives' own entries, written once more with their cotangents
+    if (!PLAIN && p.g_top) {                                   // the alternatives' own entries, written once more with their cotangents
         __threadfence_block();
         for (int k = l; k < p.top; k += G) {
             const int32_t j = p.top_move[i * p.top + k];
@@ -491,21 +494,30 @@ static LpPar pack(const agz_logprob_args* q) {
 
 using namespace agz::ops;
 
-// f(Row shape) for rows of `a` actions: lanes per row, spans per lane, elements per span; parts: rows longer than PART
-template <typename T, typename F> static int by_length(int64_t a, F&& f) {
-    constexpr int V = 16 / sizeof(T);
+// f(elements per span, lanes per row, spans per lane) for rows of `a` actions: 32 elements a lane at most, and as few lanes as hold the row, since the
+// reductions over them are what short rows spend their time on (200000 rows of 500 bf16: 106 us with 64 lanes a row, 37 us with 16).  A row above 128
+// actions of which more than four alternatives are wanted gets a whole wave: wave_top finds them in one go (40000 rows of 500, 20 alternatives: 64 us,
+// 180 us with 16 lanes that take one after the other; one alternative costs the few lanes less).
+template <typename T, typename F> static int by_length(int64_t a, int top, F&& f) {
+    constexpr int V = 16 / sizeof(T), F4 = 32 / V, F3 = F4 * 3 / 4, F2 = F4 / 2, F1 = F4 / 4;
     using std::integral_constant;
-    auto go = [&](auto vec, auto g, auto nv) { return f(vec, g, nv); };
-#define AGZ_LP(VEC, G, NV) go(integral_constant<int, VEC>{}, integral_constant<int, G>{}, integral_constant<int, NV>{})
+#define AGZ_LP(VEC, G, NV) f(integral_constant<int, VEC>{}, integral_constant<int, G>{}, integral_constant<int, NV>{})
     if (a < V) return AGZ_LP(1, 8, 1);
-    if (a <= 8 * V) return AGZ_LP(V, 8, 1);
-    if (a <= 16 * V) return AGZ_LP(V, 8, 2);
-    if (a <= 24 * V) return AGZ_LP(V, 8, 3);
-    if (a <= 32 * V) return AGZ_LP(V, 8, 4);
-    if (a <= 64 * V) return AGZ_LP(V, 64, 1);
-    if (a <= 128 * V) return AGZ_LP(V, 64, 2);
-    if (a <= 256 * V && 256 * V < PART) return AGZ_LP(V, 64, 4);
-    return AGZ_LP(V, 64, PART / 64 / V);
+    if (a <= 8 * V * F1) return AGZ_LP(V, 8, F1);
+    if (a <= 8 * V * F2) return AGZ_LP(V, 8, F2);
+    if (sizeof(T) == 4 && a <= 96) return AGZ_LP(V, 8, 3);       // (boards of 81 in 32 bits)
+    if (top > 4 && a > 128) {
+        if (a <= 64 * V * F1) return AGZ_LP(V, 64, F1);
+        if (a <= 64 * V * F2) return AGZ_LP(V, 64, F2);
+        return a <= 64 * V * F3 ? AGZ_LP(V, 64, F3) : AGZ_LP(V, 64, F4);
+    }
+    if (a <= 8 * V * F4) return AGZ_LP(V, 8, F4);
+    if (a <= 16 * V * F3) return AGZ_LP(V, 16, F3);
+    if (a <= 16 * V * F4) return AGZ_LP(V, 16, F4);
+    if (a <= 32 * V * F3) return AGZ_LP(V, 32, F3);
+    if (a <= 32 * V * F4) return AGZ_LP(V, 32, F4);
+    if (a <= 64 * V * F3) return AGZ_LP(V, 64, F3);
+    return AGZ_LP(V, 64, F4);
 #undef AGZ_LP
 }
 static bool too_many(int64_t groups) { return cdiv(groups, 4) > 0x7fffffffll; }
@@ -531,16 +543,16 @@ int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
     const LpPar p = pack(q);
     const Parts w = parts_of(p.n, p.a, p.top);
     if (too_many(p.n * w.parts)) return fail(AGZ_ERR_ARG, "agz_logprob_forward: too many rows");
+    const bool plain = !p.mask && !p.target && p.top == 0;
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
         if (p.a <= PART)
-            return by_length<T>(p.a, [&](auto vec, auto g, auto nv) {
-                return launch(k_logprob<T, vec(), g(), nv()>, dim3((uint32_t)cdiv(p.n, 256 / g())), dim3(256), 0, stream, p);
+            return by_length<T>(p.a, p.top, [&](auto vec, auto g, auto nv) {
+                return launch(plain ? k_logprob<T, vec(), g(), nv(), true> : k_logprob<T, vec(), g(), nv(), false>, dim3((uint32_t)cdiv(p.n, 256 / g())), dim3(256), 0, stream, p);
             });
         constexpr int V = 16 / sizeof(T);
         PartOut* part = (PartOut*)q->workspace;
         uint64_t* keys = (uint64_t*)(part + p.n * w.parts);
-        const bool plain = !p.mask && !p.target && p.top == 0;
         if (int rc = launch(plain ? k_logprob_part<T, V, PART / 64 / V, true> : k_logprob_part<T, V, PART / 64 / V, false>, dim3((uint32_t)cdiv(p.n * w.parts, 4)), dim3(256), 0, stream, p, w, part, keys)) return rc;
         return launch(k_logprob_join<T>, dim3((uint32_t)cdiv(p.n, 4)), dim3(256), 0, stream, p, w.parts, part, keys);
     });
@@ -561,10 +573,11 @@ int agz_logprob_backward(int device, void* stream, const agz_logprob_args* q, co
     p.g_move = g_move; p.g_entropy = g_entropy; p.g_target = g_target; p.g_top = g_top; p.dx = dx; p.ldd = ldd;
     const int64_t parts = cdiv(p.a, PART);
     if (too_many(p.n * parts)) return fail(AGZ_ERR_ARG, "agz_logprob_backward: too many rows");
+    const bool plain = !p.mask && !g_target && !g_top;
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
-        return by_length<T>(p.a, [&](auto vec, auto g, auto nv) {
-            return launch(k_logprob_grad<T, vec(), g(), nv()>, dim3((uint32_t)cdiv(p.n * parts, 256 / g())), dim3(256), 0, stream, p, (int32_t)parts);
+        return by_length<T>(p.a, 0, [&](auto vec, auto g, auto nv) {
+            return launch(plain ? k_logprob_grad<T, vec(), g(), nv(), true> : k_logprob_grad<T, vec(), g(), nv(), false>, dim3((uint32_t)cdiv(p.n * parts, 256 / g())), dim3(256), 0, stream, p, (int32_t)parts);
         });
     });
 }
