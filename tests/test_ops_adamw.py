@@ -250,6 +250,26 @@ def test_state_graph_and_another_stream(bits):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """A tensor of more than 2^32 elements: its last elements take the step that a short tensor's take (in 32 bits: no random numbers)."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GiB of free device memory")
+    n = (1 << 32) + 300
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    t = torch.randn(300, generator=torch.Generator().manual_seed(2)).bfloat16()
+    p[-300:], g[-300:] = t.cuda(), (t * 3).cuda()
+    for bits in (32, 8):
+        q = t.cuda().clone()
+        small, large = ops.AdamW([q], bits=bits, **HYPER), ops.AdamW([p], bits=bits, **HYPER)
+        small.step([(t * 3).cuda()])
+        large.step([g])
+        assert torch.equal(p[-300:], q) and not p[:5].any() and not p[(1 << 32) - 5:1 << 32].any()       # (the first step does not depend on what is held)
+        p[-300:] = t.cuda()
+        del large
+
+
+@pytest.mark.gpu
 def test_a_step_is_seen_by_autograd():
     p = torch.randn(10, device="cuda", requires_grad=True)
     y = (p * p).sum()

@@ -272,6 +272,51 @@ def test_another_stream_and_a_graph():
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^32 entries: the last rows of a quantised matrix, of its transpose and of a result."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GiB of free device memory")
+    m, k = 70000, 65536
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    tail = data(3, k, torch.bfloat16, 12)
+    x[-3:] = tail.cuda()
+    q = ops.quantize_fp8(x)
+    want = blocks(tail, 1)[0]
+    last = ops.Fp8Matrix.of(q.q[-3:], q.scale[-3:], 3, k)
+    assert torch.equal(last.dequantize().double().cpu(), want) and not q.q[-9:-3].view(torch.uint8).any()
+    t = ops.quantize_fp8(x, transposed=True)
+    got = ops.Fp8Matrix.of(t.q[-3:], t.scale[-3:], 3, m).dequantize()[:, -3:].double().cpu()
+    full = torch.zeros(3, 128)
+    full[:, m % 128 - 3:m % 128] = tail[:, -3:].t().float()       # the last block along the rows
+    assert torch.equal(got, blocks(full, 1)[0][:, m % 128 - 3:m % 128])
+    del x, q, t
+    r = torch.Generator().manual_seed(3)
+    a, b = torch.randint(-4, 5, (m, 40), generator=r).float(), torch.randint(-4, 5, (k, 40), generator=r).float()
+    out = ops.matmul_fp8(matrix(a), matrix(b))
+    assert torch.equal(out[-300:].cpu().double(), (a[-300:].double() @ b.double().t()))
+    assert torch.equal(out[:, -3:].cpu().double(), (a.double() @ b[-3:].double().t()))
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_are_refused():
+    x, w = torch.randn(4, 32, device="cuda", requires_grad=True), torch.randn(8, 32, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(ops.linear_fp8(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
+def test_changed_results_are_noticed():
+    """Behind a relu the result itself says where the gradient passes: changed in place, it is refused."""
+    x, w = torch.randn(4, 32, device="cuda", requires_grad=True), torch.randn(8, 32, device="cuda")
+    y = ops.linear_fp8(x, w, relu=True)
+    z = (y * 2).sum()
+    y.detach().add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_gpu():
     x, w = torch.randn(4, 64, device="cuda"), torch.randn(8, 64, device="cuda")
     for bad, match in ((lambda: ops.quantize_fp8(x.double()), "float32"), (lambda: ops.quantize_fp8(x, 64), "block_rows"), (lambda: ops.quantize_fp8(x.t()), "next to each other"),
@@ -301,5 +346,20 @@ def test_refusals_without_a_gpu():
     for change, match in (({"m": -1}, "-1"), ({"k": 1 << 31}, "x"), ({"ot": 7}, "dtype"), ({"bias": at, "bt": 9}, "dtype")):
         a = {**mm, **change}
         assert L.agz_fp8_matmul(0, None, *a.values()) == -1 and match in err(), (change, err())
+    lin = dict(m=2, n=2, k=4, x=at, ldx=4, w=at, ldw=4, bias=None, dtype=0, w_dtype=0, bias_dtype=0, relu=0)
+    big = (C.c_char * 65536)()
+    ws = (C.addressof(big) + 255) // 256 * 256
+    fwd = lambda ch, y=at, saved=ws, dx=1, dw=1, w=ws, n=60000: L.agz_linear_fp8_forward(0, None, C.byref(lib.LinearFp8Args(**{**lin, **ch})), y, saved, dx, dw, w, n)  # noqa: E731
+    bwd = lambda ch, dy=at, y=at, saved=ws, sdx=1, sdw=1, dx=at, dw=at, db=at, w=ws, n=60000: L.agz_linear_fp8_backward(  # noqa: E731
+        0, None, C.byref(lib.LinearFp8Args(**{**lin, **ch})), dy, y, saved, sdx, sdw, dx, dw, db, w, n)
+    for call, match in ((lambda: fwd({"m": -1}), "-1"), (lambda: fwd({"k": 1 << 24}), "x"), (lambda: fwd({"n": 65536 * 128}), "x"), (lambda: fwd({"dtype": 4}), "dtype"), (lambda: fwd({"w_dtype": -1}), "dtype"),
+                        (lambda: fwd({"bias": at, "bias_dtype": 3}), "dtype"), (lambda: fwd({"ldw": -1}), "stride"), (lambda: fwd({"x": at + 2}), "aligned"), (lambda: fwd({"x": None}), "required"),
+                        (lambda: fwd({}, y=None), "required"), (lambda: fwd({}, saved=None), "saved"), (lambda: fwd({}, n=10), "workspace"), (lambda: fwd({}, w=ws + 16), "workspace"),
+                        (lambda: bwd({}, sdx=0), "did not save"), (lambda: bwd({}, sdw=0), "did not save"), (lambda: bwd({}, saved=None), "saved"), (lambda: bwd({}, dy=None), "required"),
+                        (lambda: bwd({"relu": 1}, y=None), "required"), (lambda: bwd({}, n=0), "workspace"), (lambda: bwd({}, dx=at + 1), "aligned"), (lambda: bwd({"bias_dtype": 7}), "aligned")):
+        assert call() == -1 and match in err(), err()
+    assert L.agz_linear_fp8_forward(0, None, None, None, None, 0, 0, None, 0) == -1
+    assert L.agz_linear_fp8_workspace(-1, 1, 1) < 0 and L.agz_linear_fp8_saved(1, 1, -1, 1, 1) < 0 and L.agz_linear_fp8_backward_workspace(1, 1 << 31, 1, 1, 1, 1) < 0
+    assert L.agz_linear_fp8_saved(5, 6, 7, 0, 0) == 0
     assert L.agz_fp8_pitch(-1) == -1 and L.agz_fp8_pitch(129) == 256 and L.agz_fp8_scale_pitch(129) == 4 and L.agz_fp8_scale_pitch(513) == 8
     assert L.agz_fp8_matmul_workspace(-1, 1, 1) < 0 and L.agz_fp8_colsum_ws(-1, 1) < 0

@@ -318,6 +318,75 @@ def test_another_stream_and_a_graph():
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^32 logits: the last rows, forward and backward."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of free device memory")
+    n, a = 33000, 131072
+    x = torch.zeros(n, a, dtype=torch.bfloat16, device="cuda")
+    tail, mv, _, _, g = inputs(3, a, torch.bfloat16, 14, mask=None, target=False)
+    x[-3:] = tail.cuda()
+    x.requires_grad_()
+    moves = torch.full((n,), -1, device="cuda")
+    moves[-3:] = mv.cuda()
+    r = ops.log_probs(x, moves, top=3)
+    want, tol = plain(tail, mv, top=3, g=g)
+    for k in ("move", "entropy", "top", "top_move"):
+        close(getattr(r, k)[-3:], want[k], tol.get(k), k)
+    gm, ge = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    gm[-3:], ge[-3:] = g["move"].cuda(), g["entropy"].cuda()
+    dx, = torch.autograd.grad([r.move, r.entropy], [x], [gm, ge])
+    close(dx[-3:], want["dlogits"], tol["dlogits"])
+    assert not dx[-5:-3].any() and not dx[:2].any()
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_side_by_side():
+    """Two graphs captured one after the other have workspaces of their own: replayed in any order, on two streams at once, each gives what it gives alone."""
+    xs = [torch.randn(1, 90000, device="cuda") + k for k in range(2)]
+    graphs, outs = [], []
+    for x in xs:
+        ops.log_probs(x, top=8)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.log_probs(x, top=8))
+        graphs.append(g)
+    want = [ops.log_probs(x, top=8) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        for o, w in zip(outs, want):
+            assert torch.equal(o.entropy, w.entropy) and torch.equal(o.top_move, w.top_move) and torch.equal(o.top, w.top)
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_are_refused():
+    x = torch.randn(4, 9, device="cuda", requires_grad=True)
+    r = ops.log_probs(x, torch.zeros(4, dtype=torch.int64, device="cuda"))
+    dx, = torch.autograd.grad(r.move.sum(), x, create_graph=True)
+    want = torch.nn.functional.one_hot(torch.zeros(4, dtype=torch.int64), 9) - torch.softmax(x.detach().cpu(), 1)
+    assert (dx.detach().cpu() - want).abs().max() < 64 * E32
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
+def test_changed_logits_are_noticed():
+    x = torch.randn(4, 9, device="cuda", requires_grad=True)
+    y = x * 1.0
+    r = ops.log_probs(y, torch.zeros(4, dtype=torch.int64, device="cuda"))
+    y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.move.sum().backward()
+
+
+@pytest.mark.gpu
 def test_no_rows():
     x = torch.empty(0, 81, device="cuda", requires_grad=True)
     r = ops.log_probs(x, torch.empty(0, dtype=torch.int64, device="cuda"), top=2)
