@@ -327,11 +327,12 @@ __device__ __forceinline__ void store_row4(const MatPar& p, int64_t r, int64_t c
     else store4((f16*)p.out + at, v, valid);
 }
 
-template <int BM, int BN, int WM, int WN> struct Tile {
+template <int BM, int BN, int WM, int WN, bool WIDE> struct Tile {
     static constexpr int NT = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16, PA = BM * 8 / NT, PB = BN * 8 / NT;
+    static constexpr bool TURNS = WM * WN == 8 && !WIDE;
     static constexpr int STEP = (BM + BN) * FB, ROW = BN * 2 + 16, OUT = BM * ROW;         // bytes of a step, of a row and of all rows of a 16-bit result
     static constexpr int IN = 2 * STEP + 2 * (BM + BN) * 4, LDS = IN > OUT ? IN : OUT;     // two steps and two groups of scale words
-    static_assert((BM + BN) % NT == 0 && BM % 64 == 0 && PA * NT == BM * 8 && PB * NT == BN * 8, "whole pieces");
+    static_assert((BM + BN) % NT == 0 && BM % 64 == 0 && NT % 128 == 0 && PA * NT == BM * 8 && PB * NT == BN * 8, "whole pieces");
 };
 
 // a tile's results: through LDS (rows padded by 16 bytes, so that the 16 rows that a store covers meet different banks), then whole rows to memory;
@@ -374,7 +375,7 @@ __device__ __forceinline__ void store_tile(uint8_t* lds, const f32x4 (&acc)[TL::
 
 template <int BM, int BN, int WM, int WN, bool WIDE>
 __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
-    using TL = Tile<BM, BN, WM, WN>;
+    using TL = Tile<BM, BN, WM, WN, WIDE>;
     constexpr int NT = TL::NT, FM = TL::FM, FN = TL::FN, PA = TL::PA, PB = TL::PB;
     __shared__ __attribute__((aligned(16))) uint8_t lds[TL::LDS];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
@@ -396,84 +397,148 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
     const uint32_t lastm = (uint32_t)(p.m - 1 - m0 < BM ? p.m - 1 - m0 : BM - 1), lastn = (uint32_t)(p.n - 1 - n0 < BN ? p.n - 1 - n0 : BN - 1);
     const uint32_t pitch = (uint32_t)p.pitch, spitch = (uint32_t)p.spitch;
     const uint8_t *qa = p.qa + m0 * p.pitch, *qb = p.qb + n0 * p.pitch, *sa = p.sa + m0 * p.spitch, *sb = p.sb + n0 * p.spitch;
-    uint32_t src[PA + PB];
-#pragma unroll
-    for (int i = 0; i < PA + PB; ++i) {
-        const uint32_t piece = tid + (i < PA ? i : i - PA) * NT, r = piece >> 3, c = (piece & 7) ^ (r & 7), last = i < PA ? lastm : lastn;
-        src[i] = (r < last ? r : last) * pitch + c * 16;
-    }
+    // the pieces of a step that a thread fetches: FT threads (with turns, those of the first half of the waves), piece tid + i FT; further pieces are FT / 8 rows
+    // apart, a multiple of 8: the same place in the row.  The offsets are worked out anew each time (kept, they would cost a register each).
+    constexpr int FT = TL::TURNS ? NT / 2 : NT;
     auto fetch = [&](int k, int buf) {
+        uint32_t row0 = tid >> 3;
+        asm volatile("" : "+v"(row0));
+        const uint32_t piece0 = ((tid & 7) ^ (row0 & 7)) * 16;
+        const uint8_t *a = qa + (int64_t)k * FB, *b = qb + (int64_t)k * FB;
+        asm volatile("" : "+s"(a), "+s"(b));
+        const uint32_t to = (uint32_t)buf * TL::STEP + w * 1024;
 #pragma unroll
-        for (int i = 0; i < PA + PB; ++i)
-            __builtin_amdgcn_global_load_lds((gvoid*)((i < PA ? qa : qb) + (int64_t)k * FB + src[i]), (lvoid*)(lds + buf * TL::STEP + (i < PA ? i : i - PA) * NT * 16 + (i < PA ? 0 : BM * FB) + w * 1024), 16, 0, 0);
+        for (int i = 0; i < BM * 8 / FT; ++i) {
+            const uint32_t r = row0 + i * (FT / 8);
+            __builtin_amdgcn_global_load_lds((gvoid*)(a + (__umul24(r < lastm ? r : lastm, pitch) + piece0)), (lvoid*)(lds + to + i * FT * 16), 16, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < BN * 8 / FT; ++i) {
+            const uint32_t r = row0 + i * (FT / 8);
+            __builtin_amdgcn_global_load_lds((gvoid*)(b + (__umul24(r < lastn ? r : lastn, pitch) + piece0)), (lvoid*)(lds + BM * FB + to + i * FT * 16), 16, 0, 0);
+        }
     };
     // scale words of a group of four steps: one per row of the tile, BM + BN of them, into the buffer of the group's parity
     auto fetch_scales = [&](int word) {
 #pragma unroll
-        for (int i = 0; i < (BM + BN) / NT; ++i) {
-            const uint32_t x = tid + i * NT, r = x < BM ? x : x - BM, last = x < BM ? lastm : lastn;
-            __builtin_amdgcn_global_load_lds((gvoid*)((x < BM ? sa : sb) + (r < last ? r : last) * spitch + word * 4), (lvoid*)(lds + 2 * TL::STEP + (word & 1) * (BM + BN) * 4 + i * NT * 4 + w * 256), 4, 0, 0);
+        for (int i = 0; i < (BM + BN) / FT; ++i) {
+            uint32_t x = tid + i * FT;
+            asm volatile("" : "+v"(x));
+            const bool ofa = w * 64 + i * FT < BM;               // (a whole wave in one of them)
+            const uint32_t r = ofa ? x : x - BM, last = ofa ? lastm : lastn;
+            __builtin_amdgcn_global_load_lds((gvoid*)((ofa ? sa : sb) + word * 4 + (r < last ? r : last) * spitch), (lvoid*)(lds + 2 * TL::STEP + (word & 1) * (BM + BN) * 4 + i * FT * 4 + w * 256), 4, 0, 0);
         }
     };
     f32x4 acc[FM][FN] = {};
     uint32_t as[FM], bs[FN];
-    if (k0 < k1) {
+    if (k0 < k1 && w < FT / 64) {
         fetch_scales(k0 >> 2);
         fetch(k0, 0);
     }
     const int p0 = (g ^ (l16 & 7)) * 16, p1 = p0 ^ 64;
-    for (int k = k0; k < k1; ++k) {
-        const int buf = (k - k0) & 1;
-        __syncthreads();                                         // step k is in LDS, and everybody is done with the buffer of step k - 1
-        if (k + 1 < k1) {
-            if (((k + 1) & 3) == 0) fetch_scales((k + 1) >> 2);
-            fetch(k + 1, buf ^ 1);
-        }
-        const uint8_t* la = lds + buf * TL::STEP + (wm + l16) * FB;
-        const uint8_t* lb = lds + buf * TL::STEP + BM * FB + (wn + l16) * FB;
+    auto frag = [&](const uint8_t* base, int i) {
+        const i32x4 x = *(const i32x4*)(base + i * 16 * FB + p0), y = *(const i32x4*)(base + i * 16 * FB + p1);
+        return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    };
+    auto take_scales = [&](int k) {                              // the step's bytes at the bottom of the words
         if (k == k0 || (k & 3) == 0) {
             const uint32_t* words = (const uint32_t*)(lds + 2 * TL::STEP + ((k >> 2) & 1) * (BM + BN) * 4) + l16;
 #pragma unroll
             for (int i = 0; i < FM; ++i) as[i] = words[wm + i * 16] >> 8 * (k & 3);
 #pragma unroll
             for (int j = 0; j < FN; ++j) bs[j] = words[BM + wn + j * 16] >> 8 * (k & 3);
-        }
-        auto frag = [&](const uint8_t* base, int i) {
-            const i32x4 x = *(const i32x4*)(base + i * 16 * FB + p0), y = *(const i32x4*)(base + i * 16 * FB + p1);
-            return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        };
-        // (the scheduler would move a row's read behind the products of the row before it, into the same registers: the barriers keep it one row ahead)
-        if constexpr (WIDE) {
-            Wide bw[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) bw[j] = widen(frag(lb, j), bs[j] & 0xFF);
-            i32x8 av = frag(la, 0);
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const Wide aw = widen(av, as[i] & 0xFF);
-                if (i + 1 < FM) av = frag(la, i + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma_wide(bw[j], aw, acc[i][j]);
-            }
         } else {
-            i32x8 bv[FN], av[2];
-            av[0] = frag(la, 0);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) as[i] >>= 8;
+#pragma unroll
+            for (int j = 0; j < FN; ++j) bs[j] >>= 8;
+        }
+    };
+    auto fetch_next = [&](int k) {
+        if (k + 1 < k1) {
+            if (((k + 1) & 3) == 0) fetch_scales((k + 1) >> 2);
+            fetch(k + 1, (k + 1 - k0) & 1);
+        }
+    };
+    if constexpr (TL::TURNS) {
+        // The two waves of a SIMD (w and w + 4) take turns: while one reads its operands of a step from LDS, all of them, into registers, the other multiplies.
+        // Phase 2 k: the first four waves read step k, the others multiply step k - 1; phase 2 k + 1: the other way round; a barrier between phases.  The first
+        // four, whose registers are free then, fetch step k + 1 from phase 2 k on (its buffer was last read in phase 2 k - 1) and has to be there at the end of phase 2 k + 1.
+        i32x8 av[FM], bv[FN];
+        auto read = [&](int k) {
+            const uint8_t* la = lds + ((k - k0) & 1) * TL::STEP + (wm + l16) * FB;
+            const uint8_t* lb = lds + ((k - k0) & 1) * TL::STEP + BM * FB + (wn + l16) * FB;
 #pragma unroll
             for (int j = 0; j < FN; ++j) bv[j] = frag(lb, j);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                if (i + 1 < FM) av[(i + 1) & 1] = frag(la, i + 1);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < FM; ++i) av[i] = frag(la, i);
+            take_scales(k);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto multiply = [&]() {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma<0>(bv[j], av[i & 1], acc[i][j], (int)bs[j], (int)as[i]);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma<0>(bv[j], av[i], acc[i][j], (int)bs[j], (int)as[i]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (w < WM * WN / 2) {
+            for (int k = k0; k < k1; ++k) {
+                __syncthreads();
+                fetch_next(k);
+                read(k);
+                __builtin_amdgcn_s_barrier();
+                multiply();
+            }
+        } else {
+            for (int k = k0; k < k1; ++k) {
+                __syncthreads();
+                if (k > k0) multiply();
+                __builtin_amdgcn_s_barrier();
+                read(k);
+            }
+            if (k0 < k1) multiply();
+        }
+    } else {
+        for (int k = k0; k < k1; ++k) {
+            __syncthreads();                                     // step k is in LDS, and everybody is done with the buffer of step k - 1
+            fetch_next(k);
+            take_scales(k);
+            const uint8_t* la = lds + ((k - k0) & 1) * TL::STEP + (wm + l16) * FB;
+            const uint8_t* lb = lds + ((k - k0) & 1) * TL::STEP + BM * FB + (wn + l16) * FB;
+            // (the scheduler would move a row's read behind the products of the row before it, into the same registers: the barriers keep it one row ahead)
+            if constexpr (WIDE) {
+                Wide bw[FN];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) bw[j] = widen(frag(lb, j), bs[j] & 0xFF);
+                i32x8 av = frag(la, 0);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    const Wide aw = widen(av, as[i] & 0xFF);
+                    if (i + 1 < FM) av = frag(la, i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = mma_wide(bw[j], aw, acc[i][j]);
+                }
+            } else {
+                i32x8 bv[FN], av[2];
+                av[0] = frag(la, 0);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) bv[j] = frag(lb, j);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    if (i + 1 < FM) av[(i + 1) & 1] = frag(la, i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = mma<0>(bv[j], av[i & 1], acc[i][j], (int)bs[j], (int)as[i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < FM; ++i) as[i] >>= 8;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) bs[j] >>= 8;
     }
     if (p.slices > 1) {
         store_tile<float, TL, BM, BN, WM, WN>(lds, acc, p.part + (int64_t)slice * p.m * p.n, p.n, p.m, p.n, m0, n0);
@@ -521,34 +586,93 @@ __global__ __launch_bounds__(256) void k_matmul_join(MatPar p) {
     store_row4(p, r, c, v);
 }
 
+// 32 values of a block of 128 that four neighbouring lanes share, held in 8 bits: what k_quantize would have written, and the byte of the scale.  n: how many
+// of the 32 there are (the others count as 0).
+template <typename T> __device__ __forceinline__ int quantize32(const T* x, int n, uint8_t* to) {
+    float v[32];
+    if (n >= 32) {
+        Span<T, 8> s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] = *(const Span<T, 8>*)(x + 8 * k);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = to_f(s[k / 8].e[k % 8]);
+    } else
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = k < n ? to_f(x[k]) : 0.0f;
+    float m = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) m = fmaxf(m, fabsf(v[k]));
+    if (__any(m == INFINITY)) {
+        m = 0.0f;
+        for (int k = 0; k < 32; ++k) m = fmaxf(m, fabsf(v[k]) < INFINITY ? fabsf(v[k]) : 0.0f);
+    }
+    const int byte = scale_byte(lanes_max<4>(m));
+    const float inv = inv_scale_of(byte);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *(uint2*)(to + 8 * k) = enc8(v + 8 * k, inv);
+    return byte;
+}
+
 // Few rows (up to 16): the weights are read once, straight into the matrix unit's registers, and that is all the time there is.  A wave takes 16
-// columns and every fourth (FEW_WAVES) group of steps; the waves of a workgroup add up through LDS.
-constexpr int FEW_WAVES = 4, FEW_DEEP = 4;
-template <bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) void k_matmul_fp8_few(MatPar p) {
+// columns and every FEW_WAVES-th group of four steps; the waves of a workgroup add up through LDS.  T: uint8_t for a matrix in 8 bits, or the type of
+// x, which every workgroup then holds in 8 bits itself, in LDS (a launch less; as long as its rows are short, x comes from the caches:
+// one row of 8192 and 8192 columns 19.7 us in two launches, 15.5 us in one).
+constexpr int FEW_WAVES = 4, FEW_DEEP = 4, FEW_LDS = 32768;
+template <typename T, bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) void k_matmul_fp8_few(MatPar p, const T* x, int64_t ldx) {
     __shared__ f32x4 sum[FEW_WAVES][64];
+    constexpr bool READY = std::is_same<T, uint8_t>::value;
+    __shared__ __attribute__((aligned(16))) uint8_t held[READY ? 16 : FEW_LDS];
+    __shared__ uint8_t held_scale[READY ? 1 : FEW_LDS / FB];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16;
-    int64_t r = l16 < p.m ? l16 : p.m - 1, c = n0 + l16 < p.n ? n0 + l16 : p.n - 1;
-    const uint8_t *a = p.qa + r * p.pitch + g * 32, *b = p.qb + c * p.pitch + g * 32;
-    const int *sa = (const int*)(p.sa + r * p.spitch), *sb = (const int*)(p.sb + c * p.spitch);
+    const int r = l16 < p.m ? l16 : (int)p.m - 1;
+    const int64_t c = n0 + l16 < p.n ? n0 + l16 : p.n - 1;
+    const uint8_t *a = READY ? p.qa + r * p.pitch + g * 32 : held + r * p.pitch + g * 32, *b = p.qb + c * p.pitch + g * 32;
+    const int *sa = READY ? (const int*)(p.sa + r * p.spitch) : nullptr, *sb = (const int*)(p.sb + c * p.spitch);
     const int kb = (int)((p.k + FB - 1) / FB), whole = kb / FEW_DEEP;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto one = [&](i32x8 av, i32x8 bv, int as, int bs) {
-        if constexpr (WIDE) acc = mma_wide(widen(bv, bs & 0xFF), widen(av, as & 0xFF), acc);
-        else acc = mma<0>(bv, av, acc, bs, as);
-    };
-    for (int q = w; q < whole; q += FEW_WAVES) {                 // FEW_DEEP = 4 steps: one word of scales
-        i32x8 av[FEW_DEEP], bv[FEW_DEEP];
+    const uint8_t* sl = held_scale + r * kb;
+    i32x8 bv[FEW_DEEP];
+    int bs = 0;
+    auto weights = [&](int q) {
 #pragma unroll
         for (int k = 0; k < FEW_DEEP; ++k) bv[k] = load32(b + (int64_t)(q * FEW_DEEP + k) * FB);
+        bs = sb[q];
+    };
+    if (w < whole) weights(w);
+    if constexpr (!READY) {
+        for (int t = threadIdx.x; t < (int)p.m * kb * 4; t += FEW_WAVES * 64) {      // (m pitch <= FEW_LDS)
+            const int row = t / (kb * 4), at = t - row * kb * 4;
+            const int64_t left = p.k - at * 32;
+            const int byte = quantize32(x + row * ldx + at * 32, (int)(left < 0 ? 0 : (left < 32 ? left : 32)), held + row * p.pitch + at * 32);
+            if ((at & 3) == 0) held_scale[row * kb + (at >> 2)] = (uint8_t)byte;
+        }
+        __syncthreads();
+    }
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto one = [&](i32x8 av, i32x8 bw, int as, int bws) {
+        if constexpr (WIDE) acc = mma_wide(widen(bw, bws & 0xFF), widen(av, as & 0xFF), acc);
+        else acc = mma<0>(bw, av, acc, bws, as);
+    };
+    for (int q = w; q < whole; q += FEW_WAVES) {                 // FEW_DEEP = 4 steps: one word of scales
+        if (q > w) weights(q);
+        i32x8 av[FEW_DEEP];
+        int as[FEW_DEEP];
 #pragma unroll
         for (int k = 0; k < FEW_DEEP; ++k) av[k] = load32(a + (int64_t)(q * FEW_DEEP + k) * FB);
-        const int as = sa[q], bs = sb[q];
+        if constexpr (READY) {
+            const int word = sa[q];
 #pragma unroll
-        for (int k = 0; k < FEW_DEEP; ++k) one(av[k], bv[k], as >> 8 * k, bs >> 8 * k);
+            for (int k = 0; k < FEW_DEEP; ++k) as[k] = word >> 8 * k;
+        } else {
+#pragma unroll
+            for (int k = 0; k < FEW_DEEP; ++k) as[k] = sl[q * FEW_DEEP + k];
+        }
+#pragma unroll
+        for (int k = 0; k < FEW_DEEP; ++k) one(av[k], bv[k], as[k], bs >> 8 * k);
     }
     if (w == (whole & (FEW_WAVES - 1)))
-        for (int k = whole * FEW_DEEP; k < kb; ++k) one(load32(a + (int64_t)k * FB), load32(b + (int64_t)k * FB), sa[k >> 2] >> 8 * (k & 3), sb[k >> 2] >> 8 * (k & 3));
+        for (int k = whole * FEW_DEEP; k < kb; ++k)
+            one(load32(a + (int64_t)k * FB), load32(b + (int64_t)k * FB), READY ? sa[k >> 2] >> 8 * (k & 3) : (int)sl[k], sb[k >> 2] >> 8 * (k & 3));
     sum[w][lane] = acc;
     __syncthreads();
     if (w == 0 && l16 < p.m && n0 + g * 4 < p.n) {
@@ -616,7 +740,7 @@ int product(void* stream, int64_t m, int64_t n, int64_t k, Mat8 a, Mat8 b, const
     const Plan w = plan(m, n, k);
     const MatPar p{a.q, a.s, b.q, b.s, m, n, k, up(k, FB), up(cdiv(k, FB), 4), bias, bias_dtype, relu, out, out_dtype, ldo, w.slices, (float*)ws};
     const bool wide = out_dtype == AGZ_F32 || relu;
-    if (w.few) return launch(wide ? k_matmul_fp8_few<true> : k_matmul_fp8_few<false>, dim3((uint32_t)cdiv(n, 16)), dim3(FEW_WAVES * 64), 0, stream, p);
+    if (w.few) return launch(wide ? k_matmul_fp8_few<uint8_t, true> : k_matmul_fp8_few<uint8_t, false>, dim3((uint32_t)cdiv(n, 16)), dim3(FEW_WAVES * 64), 0, stream, p, (const uint8_t*)nullptr, (int64_t)0);
     const int64_t groups = cdiv(m, w.tile) * cdiv(n, w.tile) * w.slices;
     if (groups > 0x7fffffffll) return fail(AGZ_ERR_ARG, "a product of more than 2^31 tiles");
     const int rc = w.tile == 256 ? launch(wide ? k_matmul_fp8<256, 256, 2, 4, true> : k_matmul_fp8<256, 256, 2, 4, false>, dim3((uint32_t)groups), dim3(512), 0, stream, p)
@@ -634,6 +758,16 @@ struct Carve {
 bool good_sizes(int64_t m, int64_t n, int64_t k) { return m >= 0 && n >= 0 && k >= 0 && !too_large(m) && !too_large(n) && !too_deep(k) && cdiv(m, FB) <= 65535 && cdiv(n, FB) <= 65535; }
 struct Forward { Mat8 a, b; void* ws; };
 Forward forward_ws(Carve& c, int64_t m, int64_t n, int64_t k) { return {c.matrix(m, k), c.matrix(n, k), c.take(agz_fp8_matmul_workspace(m, n, k))}; }
+// a layer on weights in 8 bits: x in 8 bits first, or on the way where its rows are few
+struct Apply { Mat8 a; void* ws; };
+bool at_once(int64_t m, int64_t n, int64_t k) { return plan(m, n, k).few && m * up(k, FB) <= FEW_LDS; }
+Apply apply_ws(Carve& c, int64_t m, int64_t n, int64_t k) {
+    if (at_once(m, n, k)) return {};
+    Apply w;
+    w.a = c.matrix(m, k);
+    w.ws = c.take(agz_fp8_matmul_workspace(m, n, k));
+    return w;
+}
 struct Saved { Mat8 at, bt; };
 Saved saved_of(Carve& c, int64_t m, int64_t n, int64_t k, bool need_dx, bool need_dw) {
     Saved s{};
@@ -712,6 +846,12 @@ int64_t agz_linear_fp8_workspace(int64_t m, int64_t n, int64_t k) {
     forward_ws(c, m, n, k);
     return c.at;
 }
+int64_t agz_linear_fp8_apply_workspace(int64_t m, int64_t n, int64_t k) {
+    if (!good_sizes(m, n, k)) return -1;
+    Carve c{nullptr};
+    apply_ws(c, m, n, k);
+    return c.at;
+}
 int64_t agz_linear_fp8_saved(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw) {
     if (!good_sizes(m, n, k)) return -1;
     Carve c{nullptr};
@@ -739,6 +879,29 @@ int agz_linear_fp8_forward(int device, void* stream, const agz_linear_fp8_args* 
     if (int rc = quantize(stream, q->x, q->dtype, q->m, q->k, q->ldx, nullptr, 1, f.a, s.at, nullptr, 0, nullptr)) return rc;
     if (int rc = quantize(stream, q->w, q->w_dtype, q->n, q->k, q->ldw, nullptr, FB, f.b, s.bt, nullptr, 0, nullptr)) return rc;
     return product(stream, q->m, q->n, q->k, f.a, f.b, q->bias, q->bias_dtype, q->relu, y, q->dtype, q->n, f.ws);
+}
+
+int agz_linear_fp8_apply(int device, void* stream, const agz_linear_fp8_args* q, const void* qw, const void* sw, void* y, void* ws, int64_t ws_bytes) {
+    if (int rc = check_linear("agz_linear_fp8_apply", q)) return rc;
+    const int64_t m = q->m, n = q->n, k = q->k, need = agz_linear_fp8_apply_workspace(m, n, k);
+    if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 256))) return fail(AGZ_ERR_ARG, "agz_linear_fp8_apply: a workspace of %lld bytes, 256-byte aligned", (long long)need);
+    if ((m > 0 && n > 0 && (!y || !aligned(y, esize(q->dtype)))) || (m > 0 && k > 0 && !q->x) || (n > 0 && k > 0 && (!qw || !sw || !aligned(qw, 16) || !aligned(sw, 4))))
+        return fail(AGZ_ERR_ARG, "agz_linear_fp8_apply: x, y and the weights (values aligned to 16 bytes, scales to 4) are required");
+    OnDevice on(device);
+    if (on.rc != AGZ_OK) return on.rc;
+    if (m == 0 || n == 0) return AGZ_OK;
+    Carve c{(uint8_t*)ws};
+    const Apply w = apply_ws(c, m, n, k);
+    const Mat8 b{(uint8_t*)qw, (uint8_t*)sw};
+    if (!at_once(m, n, k)) {
+        if (int rc = quantize(stream, q->x, q->dtype, m, k, q->ldx, nullptr, 1, w.a, {}, nullptr, 0, nullptr)) return rc;
+        return product(stream, m, n, k, w.a, b, q->bias, q->bias_dtype, q->relu, y, q->dtype, n, w.ws);
+    }
+    const MatPar p{nullptr, nullptr, b.q, b.s, m, n, k, up(k, FB), up(cdiv(k, FB), 4), q->bias, q->bias_dtype, q->relu, y, q->dtype, n, 1, nullptr};
+    return by_dtype(q->dtype, [&](auto t) {
+        using T = decltype(t);
+        return launch(q->relu || q->dtype == AGZ_F32 ? k_matmul_fp8_few<T, true> : k_matmul_fp8_few<T, false>, dim3((uint32_t)cdiv(n, 16)), dim3(FEW_WAVES * 64), 0, stream, p, (const T*)q->x, q->ldx);
+    });
 }
 
 int agz_linear_fp8_backward(int device, void* stream, const agz_linear_fp8_args* q, const void* dy, const void* y, const void* saved, int saved_dx, int saved_dw, void* dx, void* dw, void* db, void* ws, int64_t ws_bytes) {

@@ -368,9 +368,14 @@ template <typename T> __global__ __launch_bounds__(256) void k_logprob_join(LpPa
         if (p.top_move) p.top_move[i * p.top + k] = some ? (int32_t)~(uint32_t)key : -1;
         if (p.top_logp) p.top_logp[i * p.top + k] = some ? lp_key_value(key) - base_of(mx) - f.ls : (f.bad ? NAN : -INFINITY);
     };
-    // the bound as in wave_top, over the lanes' shares of the parts' keys; a share is short (total / 64), so that the list holds `top` of them up to 100 parts or so
-    uint64_t mine = 0;
-    for (int64_t c = l; c < total; c += 64) { const uint64_t v = keys[c]; mine = v > mine ? v : mine; }
+    // the bound as in wave_top, over the lanes' shares of the parts' keys; up to SHARE keys a lane (SHARE * 64 in all) stay in its registers
+    constexpr int SHARE = 32;
+    uint64_t held[SHARE], mine = 0;
+#pragma unroll
+    for (int k = 0; k < SHARE; ++k) held[k] = l + 64 * k < total ? keys[l + 64 * k] : 0;
+#pragma unroll
+    for (int k = 0; k < SHARE; ++k) mine = held[k] > mine ? held[k] : mine;
+    for (int64_t c = l + 64 * SHARE; c < total; c += 64) { const uint64_t v = keys[c]; mine = v > mine ? v : mine; }
     const uint32_t hi = (uint32_t)(mine >> 32), lo = (uint32_t)mine;
     int before = 0;
 #pragma unroll 8
@@ -385,14 +390,17 @@ template <typename T> __global__ __launch_bounds__(256) void k_logprob_join(LpPa
         bound = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, o) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, o);
     }
     int count = 0;
-    for (int64_t c0 = 0; c0 < total; c0 += 64) {
-        const uint64_t key = c0 + l < total ? keys[c0 + l] : 0, in = __ballot(key >= bound);
+    auto note = [&](uint64_t key) {
+        const uint64_t in = __ballot(key >= bound);
         if (in) {
             const int to = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
             if (key >= bound && to < JOIN_LIST) list[to] = key;
             count += __popcll(in);
         }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < SHARE; ++k) if (64 * k < total) note(held[k]);
+    for (int64_t c0 = 64 * SHARE; c0 < total; c0 += 64) note(c0 + l < total ? keys[c0 + l] : 0);
     if (count <= JOIN_LIST) {
         wave_list_ranks(list, count, p.top, emit);
         return;
@@ -504,8 +512,8 @@ template <typename T, typename F> static int by_length(int64_t a, int top, F&& f
 #define AGZ_LP(VEC, G, NV) f(integral_constant<int, VEC>{}, integral_constant<int, G>{}, integral_constant<int, NV>{})
     if (a < V) return AGZ_LP(1, 8, 1);
     if (a <= 8 * V * F1) return AGZ_LP(V, 8, F1);
+    if (sizeof(T) == 4 && a > 64 && a <= 96) return AGZ_LP(V, 8, 3);      // (boards of 81 in 32 bits)
     if (a <= 8 * V * F2) return AGZ_LP(V, 8, F2);
-    if (sizeof(T) == 4 && a <= 96) return AGZ_LP(V, 8, 3);       // (boards of 81 in 32 bits)
     if (top > 4 && a > 128) {
         if (a <= 64 * V * F1) return AGZ_LP(V, 64, F1);
         if (a <= 64 * V * F2) return AGZ_LP(V, 64, F2);

@@ -144,11 +144,13 @@ def load_library():
         L.agz_linear_fp8_workspace.argtypes = [i64] * 3
         L.agz_linear_fp8_saved.argtypes = [i64] * 3 + [i32] * 2
         L.agz_linear_fp8_backward_workspace.argtypes = [i64] * 3 + [i32] * 3
+        L.agz_linear_fp8_apply_workspace.argtypes = [i64] * 3
+        L.agz_linear_fp8_apply.argtypes = [i32, vp, vp, vp, vp, vp, vp, i64]
         L.agz_linear_fp8_forward.argtypes = [i32, vp, vp, vp, vp, i32, i32, vp, i64]
         L.agz_linear_fp8_backward.argtypes = [i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64]
         L.agz_adamw_state_elements.argtypes = [i32, vp]
         L.agz_adamw_step.argtypes = [i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp]
-        for n in ("logprob_workspace", "fp8_pitch", "fp8_scale_pitch", "fp8_colsum_ws", "fp8_matmul_workspace", "linear_fp8_workspace", "linear_fp8_saved", "linear_fp8_backward_workspace", "adamw_state_elements"):
+        for n in ("logprob_workspace", "fp8_pitch", "fp8_scale_pitch", "fp8_colsum_ws", "fp8_matmul_workspace", "linear_fp8_workspace", "linear_fp8_saved", "linear_fp8_apply_workspace", "linear_fp8_backward_workspace", "adamw_state_elements"):
             getattr(L, "agz_" + n).restype = i64
     _LIB = L
     return L

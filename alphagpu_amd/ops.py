@@ -295,6 +295,21 @@ def _linear_forward(x, w, bias, relu, need_x, need_w):
     return y, saved, q
 
 
+def _linear_apply(x, w, bias, relu):
+    L = _lib.load_library()
+    (m, k), n, dev, i = x.shape, w.rows, x.device, x.get_device()
+    y = torch.empty(m, n, dtype=x.dtype, device=dev)
+    need = L.agz_linear_fp8_apply_workspace(m, n, k)
+    if need < 0:
+        raise ValueError(f"linear_fp8: {m} x {n} x {k} is too large")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    q = _LIN.pack(m, n, k, x.data_ptr(), _rows(x, "x"), 0, 0, 0 if bias is None else bias.data_ptr(), _CODE[x.dtype], 0, 0 if bias is None else _CODE[bias.dtype], relu)
+    rc = L.agz_linear_fp8_apply(i, _raw_stream(i), q, w.q.data_ptr(), w.scale.data_ptr(), y.data_ptr(), _ptr(ws), need)
+    if rc:
+        _lib_call(rc, L)
+    return y
+
+
 def _linear_backward(ctx, dy):
     saved, y = ctx.saved_tensors
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -355,8 +370,7 @@ def linear_fp8(x, w, bias=None, relu=False):
         _need(not ready, "w: gradients need the weights themselves, not Fp8Weight")
         y = _LinearFp8.apply(two, w, bias, bool(relu))
     elif ready:
-        a, _, _ = _quantize(two, 1, True, False)
-        y = _product(a, w.matrix, bias, relu, x.dtype)
+        y = _linear_apply(two, w.matrix, bias, bool(relu))
     else:
         y = _linear_forward(two, w, bias, bool(relu), False, False)[0]
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)

@@ -333,6 +333,10 @@ typedef struct {
 } agz_linear_fp8_args;
 int64_t agz_linear_fp8_workspace(int64_t m, int64_t n, int64_t k);
 int64_t agz_linear_fp8_saved(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw);
+/* the same y on weights that are held in 8 bits already (qw [n][pitch], sw as of agz_fp8_quantize with block_rows 128): args->w, ldw, w_dtype are not read;
+ * up to 16 rows of together up to 32768 entries in one launch, x held in 8 bits on the way */
+int64_t agz_linear_fp8_apply_workspace(int64_t m, int64_t n, int64_t k);
+int  agz_linear_fp8_apply(int device, void *stream, const agz_linear_fp8_args *args, const void *qw, const void *sw, void *y, void *workspace, int64_t workspace_bytes);
 int64_t agz_linear_fp8_backward_workspace(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, int need_db);
 int  agz_linear_fp8_forward(int device, void *stream, const agz_linear_fp8_args *args, void *y, void *saved, int need_dx, int need_dw, void *workspace, int64_t workspace_bytes);
 int  agz_linear_fp8_backward(int device, void *stream, const agz_linear_fp8_args *args, const void *dy, const void *y, const void *saved, int saved_dx, int saved_dw,

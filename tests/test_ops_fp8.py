@@ -242,6 +242,25 @@ def test_linear_forms():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_few_rows_on_ready_weights(dtype):
+    """Up to 16 rows are held in 8 bits on the way: the same bits as in two steps, with rows of a wider tensor, NaN, infinities and zeros among them."""
+    for m, n, k in ((1, 300, 1024), (2, 17, 5), (5, 33, 700), (16, 128, 130), (16, 64, 2049), (7, 1000, 128), (17, 40, 300), (3, 16, 31)):
+        x = data(m, k + 3, dtype, 20)[:, 1:k + 1]
+        if m > 4 and k > 600:
+            x = x.clone()
+            x[2, 600], x[3, 0], x[4, :128] = math.nan, -math.inf, 0.0
+        w, b = data(n, k, torch.float32, 21), torch.randn(n, generator=torch.Generator().manual_seed(1)).cuda()
+        ready = ops.Fp8Weight(w.cuda())
+        wide = torch.zeros(m, k + 3, dtype=dtype, device="cuda")
+        wide[:, 1:k + 1] = x.cuda()
+        for relu in (False, True):
+            got = ops.linear_fp8(wide[:, 1:k + 1], ready, b, relu=relu)
+            want = ops.matmul_fp8(ops.quantize_fp8(x.cuda()), ready.matrix, b, relu=relu, dtype=dtype)
+            assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(7), want.nan_to_num(7)), (m, n, k, relu)
+
+
+@pytest.mark.gpu
 def test_another_stream_and_a_graph():
     def step(x, w, b, g):
         leaves = [t.detach().requires_grad_() for t in (x, w, b)]
@@ -358,6 +377,11 @@ def test_refusals_without_a_gpu():
                         (lambda: bwd({}, sdx=0), "did not save"), (lambda: bwd({}, sdw=0), "did not save"), (lambda: bwd({}, saved=None), "saved"), (lambda: bwd({}, dy=None), "required"),
                         (lambda: bwd({"relu": 1}, y=None), "required"), (lambda: bwd({}, n=0), "workspace"), (lambda: bwd({}, dx=at + 1), "aligned"), (lambda: bwd({"bias_dtype": 7}), "aligned")):
         assert call() == -1 and match in err(), err()
+    app = lambda ch, qw=at, sw=at, y=at, w=ws, n=60000: L.agz_linear_fp8_apply(0, None, C.byref(lib.LinearFp8Args(**{**lin, **ch})), qw, sw, y, w, n)  # noqa: E731
+    for call, match in ((lambda: app({"m": -1}), "-1"), (lambda: app({"dtype": 3}), "dtype"), (lambda: app({"x": None}), "required"), (lambda: app({}, qw=None), "required"), (lambda: app({}, sw=at + 1), "required"),
+                        (lambda: app({}, y=at + 1), "required"), (lambda: app({"m": 20}, n=3), "workspace"), (lambda: app({"m": 20}, w=None), "workspace")):
+        assert call() == -1 and match in err(), err()
+    assert L.agz_linear_fp8_apply_workspace(1, -1, 1) < 0 and L.agz_linear_fp8_apply_workspace(16, 100, 100) == 0
     assert L.agz_linear_fp8_forward(0, None, None, None, None, 0, 0, None, 0) == -1
     assert L.agz_linear_fp8_workspace(-1, 1, 1) < 0 and L.agz_linear_fp8_saved(1, 1, -1, 1, 1) < 0 and L.agz_linear_fp8_backward_workspace(1, 1 << 31, 1, 1, 1, 1) < 0
     assert L.agz_linear_fp8_saved(5, 6, 7, 0, 0) == 0
