@@ -189,7 +189,7 @@ __device__ __forceinline__ Done finish(const LpPar& p, int64_t i, const Sums& q,
     const float ls = none ? 0.0f : (bad ? NAN : logf(q.s)), base = base_of(q.mx);
     const float h = none ? 0.0f : ls - q.sd / q.s;
     if (writes) {
-        *(float4*)(p.stats + i * 4) = make_float4(base, ls, h, q.ts);
+        if (p.stats) *(float4*)(p.stats + i * 4) = make_float4(base, ls, h, q.ts);
         if (p.entropy) p.entropy[i] = h;
         if (p.target_logp) p.target_logp[i] = q.tx - ls * q.ts;
         if (p.move_logp) p.move_logp[i] = bad ? NAN : (given ? xm - base - ls : 0.0f);
@@ -482,7 +482,7 @@ static int check(const char* who, const agz_logprob_args* q) {
     if (q->top < 0 || q->top > AGZ_TOP_MAX) return fail(AGZ_ERR_ARG, "%s: %d alternatives (0 to %d)", who, q->top, AGZ_TOP_MAX);
     if (q->ld < 0 || q->ld_mask < 0 || q->ld_target < 0) return fail(AGZ_ERR_ARG, "%s: a negative stride", who);
     if (q->n == 0) return AGZ_OK;
-    if (!q->logits || !q->stats) return fail(AGZ_ERR_ARG, "%s: logits and stats are required", who);
+    if (!q->logits) return fail(AGZ_ERR_ARG, "%s: logits are required", who);
     if (!aligned(q->logits, esize(q->dtype)) || !aligned(q->target, 4) || !aligned(q->moves, 8) || !aligned(q->stats, 16) || !aligned(q->top_logp, 4) || !aligned(q->top_move, 4) ||
         !aligned(q->move_logp, 4) || !aligned(q->entropy, 4) || !aligned(q->target_logp, 4))
         return fail(AGZ_ERR_ARG, "%s: a pointer is not aligned to its type (stats: to 16 bytes)", who);
@@ -569,6 +569,7 @@ int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
 int agz_logprob_backward(int device, void* stream, const agz_logprob_args* q, const float* g_move, const float* g_entropy, const float* g_target, const float* g_top, void* dx, int64_t ldd) {
     if (int rc = check("agz_logprob_backward", q)) return rc;
     if (q->n > 0) {
+        if (!q->stats) return fail(AGZ_ERR_ARG, "agz_logprob_backward: the forward call's stats are required");
         if (!dx || ldd < q->a || !aligned(dx, esize(q->dtype))) return fail(AGZ_ERR_ARG, "agz_logprob_backward: dlogits with a row stride of at least %lld", (long long)q->a);
         if (g_move && !q->moves) return fail(AGZ_ERR_ARG, "agz_logprob_backward: g_move without moves");
         if (g_target && !q->target) return fail(AGZ_ERR_ARG, "agz_logprob_backward: g_target without a target");

@@ -9,11 +9,13 @@ stream of their device, nothing waits for it, and it can be captured into a grap
 queued, errors of the library AgzError.  There is no CPU path.
 """
 import ctypes as C
+import functools
 import struct
 from collections import namedtuple
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream     # the current stream's handle without a Stream object around it
+from torch._C import _cuda_isCurrentStreamCapturing as _capturing
 
 from . import lib as _lib
 
@@ -68,60 +70,59 @@ _LP = struct.Struct("=qqqqii13q")
 assert _LP.size == C.sizeof(_lib.LogProbArgs)
 
 
-def _log_probs_forward(logits, moves, mask, target, top):
-    """Checked arguments -> (what the backward pass needs besides the tensors, move, entropy, target, top, top_move)."""
-    L = _lib.load_library()
+def _log_probs_forward(logits, head, moves, target, top, stats):
+    """head: the inputs, checked and packed -> move, entropy, target, top, top_move; stats [n, 4] (None: not wanted): what the backward pass reads."""
     n, a = logits.shape
-    i = logits.get_device()
-    f32 = {"dtype": torch.float32, "device": logits.device}
-    stats, entropy = torch.empty(n, 4, **f32), torch.empty(n, **f32)
-    move = None if moves is None else torch.empty(n, **f32)
-    expected = None if target is None else torch.empty(n, **f32)
-    tops = top_move = ws = None
+    dev, f32 = logits.device, torch.float32
+    entropy = torch.empty(n, dtype=f32, device=dev)
+    move = None if moves is None else torch.empty(n, dtype=f32, device=dev)
+    expected = None if target is None else torch.empty(n, dtype=f32, device=dev)
+    tops = top_move = None
     if top:
-        tops, top_move = torch.empty(n, top, **f32), torch.empty(n, top, dtype=torch.int32, device=logits.device)
-    need = L.agz_logprob_workspace(n, a, top) if a > 1024 else 0      # (rows that fit a wave's registers need none)
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    head = (n, a, logits.data_ptr(), _rows(logits, "logits"), _CODE[logits.dtype], top,
-            0 if mask is None else mask.data_ptr(), 0 if mask is None or mask.shape[0] == 1 else mask.stride(0), 0 if moves is None else moves.data_ptr(),
-            0 if target is None else target.data_ptr(), 0 if target is None else _rows(target, "target"))
+        tops, top_move = torch.empty(n, top, dtype=f32, device=dev), torch.empty(n, top, dtype=torch.int32, device=dev)
+    L, need, ws = _lib.load_library(), 0, None
+    if a > 1024:                                             # (shorter rows need no workspace)
+        need = L.agz_logprob_workspace(n, a, top)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
     q = _LP.pack(*head, 0 if move is None else move.data_ptr(), entropy.data_ptr(), 0 if expected is None else expected.data_ptr(),
-                 tops.data_ptr() if top else 0, top_move.data_ptr() if top else 0, stats.data_ptr(), ws.data_ptr() if need else 0, need)
+                 tops.data_ptr() if top else 0, top_move.data_ptr() if top else 0, 0 if stats is None else stats.data_ptr(), ws.data_ptr() if need else 0, need)
+    i = dev.index
     rc = L.agz_logprob_forward(i, _raw_stream(i), q)
     if rc:
         _lib_call(rc, L)
-    return (head, stats), move, entropy, expected, tops, top_move
+    return move, entropy, expected, tops, top_move
 
 
 def _log_probs_backward(ctx, g_move, g_entropy, g_target, g_top, _):
-    if g_move is None and g_entropy is None and g_target is None and g_top is None:
-        return None, None, None, None, None
-    logits, _, _, _, top_move, stats = ctx.saved_tensors
-    L = _lib.load_library()
+    logits, stats, top_move = ctx.saved_tensors[:3]
     head = ctx.head
-    q = _LP.pack(*head, 0, 0, 0, 0, 0 if top_move is None else top_move.data_ptr(), stats.data_ptr(), 0, 0)
     g = [None if x is None else x.contiguous() for x in (g_move, g_entropy, g_target, g_top)]     # (held here until the call is queued)
     dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    i = logits.get_device()
-    rc = L.agz_logprob_backward(i, _raw_stream(i), q, *map(_ptr, g), dx.data_ptr(), head[1])
+    L, i = _lib.load_library(), logits.get_device()
+    rc = L.agz_logprob_backward(i, _raw_stream(i), _LP.pack(*head, 0, 0, 0, 0, 0 if top_move is None else top_move.data_ptr(), stats.data_ptr(), 0, 0),
+                                _ptr(g[0]), _ptr(g[1]), _ptr(g[2]), _ptr(g[3]), dx.data_ptr(), head[1])
     if rc:
         _lib_call(rc, L)
-    return dx, None, None, None, None
+    return dx, None, None
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, moves, mask, target, top):
-        (ctx.head, stats), *out = _log_probs_forward(logits, moves, mask, target, top)
+    def forward(ctx, logits, head, rest):
+        moves, mask, target, top = rest
+        stats = torch.empty(logits.shape[0], 4, dtype=torch.float32, device=logits.device)
+        out = _log_probs_forward(logits, head, moves, target, top, stats)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, moves, mask, target, out[4], stats)
+        ctx.head = head
+        ctx.save_for_backward(logits, stats, out[4], moves, mask, target)
         if top:
             ctx.mark_non_differentiable(out[4])
-        return tuple(out)
+        return out
 
     @staticmethod
     def backward(ctx, *g):
+        if g[0] is None and g[1] is None and g[2] is None and g[3] is None:
+            return None, None, None
         # a backward pass that is recorded itself (create_graph): its own gradient is refused where it is asked for
         return (_LogProbs._once if torch.is_grad_enabled() else _log_probs_backward)(ctx, *g)
 
@@ -141,19 +142,24 @@ def log_probs(logits, moves=None, mask=None, target=None, top=0):
     is not allowed either.  A row without an allowed move has entropy 0 and gradient 0; a row with NaN or +inf among the allowed is NaN.
     Differentiable in the logits through move, entropy, target and top."""
     _on_gpu(logits, "logits")
-    _float_type(logits, "logits")
-    _rows(logits, "logits")
+    code = _CODE.get(logits.dtype)
+    if code is None:
+        _float_type(logits, "logits")
+    ld = _rows(logits, "logits")
     n, a = logits.shape
     dev = logits.device
-    _need(a >= 1, "logits: no actions")
-    if not (isinstance(top, int) and 0 <= top <= min(TOP_MAX, a)):
+    if a < 1:
+        raise ValueError("logits: no actions")
+    if not (isinstance(top, int) and 0 <= top <= TOP_MAX and top <= a):
         raise ValueError(f"top: 0 to {TOP_MAX} and at most the number of actions, not {top!r}")
+    moves_at = mask_at = mask_ld = target_at = target_ld = 0
     if moves is not None:
         _on_gpu(moves, "moves", dev)
         if moves.shape != (n,) or moves.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"moves: int64 or int32 [{n}], not {moves.dtype} {list(moves.shape)}")
         if moves.dtype != torch.int64 or not moves.is_contiguous():
             moves = moves.long().contiguous()
+        moves_at = moves.data_ptr()
     if mask is not None:
         _on_gpu(mask, "mask", dev)
         if mask.dtype not in (torch.bool, torch.uint8):
@@ -162,16 +168,20 @@ def log_probs(logits, moves=None, mask=None, target=None, top=0):
             mask = mask[None]
         if mask.shape != (n, a) and mask.shape != (1, a):
             raise ValueError(f"mask: [{n}, {a}], [1, {a}] or [{a}], not {list(mask.shape)}")
-        _rows(mask, "mask")
+        mask_ld, mask_at = _rows(mask, "mask"), mask.data_ptr()
+        if mask.shape[0] == 1:
+            mask_ld = 0
     if target is not None:
         _on_gpu(target, "target", dev)
         if target.dtype != torch.float32 or target.shape != (n, a):
             raise ValueError(f"target: float32 [{n}, {a}], not {target.dtype} {list(target.shape)}")
-        _need(not target.requires_grad, "target: a constant is needed (detach() it)")
-        _rows(target, "target")
+        if target.requires_grad:
+            raise ValueError("target: a constant is needed (detach() it)")
+        target_ld, target_at = _rows(target, "target"), target.data_ptr()
+    head = (n, a, logits.data_ptr(), ld, code, top, mask_at, mask_ld, moves_at, target_at, target_ld)
     if logits.requires_grad and torch.is_grad_enabled():
-        return LogProbs(*_LogProbs.apply(logits, moves, mask, target, top))
-    return LogProbs(*_log_probs_forward(logits, moves, mask, target, top)[1:])
+        return LogProbs(*_LogProbs.apply(logits, head, (moves, mask, target, top)))
+    return LogProbs(*_log_probs_forward(logits, head, moves, target, top, None))
 
 
 # ---------------------------------------------------------------------------------------------------------------------------------------
@@ -194,6 +204,10 @@ class Fp8Matrix:
 
     @classmethod
     def of(cls, q, scale, rows, cols):
+        """From tensors that are laid out as above already."""
+        for t, name, shape, kind in ((q, "q", (rows, -(-cols // 128) * 128), FP8), (scale, "scale", (rows, -(-cols // 512) * 4), E8M0)):
+            _on_gpu(t, name, q.device)
+            _need(t.shape == shape and t.dtype == kind and t.is_contiguous() and t.data_ptr() % 16 == 0, f"{name}: {kind} {list(shape)}, contiguous and aligned to 16 bytes, is needed, not {t.dtype} {list(t.shape)}")
         m = cls.__new__(cls)
         m.q, m.scale, m.rows, m.cols = q, scale, rows, cols
         return m
@@ -273,22 +287,25 @@ _LIN = struct.Struct("=qqqqqqqqiiii")               # agz_linear_fp8_args
 assert _LIN.size == C.sizeof(_lib.LinearFp8Args)
 
 
-def _linear_args(x, w, bias, relu):
-    m, k = x.shape
-    return _LIN.pack(m, w.shape[0], k, x.data_ptr(), _rows(x, "x"), w.data_ptr(), _rows(w, "w"), 0 if bias is None else bias.data_ptr(),
-                     _CODE[x.dtype], _CODE[w.dtype], 0 if bias is None else _CODE[bias.dtype], relu)
-
-
-def _linear_forward(x, w, bias, relu, need_x, need_w):
+@functools.lru_cache(maxsize=4096)
+def _linear_sizes(m, n, k, need_x, need_w, need_b):
+    """Bytes of (the forward call's workspace, what it saves, the backward call's workspace) of a product of this size."""
     L = _lib.load_library()
-    (m, k), n, dev, i = x.shape, w.shape[0], x.device, x.get_device()
-    y = torch.empty(m, n, dtype=x.dtype, device=dev)
-    need = L.agz_linear_fp8_workspace(m, n, k)
-    if need < 0:
+    sizes = L.agz_linear_fp8_workspace(m, n, k), L.agz_linear_fp8_saved(m, n, k, need_x, need_w), L.agz_linear_fp8_backward_workspace(m, n, k, need_x, need_w, need_b)
+    if min(sizes) < 0:
         raise ValueError(f"linear_fp8: {m} x {n} x {k} is too large")
+    return sizes
+
+
+def _linear_forward(x, w, bias, relu, need_x, need_w, need_b):
+    (m, k), n, dev = x.shape, w.shape[0], x.device
+    need, keep, _ = _linear_sizes(m, n, k, need_x, need_w, need_b)
+    y = torch.empty(m, n, dtype=x.dtype, device=dev)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    saved = torch.empty(L.agz_linear_fp8_saved(m, n, k, need_x, need_w), dtype=torch.uint8, device=dev) if need_x or need_w else None
-    q = _linear_args(x, w, bias, relu)
+    saved = torch.empty(keep, dtype=torch.uint8, device=dev) if need_x or need_w else None
+    q = _LIN.pack(m, n, k, x.data_ptr(), _rows(x, "x"), w.data_ptr(), _rows(w, "w"), 0 if bias is None else bias.data_ptr(),
+                  _CODE[x.dtype], _CODE[w.dtype], 0 if bias is None else _CODE[bias.dtype], relu)
+    L, i = _lib.load_library(), dev.index
     rc = L.agz_linear_fp8_forward(i, _raw_stream(i), q, y.data_ptr(), _ptr(saved), need_x, need_w, ws.data_ptr(), need)
     if rc:
         _lib_call(rc, L)
@@ -312,17 +329,17 @@ def _linear_apply(x, w, bias, relu):
 
 def _linear_backward(ctx, dy):
     saved, y = ctx.saved_tensors
-    need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    L = _lib.load_library()
-    m, n, k = ctx.sizes
-    dev, i = dy.device, dy.get_device()
+    need_x, need_w, need_b = need_grad = ctx.needs_input_grad[:3]
+    (m, n, k), w_type, b_type, q, kept = ctx.call
+    dev = dy.device
     dy = dy.contiguous()
     dx = torch.empty(m, k, dtype=dy.dtype, device=dev) if need_x else None
-    dw = torch.empty(n, k, dtype=ctx.types[0], device=dev) if need_w else None
-    db = torch.empty(n, dtype=ctx.types[1], device=dev) if need_b else None
-    need = L.agz_linear_fp8_backward_workspace(m, n, k, need_x, need_w, need_b)
+    dw = torch.empty(n, k, dtype=w_type, device=dev) if need_w else None
+    db = torch.empty(n, dtype=b_type, device=dev) if need_b else None
+    need = _linear_sizes(m, n, k, *need_grad)[2]
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    rc = L.agz_linear_fp8_backward(i, _raw_stream(i), ctx.args, dy.data_ptr(), _ptr(y), _ptr(saved), ctx.kept[0], ctx.kept[1], _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), need)
+    L, i = _lib.load_library(), dev.index
+    rc = L.agz_linear_fp8_backward(i, _raw_stream(i), q, dy.data_ptr(), _ptr(y), _ptr(saved), kept[0], kept[1], _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), need)
     if rc:
         _lib_call(rc, L)
     return dx, dw, db, None
@@ -331,9 +348,9 @@ def _linear_backward(ctx, dy):
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, relu):
-        ctx.kept = need_x, need_w = ctx.needs_input_grad[:2]
-        y, saved, ctx.args = _linear_forward(x, w, bias, relu, need_x, need_w)
-        ctx.sizes, ctx.types = (x.shape[0], *w.shape), (w.dtype, None if bias is None else bias.dtype)
+        need = ctx.needs_input_grad[:3]
+        y, saved, q = _linear_forward(x, w, bias, relu, *need)
+        ctx.call = (x.shape[0], *w.shape), w.dtype, None if bias is None else bias.dtype, q, need
         ctx.save_for_backward(saved, y if relu else None)
         return y
 
@@ -372,7 +389,7 @@ def linear_fp8(x, w, bias=None, relu=False):
     elif ready:
         y = _linear_apply(two, w.matrix, bias, bool(relu))
     else:
-        y = _linear_forward(two, w, bias, bool(relu), False, False)[0]
+        y = _linear_forward(two, w, bias, bool(relu), False, False, False)[0]
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
@@ -412,7 +429,7 @@ class AdamW:
             _need(end <= start, f"params[{i}] and params[{j}] overlap")
         self.device, self.lr, self.betas, self.eps, self.weight_decay, self.bits, self.seed = dev, lr, tuple(betas), eps, weight_decay, bits, int(seed)
         count = len(self.params)
-        self._numel = (C.c_int64 * count)(*[p.numel() for p in self.params])
+        self._numel, self._pointers, self._shapes = (C.c_int64 * count)(*[p.numel() for p in self.params]), struct.Struct(f"={count}q"), [p.shape for p in self.params]
         self.offsets, at = [], 0
         for p in self.params:
             self.offsets.append(at)
@@ -448,37 +465,44 @@ class AdamW:
 
     def step(self, grads=None):
         """One step with `grads` (one per tensor, of one type; None: p.grad).  A tensor whose gradient is None is left as it is."""
-        L = _lib.load_library()
-        grads = [p.grad for p in self.params] if grads is None else list(grads)
-        count = len(self.params)
-        _need(len(grads) == count, f"{len(grads)} gradients for {count} tensors")
-        kind, gp, pp = None, (C.c_void_p * count)(), (C.c_void_p * count)()
-        for i, (p, g) in enumerate(zip(self.params, grads)):
-            _need(p.numel() == self._numel[i] and p.is_contiguous(), f"params[{i}] has changed its shape")
-            pp[i] = p.data_ptr()
+        params = self.params
+        grads = [p.grad for p in params] if grads is None else list(grads)
+        if len(grads) != len(params):
+            raise ValueError(f"{len(grads)} gradients for {len(params)} tensors")
+        kind, device, at = None, self.device.index, []
+        for i, (p, g, shape) in enumerate(zip(params, grads, self._shapes)):
+            if p.shape != shape or not p.is_contiguous():
+                raise ValueError(f"params[{i}] has changed its shape")
             if g is None:
+                at.append(0)
                 continue
-            if g.get_device() != self.device.index:
+            if g.get_device() != device:
                 raise ValueError(f"grads[{i}] is on {g.device}, the tensors on {self.device}")
-            kind = kind or g.dtype
-            if g.dtype != kind or kind not in _CODE:
-                raise ValueError(f"grads[{i}] is {g.dtype}: one of float32, bfloat16, float16 for all")
-            if g.shape != p.shape:
-                raise ValueError(f"grads[{i}] is {list(g.shape)}, the tensor {list(p.shape)}")
+            if g.dtype is not kind:
+                if kind is not None or g.dtype not in _CODE:
+                    raise ValueError(f"grads[{i}] is {g.dtype}: one of float32, bfloat16, float16 for all")
+                kind = g.dtype
+            if g.shape != shape:
+                raise ValueError(f"grads[{i}] is {list(g.shape)}, the tensor {list(shape)}")
             if not g.is_contiguous():
                 g = grads[i] = g.contiguous()
-            gp[i] = g.data_ptr()
+            at.append(g.data_ptr())
         if self.step_dev is None:
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing():
                 raise RuntimeError("AdamW.step in a graph: capturable=True is needed (a replay has to count its step on the device)")
+            counter = 0
         else:
             self.step_dev.add_(1)
+            counter = self.step_dev.data_ptr()
         t = self.steps + 1
-        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[self.params[0].dtype], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t,
-                        0 if self.step_dev is None else self.step_dev.data_ptr())
+        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[params[0].dtype], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter)
         second, ms, rs = (self.v, None, None) if self.bits == 32 else (self.r, self.m_scale, self.r_scale)
-        _lib_call(L.agz_adamw_step(self.device.index, _raw_stream(self.device.index), o, count, pp, gp, self._numel, self.m.data_ptr(), second.data_ptr(), _ptr(ms), _ptr(rs)), L)
-        torch.autograd.graph.increment_version(self.params)
+        L = _lib.load_library()
+        rc = L.agz_adamw_step(device, _raw_stream(device), o, len(params), self._pointers.pack(*[p.data_ptr() for p in params]), self._pointers.pack(*at), self._numel,
+                              self.m.data_ptr(), second.data_ptr(), _ptr(ms), _ptr(rs))
+        if rc:
+            _lib_call(rc, L)
+        torch.autograd.graph.increment_version(params)
         self.steps = t
 
 

@@ -286,7 +286,7 @@ typedef struct {
     float *target_logp;         /* [n] */
     float *top_logp;            /* [n][top] */
     int32_t *top_move;          /* [n][top] */
-    float *stats;               /* [n][4]: largest logit, log of the sum above it, entropy, sum of targets: what the backward pass reads; required */
+    float *stats;               /* [n][4]: largest logit, log of the sum above it, entropy, sum of targets: what the backward call needs */
     void *workspace;            /* agz_logprob_workspace bytes (16-byte aligned); NULL where that is 0 */
     int64_t workspace_bytes;
 } agz_logprob_args;

@@ -301,10 +301,10 @@ def test_offsets_beyond_32_bits():
     x[-3:] = tail.cuda()
     q = ops.quantize_fp8(x)
     want = blocks(tail, 1)[0]
-    last = ops.Fp8Matrix.of(q.q[-3:], q.scale[-3:], 3, k)
+    last = ops.Fp8Matrix.of(q.q[-3:].clone(), q.scale[-3:].clone(), 3, k)
     assert torch.equal(last.dequantize().double().cpu(), want) and not q.q[-9:-3].view(torch.uint8).any()
     t = ops.quantize_fp8(x, transposed=True)
-    got = ops.Fp8Matrix.of(t.q[-3:], t.scale[-3:], 3, m).dequantize()[:, -3:].double().cpu()
+    got = ops.Fp8Matrix.of(t.q[-3:].clone(), t.scale[-3:].clone(), 3, m).dequantize()[:, -3:].double().cpu()
     full = torch.zeros(3, 128)
     full[:, m % 128 - 3:m % 128] = tail[:, -3:].t().float()       # the last block along the rows
     assert torch.equal(got, blocks(full, 1)[0][:, m % 128 - 3:m % 128])
@@ -338,7 +338,10 @@ def test_changed_results_are_noticed():
 @pytest.mark.gpu
 def test_refusals_on_the_gpu():
     x, w = torch.randn(4, 64, device="cuda"), torch.randn(8, 64, device="cuda")
-    for bad, match in ((lambda: ops.quantize_fp8(x.double()), "float32"), (lambda: ops.quantize_fp8(x, 64), "block_rows"), (lambda: ops.quantize_fp8(x.t()), "next to each other"),
+    q = matrix(x)
+    assert torch.equal(ops.Fp8Matrix.of(q.q, q.scale, 4, 64).dequantize(), q.dequantize())
+    for bad, match in ((lambda: ops.Fp8Matrix.of(q.q, q.scale, 5, 64), "q:"), (lambda: ops.Fp8Matrix.of(q.q, q.scale, 4, 129), "q:"), (lambda: ops.Fp8Matrix.of(q.q, q.scale[:, :3], 4, 64), "scale:"),
+                       (lambda: ops.Fp8Matrix.of(q.q.view(torch.uint8), q.scale, 4, 64), "q:"), (lambda: ops.Fp8Matrix.of(q.q, q.scale.cpu(), 4, 64), "GPU"), (lambda: ops.quantize_fp8(x.double()), "float32"), (lambda: ops.quantize_fp8(x, 64), "block_rows"), (lambda: ops.quantize_fp8(x.t()), "next to each other"),
                        (lambda: ops.quantize_fp8(x[0]), "two dimensions"), (lambda: ops.matmul_fp8(x, w), "Fp8Matrix"),
                        (lambda: ops.matmul_fp8(matrix(x), matrix(w[:, :32].contiguous())), "columns"), (lambda: ops.matmul_fp8(matrix(x), matrix(w), dtype=torch.float64), "dtype"),
                        (lambda: ops.matmul_fp8(matrix(x), matrix(w), torch.randn(7, device="cuda")), "bias"), (lambda: ops.linear_fp8(x, w[:, :32]), "columns"),

@@ -436,12 +436,12 @@ def test_refusals_without_a_gpu():
     refused("alternatives", top=33)
     refused("stride", ld=-1)
     refused("required", logits=None)
-    refused("required", stats=None)
     refused("aligned", logits=at + 2)
     refused("aligned", stats=at + 4)
     refused("without moves", move_logp=at)
     refused("without a target", target_logp=at)
     back = L.agz_logprob_backward
+    refused("stats are required", back, (None, None, None, None, at, 4), stats=None)
     refused("row stride", back, (None, None, None, None, None, 4))
     refused("row stride", back, (None, None, None, None, at, 3))
     refused("without moves", back, (at, None, None, None, at, 4))
