@@ -244,13 +244,17 @@ template <typename T, int VEC, int G, int NV, bool PLAIN> __global__ __launch_bo
 // is one block of PART elements where alternatives are wanted or rows are few, up to MOST blocks where there are waves enough without: a lane then carries its
 // own maximum and sums from block to block (the sums rescaled where the maximum grows), the next block's loads under way behind them,
 // and the lanes are joined once.  (4096 rows of 50001 bf16: a block a wave 221 us.)
-constexpr int PART = 2048, MOST = 16, WAVES_ENOUGH = 8192;
+// Without mask and target the spans lie on 16-byte borders of memory wherever the row begins: the first one begins up to seven elements before the row (and is read
+// from the row's start, the elements that are not its own left out), since unaligned spans cost a tenth (50001 against 50000 bf16).
+constexpr int PART = 2048, MOST = 16, WAVES_ENOUGH = 8192, MOST_PAD = 7;
+template <typename T, int VEC> __device__ __forceinline__ int pad_of(const T* row) { return (int)((uintptr_t)row / sizeof(T) & (VEC - 1)); }
+__device__ __forceinline__ int64_t span_at(int64_t own, int64_t last) { return own < 0 ? 0 : (own < last ? own : last); }     // last: a - VEC
 struct PartOut { Sums q; float pad[3]; };
 
 // blocks of a part and parts of a row
 struct Parts { int32_t blocks, parts; };
-static Parts parts_of(int64_t n, int64_t a, int top) {
-    const int64_t all = cdiv(a, PART);
+static Parts parts_of(int64_t n, int64_t a, int top, bool plain) {
+    const int64_t all = cdiv(plain ? a + MOST_PAD : a, PART);
     int64_t blocks = top > 0 ? 1 : n * all / WAVES_ENOUGH;
     blocks = blocks < 1 ? 1 : (blocks > MOST ? MOST : blocks);
     const int64_t parts = cdiv(all, blocks);
@@ -271,15 +275,14 @@ template <typename T, int VEC, int NV, bool PLAIN> __global__ __launch_bounds__(
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int64_t i = w / s.parts;
     if (i >= p.n) return;
-    const int64_t begin = (w - i * s.parts) * s.blocks * PART, stop = begin + (int64_t)s.blocks * PART < p.a ? begin + (int64_t)s.blocks * PART : p.a;
     const T* x = (const T*)p.x + i * p.ld;
+    const int64_t begin = (w - i * s.parts) * s.blocks * PART - (PLAIN ? pad_of<T, VEC>(x) : 0), stop = begin + (int64_t)s.blocks * PART < p.a ? begin + (int64_t)s.blocks * PART : p.a;
     if constexpr (PLAIN) {                                     // no mask, no target, no alternatives
         Span<T, VEC> v[NV], u[NV];
         auto fetch = [&](Span<T, VEC> (&to)[NV], int64_t first) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int64_t own = first + VEC * (l + 64 * k);
-                to[k] = *(const Span<T, VEC>*)(x + (own < p.a - VEC ? own : p.a - VEC));
+                to[k] = *(const Span<T, VEC>*)(x + span_at(first + VEC * (l + 64 * k), p.a - VEC));
             }
         };
         Sums q{-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -289,12 +292,12 @@ template <typename T, int VEC, int NV, bool PLAIN> __global__ __launch_bounds__(
             float f[NV * VEC], mx = -INFINITY;
 #pragma unroll
             for (int k = 0; k < NV * VEC; ++k) f[k] = to_f(v[k / VEC].e[k % VEC]);
-            if (first + PART > p.a) {                          // the row's last block: entries outside it, and those that a span before it has, count as not there
+            if (first < 0 || first + PART > p.a) {             // the row's first and last block: entries that are not the span's own count as not there
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
-                    const int64_t own = first + VEC * (l + 64 * k), at = own < p.a - VEC ? own : p.a - VEC;
+                    const int64_t own = first + VEC * (l + 64 * k), at = span_at(own, p.a - VEC);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) f[k * VEC + e] = own < p.a && at + e >= own ? f[k * VEC + e] : -INFINITY;
+                    for (int e = 0; e < VEC; ++e) f[k * VEC + e] = at + e >= own && at + e < own + VEC ? f[k * VEC + e] : -INFINITY;
                 }
             }
 #pragma unroll
@@ -475,6 +478,38 @@ template <typename T, int VEC, int G, int NV, bool PLAIN> __global__ __launch_bo
     }
 }
 
+// ... of long rows without mask, target and cotangents of alternatives: a wave per block, spans on 16-byte borders as in the forward pass (the gradient's rows lie
+// like the logits' where their strides agree)
+template <typename T, int VEC, int NV> __global__ __launch_bounds__(256) void k_logprob_grad_part(LpPar p, int32_t parts) {
+    const int l = threadIdx.x & 63;
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), i = w / parts;
+    if (i >= p.n) return;
+    const T* x = (const T*)p.x + i * p.ld;
+    T* dx = (T*)p.dx + i * p.ldd;
+    const int64_t first = (w - i * parts) * PART - pad_of<T, VEC>(x);
+    Span<T, VEC> v[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] = *(const Span<T, VEC>*)(x + span_at(first + VEC * (l + 64 * k), p.a - VEC));
+    const float4 st = *(const float4*)(p.stats + i * 4);
+    GradRow c{st.x, st.y, p.g_entropy ? p.g_entropy[i] : 0.0f, 0.0f, 0.0f, 0.0f, -1};
+    if (p.moves && p.g_move) {
+        const int64_t mv = p.moves[i];
+        if (mv >= 0 && mv < p.a) { c.mv = (int32_t)mv; c.gm = p.g_move[i]; }
+    }
+    c.whole = c.gm + c.gh * st.z;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int64_t own = first + VEC * (l + 64 * k), at = span_at(own, p.a - VEC);
+        Span<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.e[e] = from_f<T>(grad_at(c, to_f(v[k].e[e]), 0.0f, at + e == c.mv));
+        if (at == own) *(Span<T, VEC>*)(dx + own) = o;
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) if (at + e >= own && at + e < own + VEC) dx[at + e] = o.e[e];
+    }
+}
+
 static int check(const char* who, const agz_logprob_args* q) {
     if (!q) return fail(AGZ_ERR_ARG, "%s: no arguments", who);
     if (q->n < 0 || q->a < 1 || q->a > (1ll << 30)) return fail(AGZ_ERR_ARG, "%s: %lld rows of %lld actions (rows >= 0, 1 <= actions <= 2^30)", who, (long long)q->n, (long long)q->a);
@@ -535,7 +570,7 @@ extern "C" {
 int64_t agz_logprob_workspace(int64_t n, int64_t a, int32_t top) {
     if (n < 0 || a < 1 || a > (1ll << 30) || top < 0 || top > AGZ_TOP_MAX) return -1;
     if (a <= PART) return 0;
-    return n * parts_of(n, a, top).parts * (int64_t)(sizeof(PartOut) + 8 * top);
+    return n * parts_of(n, a, top, true).parts * (int64_t)(sizeof(PartOut) + 8 * top);
 }
 
 int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
@@ -549,9 +584,9 @@ int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
     if (on.rc != AGZ_OK) return on.rc;
     if (q->n == 0) return AGZ_OK;
     const LpPar p = pack(q);
-    const Parts w = parts_of(p.n, p.a, p.top);
-    if (too_many(p.n * w.parts)) return fail(AGZ_ERR_ARG, "agz_logprob_forward: too many rows");
     const bool plain = !p.mask && !p.target && p.top == 0;
+    const Parts w = parts_of(p.n, p.a, p.top, plain);
+    if (too_many(p.n * w.parts)) return fail(AGZ_ERR_ARG, "agz_logprob_forward: too many rows");
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
         if (p.a <= PART)
@@ -580,11 +615,13 @@ int agz_logprob_backward(int device, void* stream, const agz_logprob_args* q, co
     if (q->n == 0) return AGZ_OK;
     LpPar p = pack(q);
     p.g_move = g_move; p.g_entropy = g_entropy; p.g_target = g_target; p.g_top = g_top; p.dx = dx; p.ldd = ldd;
-    const int64_t parts = cdiv(p.a, PART);
-    if (too_many(p.n * parts)) return fail(AGZ_ERR_ARG, "agz_logprob_backward: too many rows");
     const bool plain = !p.mask && !g_target && !g_top;
+    const int64_t parts = p.a <= PART ? 1 : cdiv(plain ? p.a + MOST_PAD : p.a, PART);
+    if (too_many(p.n * parts)) return fail(AGZ_ERR_ARG, "agz_logprob_backward: too many rows");
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
+        constexpr int V = 16 / sizeof(T);
+        if (plain && parts > 1) return launch(k_logprob_grad_part<T, V, PART / 64 / V>, dim3((uint32_t)cdiv(p.n * parts, 4)), dim3(256), 0, stream, p, (int32_t)parts);
         return by_length<T>(p.a, 0, [&](auto vec, auto g, auto nv) {
             return launch(plain ? k_logprob_grad<T, vec(), g(), nv(), true> : k_logprob_grad<T, vec(), g(), nv(), false>, dim3((uint32_t)cdiv(p.n * parts, 256 / g())), dim3(256), 0, stream, p, (int32_t)parts);
         });
