@@ -73,7 +73,7 @@ __device__ __forceinline__ Sums row_sums(const Row<T, VEC, G, NV>& r, const floa
     for (int k = 0; k < NV * VEC; ++k) {
         const float d = r.x[k] - base, e = __builtin_amdgcn_exp2f(d * LOG2E);
         o.s += e;
-        o.sd += e * fmaxf(d, -3.0e38f);                        // (0 * -inf)
+        o.sd = __builtin_fmaf(e, fmaxf(d, -3.0e38f), o.sd);     // (0 * -inf)
     }
     o.s = lanes_sum<G>(o.s);
     o.sd = lanes_sum<G>(o.sd);
@@ -308,7 +308,7 @@ template <typename T, int VEC, int NV, bool PLAIN> __global__ __launch_bounds__(
             for (int k = 0; k < NV * VEC; ++k) {
                 const float d = f[k] - base, e = __builtin_amdgcn_exp2f(d * LOG2E);
                 q.s += e;
-                q.sd += e * fmaxf(d, -3.0e38f);
+                q.sd = __builtin_fmaf(e, fmaxf(d, -3.0e38f), q.sd);
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) v[k] = u[k];
