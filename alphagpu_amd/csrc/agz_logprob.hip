@@ -570,7 +570,8 @@ extern "C" {
 int64_t agz_logprob_workspace(int64_t n, int64_t a, int32_t top) {
     if (n < 0 || a < 1 || a > (1ll << 30) || top < 0 || top > AGZ_TOP_MAX) return -1;
     if (a <= PART) return 0;
-    return n * parts_of(n, a, top, true).parts * (int64_t)(sizeof(PartOut) + 8 * top);
+    const int64_t p = parts_of(n, a, top, true).parts, q = parts_of(n, a, top, false).parts;     // (one block more may be longer parts, and fewer)
+    return n * (p > q ? p : q) * (int64_t)(sizeof(PartOut) + 8 * top);
 }
 
 int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {

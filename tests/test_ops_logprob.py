@@ -248,6 +248,26 @@ def test_the_gradient_against_differences():
         assert ((dx[:, j].cpu().double() - num).abs() <= size * (1 + most) * h * h + ftol / h + tol["dlogits"][:, j])[smooth].all(), j
 
 
+def test_the_workspace_holds_every_plan():
+    """Rows without mask and target are planned with room for one more block of 2048 at their end, and with longer parts earlier: 4096 rows of 6144 are two
+    parts each so, and three with a mask.  32 bytes for each part."""
+    L = lib.load_library()
+    for n, a, parts in ((4096, 6144, 3), (2731, 6140, 3), (8191, 2049, 2), (1366, 12288, 6), (1, 33552384, 16383)):
+        assert L.agz_logprob_workspace(n, a, 0) >= n * parts * 32, (n, a)
+
+
+@pytest.mark.gpu
+def test_many_long_rows_with_a_mask():
+    """Numbers of rows from which a masked call is cut into other parts than a plain one."""
+    for n, a in ((4096, 6144), (1366, 12288)):
+        x, mv, mk, t, g = inputs(n, a, torch.bfloat16, 15, mask="one")
+        r = ops.log_probs(x.cuda(), mv.cuda(), mask=mk.cuda(), target=t.cuda())
+        rows = torch.tensor([0, 1, n // 2, n - 2, n - 1])
+        want, tol = plain(x[rows], mv[rows], mk, t[rows])
+        for k in ("move", "entropy", "target"):
+            close(getattr(r, k).cpu()[rows], want[k], tol[k], (n, a, k))
+
+
 @pytest.mark.gpu
 def test_equal_logits_come_by_index():
     for a in (81, 300, 9000, 70000):
