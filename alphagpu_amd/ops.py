@@ -70,6 +70,20 @@ _LP = struct.Struct("=qqqqii13q")
 assert _LP.size == C.sizeof(_lib.LogProbArgs)
 
 
+def _log_probs_head(logits, moves, mask, target, top):
+    """The first fields of agz_logprob_args: sizes, pointers, row strides."""
+    ld = _rows(logits, "logits")
+    n, a = logits.shape
+    mask_at = mask_ld = target_at = target_ld = 0
+    if mask is not None:
+        mask_ld, mask_at = _rows(mask, "mask"), mask.data_ptr()
+        if mask.shape[0] == 1:
+            mask_ld = 0
+    if target is not None:
+        target_ld, target_at = _rows(target, "target"), target.data_ptr()
+    return n, a, logits.data_ptr(), ld, _CODE[logits.dtype], top, mask_at, mask_ld, 0 if moves is None else moves.data_ptr(), target_at, target_ld
+
+
 def _log_probs_forward(logits, head, moves, target, top, stats):
     """head: the inputs, checked and packed -> move, entropy, target, top, top_move; stats [n, 4] (None: not wanted): what the backward pass reads."""
     n, a = logits.shape
@@ -94,8 +108,10 @@ def _log_probs_forward(logits, head, moves, target, top, stats):
 
 
 def _log_probs_backward(ctx, g_move, g_entropy, g_target, g_top, _):
-    logits, stats, top_move = ctx.saved_tensors[:3]
+    logits, stats, top_move, moves, mask, target = ctx.saved_tensors
     head = ctx.head
+    if head != (now := _log_probs_head(logits, moves, mask, target, head[5])):      # (hooks on saved tensors may give back copies of them)
+        head = now
     g = [None if x is None else x.contiguous() for x in (g_move, g_entropy, g_target, g_top)]     # (held here until the call is queued)
     dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     L, i = _lib.load_library(), logits.get_device()
@@ -142,24 +158,21 @@ def log_probs(logits, moves=None, mask=None, target=None, top=0):
     is not allowed either.  A row without an allowed move has entropy 0 and gradient 0; a row with NaN or +inf among the allowed is NaN.
     Differentiable in the logits through move, entropy, target and top."""
     _on_gpu(logits, "logits")
-    code = _CODE.get(logits.dtype)
-    if code is None:
+    if logits.dtype not in _CODE:
         _float_type(logits, "logits")
-    ld = _rows(logits, "logits")
+    _rows(logits, "logits")
     n, a = logits.shape
     dev = logits.device
-    if a < 1:
-        raise ValueError("logits: no actions")
+    if not 1 <= a <= 1 << 30:
+        raise ValueError(f"logits: {a} actions (1 to 2^30)")
     if not (isinstance(top, int) and 0 <= top <= TOP_MAX and top <= a):
         raise ValueError(f"top: 0 to {TOP_MAX} and at most the number of actions, not {top!r}")
-    moves_at = mask_at = mask_ld = target_at = target_ld = 0
     if moves is not None:
         _on_gpu(moves, "moves", dev)
         if moves.shape != (n,) or moves.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"moves: int64 or int32 [{n}], not {moves.dtype} {list(moves.shape)}")
         if moves.dtype != torch.int64 or not moves.is_contiguous():
             moves = moves.long().contiguous()
-        moves_at = moves.data_ptr()
     if mask is not None:
         _on_gpu(mask, "mask", dev)
         if mask.dtype not in (torch.bool, torch.uint8):
@@ -168,17 +181,13 @@ def log_probs(logits, moves=None, mask=None, target=None, top=0):
             mask = mask[None]
         if mask.shape != (n, a) and mask.shape != (1, a):
             raise ValueError(f"mask: [{n}, {a}], [1, {a}] or [{a}], not {list(mask.shape)}")
-        mask_ld, mask_at = _rows(mask, "mask"), mask.data_ptr()
-        if mask.shape[0] == 1:
-            mask_ld = 0
     if target is not None:
         _on_gpu(target, "target", dev)
         if target.dtype != torch.float32 or target.shape != (n, a):
             raise ValueError(f"target: float32 [{n}, {a}], not {target.dtype} {list(target.shape)}")
         if target.requires_grad:
             raise ValueError("target: a constant is needed (detach() it)")
-        target_ld, target_at = _rows(target, "target"), target.data_ptr()
-    head = (n, a, logits.data_ptr(), ld, code, top, mask_at, mask_ld, moves_at, target_at, target_ld)
+    head = _log_probs_head(logits, moves, mask, target, top)
     if logits.requires_grad and torch.is_grad_enabled():
         return LogProbs(*_LogProbs.apply(logits, head, (moves, mask, target, top)))
     return LogProbs(*_log_probs_forward(logits, head, moves, target, top, None))

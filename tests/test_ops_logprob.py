@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from alphagpu_amd import lib, ops
 
@@ -383,6 +384,31 @@ def test_two_captured_graphs_side_by_side():
             torch.cuda.current_stream().wait_stream(s)
         for o, w in zip(outs, want):
             assert torch.equal(o.entropy, w.entropy) and torch.equal(o.top_move, w.top_move) and torch.equal(o.top, w.top)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_that_come_back_elsewhere():
+    """Hooks that keep what a backward pass needs in host memory, and a part that is computed again (checkpoint): the memory of the first forward pass
+    belongs to others by the time of the backward pass."""
+    for a in (81, 5000):
+        x, mv, mk, t, g = (v.cuda() if isinstance(v, torch.Tensor) else v for v in inputs(40, a, torch.float32, 16, top=3))
+        g = {k: v.cuda() for k, v in g.items()}
+
+        def part(x):
+            r = ops.log_probs(x * 1.0, mv + 0, mask=mk.clone(), target=t + 0, top=3)
+            return [getattr(r, k) for k in g]
+
+        def grad(out, leaf):
+            junk = [torch.full_like(v, 1) for v in (x, mv, mk, t) for _ in range(4)]       # what was let go is written to
+            return torch.autograd.grad(out, [leaf], list(g.values()))[0], junk
+
+        leaf = x.clone().requires_grad_()
+        want, _ = grad(part(leaf), leaf)
+        with torch.autograd.graph.save_on_cpu():
+            out = part(leaf)
+        assert torch.equal(grad(out, leaf)[0], want)
+        out = torch.utils.checkpoint.checkpoint(part, leaf, use_reentrant=False)
+        assert torch.equal(grad(out, leaf)[0], want)
 
 
 @pytest.mark.gpu
