@@ -47,6 +47,7 @@ __device__ __forceinline__ float aw_round(float y, uint32_t u) {
 // A workgroup takes AW_CHUNK neighbouring elements of one tensor, a lane AW_TURNS times four of them: every access is 16 (8, 4) bytes a lane and whole lines a
 // wave, and all of a lane's loads are under way before the first is used.  A block of 128 is half a wave: its largest is a reduction over 32 lanes.
 constexpr int AW_TURNS = 2, AW_CHUNK = 256 * 4 * AW_TURNS, AW_BLOCKS = AW_CHUNK / AW_BLOCK;
+constexpr int64_t AW_MOST = 1ll << 27;      // blocks of a launch: 2^23 workgroups of 256 lanes, and one more a tensor (a launch has fewer than 2^32 lanes)
 
 template <typename T> __device__ __forceinline__ void load4(float* to, const T* from, int64_t i, int64_t n) {
     if (i + 4 <= n) {
@@ -193,6 +194,7 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
     if (agz_adamw_state_elements(count, numel) < 0) return fail(AGZ_ERR_ARG, "agz_adamw_step: a negative or far too large tensor");
     if (count > 0 && (!aligned(m, 16) || !aligned(v, 16))) return fail(AGZ_ERR_ARG, "agz_adamw_step: the states have to begin at a multiple of 16 bytes");
     for (int i = 0; i < count; ++i) {
+        if (cdiv(numel[i], AW_BLOCK) > AW_MOST) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d has more than 2^34 elements", i);
         if (numel[i] == 0 || !grads[i]) continue;
         if (!params[i]) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d is null", i);
         if (!aligned(params[i], esize(o->param_dtype)) || !aligned(grads[i], esize(o->grad_dtype))) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d is not aligned to its type", i);
@@ -209,7 +211,7 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
         a.inv_root = (float)(1.0 / std::sqrt(1.0 - std::pow(a.b2d, (double)o->step)));
     }
     a.seed = o->seed;
-    // launches of at most AW_MAX tensors and 2^30 blocks; a tensor of more is cut at a block (its hash index would not be: such a tensor is refused)
+    // launches of at most AW_MAX tensors and AW_MOST blocks
     int i = 0;
     int64_t state_block = 0;
     while (i < count) {
@@ -220,8 +222,7 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
         const int first = i;
         for (; i < count && k < AW_MAX; ++i) {
             const int64_t blocks = cdiv(numel[i], AW_BLOCK);
-            if (blocks > (1ll << 29)) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d has more than 2^36 elements", i);
-            if (k > 0 && (state_block - base) + blocks > (1ll << 30)) break;
+            if (k > 0 && (state_block - base) + blocks > AW_MOST) break;
             tab.t[k++] = AwTensor{params[i], grads[i], (uint32_t)numel[i], (uint32_t)(numel[i] >> 32), chunks, (uint32_t)(state_block - base)};
             chunks += grads[i] ? (uint32_t)cdiv(blocks, AW_BLOCKS) : 0;
             state_block += blocks;

@@ -563,7 +563,8 @@ template <typename T, typename F> static int by_length(int64_t a, int top, F&& f
     return AGZ_LP(V, 64, F4);
 #undef AGZ_LP
 }
-static bool too_many(int64_t groups) { return cdiv(groups, 4) > 0x7fffffffll; }
+// waves of a call: with 256 lanes for four of them fewer than 2^32 lanes (short rows need fewer: the launch itself looks again)
+static bool too_many(int64_t waves) { return waves >= 1ll << 26; }
 
 extern "C" {
 

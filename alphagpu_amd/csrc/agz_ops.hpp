@@ -35,6 +35,7 @@ struct OnDevice {
 
 // a launch that reports its own status (hipGetLastError would also report an error that somebody else's call left behind)
 template <typename... P, typename... A> int launch(void (*k)(P...), dim3 grid, dim3 block, size_t lds, void* stream, A&&... a) {
+    if ((uint64_t)grid.x * block.x > 0xFFFFFFFFull || grid.y > 65535) return fail(AGZ_ERR_ARG, "a launch of %u x %u workgroups: too large", grid.x, grid.y);
     std::tuple<P...> args(static_cast<P>(a)...);
     hipError_t e = std::apply([&](auto&... x) { void* p[] = {(void*)&x...}; return hipLaunchKernel((const void*)k, grid, block, p, lds, (hipStream_t)stream); }, args);
     if (e == hipSuccess) return AGZ_OK;

@@ -436,7 +436,7 @@ class AdamW:
         ends.sort()
         for (_, end, i), (start, _, j) in zip(ends, ends[1:]):
             _need(end <= start, f"params[{i}] and params[{j}] overlap")
-        self.device, self.lr, self.betas, self.eps, self.weight_decay, self.bits, self.seed = dev, lr, tuple(betas), eps, weight_decay, bits, int(seed)
+        self.device, self.dtype, self.lr, self.betas, self.eps, self.weight_decay, self.bits, self.seed = dev, kind, lr, tuple(betas), eps, weight_decay, bits, int(seed)
         count = len(self.params)
         self._numel, self._pointers, self._shapes = (C.c_int64 * count)(*[p.numel() for p in self.params]), struct.Struct(f"={count}q"), [p.shape for p in self.params]
         self.offsets, at = [], 0
@@ -478,10 +478,10 @@ class AdamW:
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} tensors")
-        kind, device, at = None, self.device.index, []
+        kind, own, device, at = None, self.dtype, self.device.index, []
         for i, (p, g, shape) in enumerate(zip(params, grads, self._shapes)):
-            if p.shape != shape or not p.is_contiguous():
-                raise ValueError(f"params[{i}] has changed its shape")
+            if p.shape != shape or p.get_device() != device or p.dtype is not own or not p.is_contiguous():
+                raise ValueError(f"params[{i}] has changed its shape, type or device")
             if g is None:
                 at.append(0)
                 continue
@@ -504,7 +504,7 @@ class AdamW:
             self.step_dev.add_(1)
             counter = self.step_dev.data_ptr()
         t = self.steps + 1
-        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[params[0].dtype], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter)
+        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[own], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter)
         second, ms, rs = (self.v, None, None) if self.bits == 32 else (self.r, self.m_scale, self.r_scale)
         L = _lib.load_library()
         rc = L.agz_adamw_step(device, _raw_stream(device), o, len(params), self._pointers.pack(*[p.data_ptr() for p in params]), self._pointers.pack(*at), self._numel,

@@ -291,6 +291,24 @@ def test_refusals_on_the_gpu():
             bad()
 
 
+@pytest.mark.gpu
+def test_weights_that_have_moved_are_refused():
+    """A tensor's memory exchanged behind the optimiser's back: for another place of the same kind it follows, for another device or type it refuses."""
+    for move in (lambda p: p.cpu(), lambda p: p.half()):
+        p, g = torch.randn(300, device="cuda"), torch.randn(300, device="cuda")
+        o = ops.AdamW([p])
+        p.data = move(p)
+        with pytest.raises(ValueError, match="shape, type or device"):
+            o.step([g])
+        assert o.steps == 0
+    p, q = torch.randn(300, device="cuda"), torch.randn(300, device="cuda")
+    one, two = ops.AdamW([p], capturable=True), ops.AdamW([q])
+    p.data = q.clone()
+    one.step([g])
+    two.step([g])
+    assert torch.equal(p, q)
+
+
 def test_refusals_without_a_gpu():
     with pytest.raises(ValueError, match="GPU"):
         ops.AdamW([torch.randn(3)])
@@ -309,6 +327,7 @@ def test_refusals_without_a_gpu():
     refused("dtype", param_dtype=3)
     refused("dtype", grad_dtype=-1)
     refused("bits", bits=16)
+    refused("2^34", n=2 ** 34 + 1)
     refused("scales", bits=8)
     refused("step", step=0)
     refused("betas", beta1=1.0)
