@@ -6,7 +6,8 @@
 
 The reference does this in Flux (train.jl:12-15, :50; DenseNet.jl:161-198).  Tensors are torch tensors on a GPU; the work runs on the current
 stream of their device, nothing waits for it, and it can be captured into a graph.  Wrong arguments raise ValueError before anything is
-queued, errors of the library AgzError.  There is no CPU path.
+queued, errors of the library AgzError.  There is no CPU path.  A backward pass that is captured into a graph needs leaves of its own
+(detach().requires_grad_(), and autograd.grad): gradients that another, living autograd graph accumulates into the same leaves are torch's to order.
 """
 import ctypes as C
 import functools
@@ -213,7 +214,7 @@ class Fp8Matrix:
 
     @classmethod
     def of(cls, q, scale, rows, cols):
-        """From tensors that are laid out as above already."""
+        """From tensors that are laid out as above already (no scale of NaN)."""
         for t, name, shape, kind in ((q, "q", (rows, -(-cols // 128) * 128), FP8), (scale, "scale", (rows, -(-cols // 512) * 4), E8M0)):
             _on_gpu(t, name, q.device)
             _need(t.shape == shape and t.dtype == kind and t.is_contiguous() and t.data_ptr() % 16 == 0, f"{name}: {kind} {list(shape)}, contiguous and aligned to 16 bytes, is needed, not {t.dtype} {list(t.shape)}")
@@ -417,7 +418,8 @@ class AdamW:
     params: contiguous tensors of one type on one device that do not overlap.  bits = 32: states m, v in float32.  bits = 8: m and r = sqrt(v) in
     float8_e4m3fn with one power-of-two scale per 128 elements, rounded up or down at random in proportion (from `seed`, the step and the
     element: equal calls give equal results).  The states of all tensors lie in the buffers m, v (or m, m_scale, r, r_scale), tensor i from element offsets[i] on.
-    capturable: the number of the step is kept on the device, so that a step captured into a graph counts on in its replays."""
+    capturable: the number of the step is kept on the device, so that a step captured into a graph counts on in its replays (with the lr, betas, eps
+    and weight_decay it was captured with)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, seed=0, capturable=False):
         self.params = list(params)

@@ -302,7 +302,7 @@ int  agz_logprob_backward(int device, void *stream, const agz_logprob_args *args
 /* Matrices in 8 bits: e4m3 values [rows][pitch], pitch = cols rounded up to 128 (the columns behind `cols` are 0), and one scale 2^(byte - 127)
  * (e8m0) per row and 128 columns: bytes [rows][scale_pitch], scale_pitch = (cols / 128 rounded up) rounded up to 4.  The scale of a block is
  * the smallest power of two (from 2^-127 on) with |x| <= 448 scale for its finite entries (1 for a block of zeros); values are rounded to the nearest, ties to even; NaN and
- * infinities become NaN.  A power of two: the matrix unit applies such scales itself, and the scaling rounds nothing. */
+ * infinities become NaN (a scale byte of 255, which the format calls NaN, is not written and not allowed).  A power of two: the matrix unit applies such scales itself, and the scaling rounds nothing. */
 int64_t agz_fp8_pitch(int64_t cols);
 int64_t agz_fp8_scale_pitch(int64_t cols);
 /* x [rows][cols] (dtype, row stride ld) -> q, s in blocks of block_rows (1 or 128) x 128, and / or qt, st: the transposed matrix [cols][rows] with its blocks along
@@ -349,7 +349,7 @@ int  agz_linear_fp8_backward(int device, void *stream, const agz_linear_fp8_args
  * held in e4m3 with one power-of-two scale (e8m0 byte, as in agz_fp8_quantize) per 128 elements and rounded up or down at random in
  * proportion (unbiased: to the nearest, v could no longer shrink, its steps of 1 - b2 are below half a rounding step); r is 0 only where v is.
  * The random bits are a hash of (seed, t, tensor index + tensor_base, element): equal arguments give equal results.
- * A tensor whose gradient is NULL is left as it is, its states too.  Tensors must not overlap. */
+ * A tensor whose gradient is NULL is left as it is, its states too.  Tensors must not overlap; each has at most 2^34 elements. */
 typedef struct {
     double lr, beta1, beta2, eps, weight_decay;
     int32_t param_dtype, grad_dtype;   /* agz_dtype */
