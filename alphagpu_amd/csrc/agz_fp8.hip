@@ -629,7 +629,8 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) vo
     constexpr bool READY = std::is_same<T, uint8_t>::value;
     __shared__ __attribute__((aligned(16))) uint8_t held[READY ? 16 : FEW_LDS];
     __shared__ uint8_t held_scale[READY ? 1 : FEW_LDS / FB];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    // (the wave's number as one value of the wave: the matrix unit takes no heed of a lane condition, so none may stand around its instructions)
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16;
     const int r = l16 < p.m ? l16 : (int)p.m - 1;
     const int64_t c = n0 + l16 < p.n ? n0 + l16 : p.n - 1;
@@ -686,6 +687,106 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) vo
         for (int k = 1; k < FEW_WAVES; ++k) acc += sum[k][lane];
         store_row4(p, l16, n0 + g * 4, acc);
     }
+}
+
+// More rows on ready weights where the k axis has up to SHORT_STEPS steps: one launch too.  A workgroup turns its SHORT_M rows of x into 8 bits on their way into LDS (the
+// same bits that k_quantize writes, 16 lanes a row and step), the weights' 128 rows come straight from memory, all steps at once; then products and results as in the
+// tiles above.  Bound by latency where a workgroup or two a CU do it all (20001 x 162 -> 128 bf16, relu: 10.2 us a call in a graph, 11.6 MB), by memory above:
+// 200000 x 128 -> 128 30.6 us (102 MB, 3.3 TB/s).
+constexpr int SHORT_STEPS = 4, SHORT_M = 64, SHORT_N = 128;
+template <int KB> struct Short {
+    static constexpr int NT = 256, FM = 2, FN = 4, STEP = (SHORT_M + SHORT_N) * FB, IN = KB * STEP + KB * SHORT_M, OUT = SHORT_M * (SHORT_N * 2 + 16), LDS = IN > OUT ? IN : OUT;
+};
+template <typename T, int KB, bool WIDE> __global__ __launch_bounds__(256) void k_linear_short(MatPar p, const T* x, int64_t ldx) {
+    using TL = Short<KB>;
+    constexpr int FM = TL::FM, FN = TL::FN, PASSES = SHORT_M / 16;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[TL::LDS];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
+    const int64_t m0 = (int64_t)blockIdx.x * SHORT_M, n0 = (int64_t)blockIdx.y * SHORT_N;
+    const int wm = (w >> 1) * 32, wn = (w & 1) * 64;
+    // x: pass s of step k reads row 16 s + tid / 16, eight entries from column 128 k + 8 (tid % 16) on; entry by entry where the row ends inside the eight
+    Span<T, 8> raw[KB][PASSES];
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int s = 0; s < PASSES; ++s) {
+            const int64_t r = m0 + s * 16 + (tid >> 4) < p.m ? m0 + s * 16 + (tid >> 4) : p.m - 1;
+            const T* row = x + r * ldx;
+            const int at = k * FB + (tid & 15) * 8;
+            if (k + 1 < KB || at + 8 <= (int)p.k) raw[k][s] = *(const Span<T, 8>*)(row + at);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) raw[k][s].e[e] = at + e < (int)p.k ? row[at + e] : from_f<T>(0.0f);
+        }
+    // the weights' rows: their pieces as in the tiles above, and a word of scales for all steps
+    const uint32_t lastn = (uint32_t)(p.n - 1 - n0 < SHORT_N ? p.n - 1 - n0 : SHORT_N - 1), pitch = (uint32_t)p.pitch;
+    const uint8_t* qb = p.qb + n0 * p.pitch;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int i = 0; i < SHORT_N * 8 / 256; ++i) {
+            const uint32_t r = (tid >> 3) + i * 32, piece = ((tid & 7) ^ (r & 7)) * 16;
+            __builtin_amdgcn_global_load_lds((gvoid*)(qb + k * FB + (r < lastn ? r : lastn) * pitch + piece), (lvoid*)(lds + k * TL::STEP + SHORT_M * FB + i * 4096 + w * 1024), 16, 0, 0);
+        }
+    uint32_t bs[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const uint32_t c = wn + j * 16 + l16;
+        bs[j] = *(const uint32_t*)(p.sb + (n0 + (c < lastn ? c : lastn)) * p.spitch);
+    }
+    uint8_t* scale = lds + KB * TL::STEP;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int s = 0; s < PASSES; ++s) {
+            float v[8], m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { v[e] = to_f(raw[k][s].e[e]); m = fmaxf(m, fabsf(v[e])); }
+            if (__any(m == INFINITY)) {
+                m = 0.0f;
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+            }
+            const int byte = scale_byte(lanes_max<16>(m)), r = s * 16 + (tid >> 4);
+            *(uint2*)(lds + k * TL::STEP + r * FB + (((tid & 15) >> 1) ^ (r & 7)) * 16 + (tid & 1) * 8) = enc8(v, inv_scale_of(byte));
+            if ((tid & 15) == 0) scale[k * SHORT_M + r] = (uint8_t)byte;
+        }
+    __syncthreads();
+    f32x4 acc[FM][FN] = {};
+    const int p0 = (g ^ (l16 & 7)) * 16, p1 = p0 ^ 64;
+    auto frag = [&](const uint8_t* base, int i) {
+        const i32x4 x = *(const i32x4*)(base + i * 16 * FB + p0), y = *(const i32x4*)(base + i * 16 * FB + p1);
+        return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    };
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+        const uint8_t *la = lds + k * TL::STEP + (wm + l16) * FB, *lb = lds + k * TL::STEP + SHORT_M * FB + (wn + l16) * FB;
+        i32x8 av[FM];
+        int as[FM];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) { av[i] = frag(la, i); as[i] = scale[k * SHORT_M + wm + i * 16 + l16]; }
+        Wide aw[WIDE ? FM : 1];
+        if constexpr (WIDE)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) aw[i] = widen(av[i], as[i]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const i32x8 bv = frag(lb, j);
+            if constexpr (WIDE) {
+                const Wide bw = widen(bv, bs[j] >> 8 * k & 0xFF);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[i][j] = mma_wide(bw, aw[i], acc[i][j]);
+            } else
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[i][j] = mma<0>(bv, av[i], acc[i][j], (int)(bs[j] >> 8 * k), as[i]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const f32x4 b = bias4(p, n0 + wn + j * 16 + g * 4);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[i][j] = finish4(p, acc[i][j], b);
+    }
+    store_tile<T, TL, SHORT_M, SHORT_N, 2, 2>(lds, acc, (T*)p.out, p.ldo, p.m, p.n, m0, n0);
 }
 
 }  // namespace ops
@@ -768,8 +869,34 @@ Forward forward_ws(Carve& c, int64_t m, int64_t n, int64_t k) { return {c.matrix
 // a layer on weights in 8 bits: x in 8 bits first, or on the way where its rows are few
 struct Apply { Mat8 a; void* ws; };
 bool at_once(int64_t m, int64_t n, int64_t k) { return plan(m, n, k).few && m * up(k, FB) <= FEW_LDS; }
+// ... or, where the k axis is short too, x in 8 bits in the product's own launch.  Every 128 columns turn x into 8 bits again: up to 256 of them, or up to eight workgroups a
+// CU; with four steps a workgroup fills a CU's LDS, and more than one a CU wait for each other.  In one launch and in two: 20001 x 162 -> 128 bf16 10.2 and 15.0 us,
+// 1000 x 128 -> 128 5.8 and 10.4, 200000 x 128 -> 128 30.6 and 44.8, 32768 x 256 -> 512 25.7 and 29.4; but -> 1024 46.1 and 43.9, 8192 x 512 -> 512 16.7 and 15.0,
+// 65536 x 512 -> 128 43.4 and 37.3.
+bool in_one(int64_t m, int64_t n, int64_t k) {
+    const int64_t steps = cdiv(k, FB), across = cdiv(n, SHORT_N), groups = cdiv(m, SHORT_M) * across;
+    if (m <= 16 || k == 0 || steps > SHORT_STEPS) return false;
+    return steps == SHORT_STEPS ? groups <= CUS : across <= 2 || groups <= 8 * CUS;
+}
+int layer_in_one(void* stream, const agz_linear_fp8_args* q, Mat8 b, void* y) {
+    const MatPar p{nullptr, nullptr, b.q, b.s, q->m, q->n, q->k, up(q->k, FB), up(cdiv(q->k, FB), 4), q->bias, q->bias_dtype, q->relu, y, q->dtype, q->n, 1, nullptr};
+    return by_dtype(q->dtype, [&](auto t) {
+        using T = decltype(t);
+        auto go = [&](auto kb) {
+            return launch(q->relu || q->dtype == AGZ_F32 ? k_linear_short<T, kb(), true> : k_linear_short<T, kb(), false>,
+                          dim3((uint32_t)cdiv(p.m, SHORT_M), (uint32_t)cdiv(p.n, SHORT_N)), dim3(256), 0, stream, p, (const T*)q->x, q->ldx);
+        };
+        using std::integral_constant;
+        switch (cdiv(p.k, FB)) {
+            case 1: return go(integral_constant<int, 1>{});
+            case 2: return go(integral_constant<int, 2>{});
+            case 3: return go(integral_constant<int, 3>{});
+            default: return go(integral_constant<int, 4>{});
+        }
+    });
+}
 Apply apply_ws(Carve& c, int64_t m, int64_t n, int64_t k) {
-    if (at_once(m, n, k)) return {};
+    if (at_once(m, n, k) || in_one(m, n, k)) return {};
     Apply w;
     w.a = c.matrix(m, k);
     w.ws = c.take(agz_fp8_matmul_workspace(m, n, k));
@@ -883,8 +1010,9 @@ int agz_linear_fp8_forward(int device, void* stream, const agz_linear_fp8_args* 
     Carve c{(uint8_t*)ws}, d{(uint8_t*)saved};
     const Forward f = forward_ws(c, q->m, q->n, q->k);
     const Saved s = saved_of(d, q->m, q->n, q->k, need_dx, need_dw);
-    if (int rc = quantize(stream, q->x, q->dtype, q->m, q->k, q->ldx, nullptr, 1, f.a, s.at, nullptr, 0, nullptr)) return rc;
     if (int rc = quantize(stream, q->w, q->w_dtype, q->n, q->k, q->ldw, nullptr, FB, f.b, s.bt, nullptr, 0, nullptr)) return rc;
+    if (!need_dw && q->m > 0 && q->n > 0 && in_one(q->m, q->n, q->k)) return layer_in_one(stream, q, f.b, y);
+    if (int rc = quantize(stream, q->x, q->dtype, q->m, q->k, q->ldx, nullptr, 1, f.a, s.at, nullptr, 0, nullptr)) return rc;
     return product(stream, q->m, q->n, q->k, f.a, f.b, q->bias, q->bias_dtype, q->relu, y, q->dtype, q->n, f.ws);
 }
 
@@ -900,6 +1028,7 @@ int agz_linear_fp8_apply(int device, void* stream, const agz_linear_fp8_args* q,
     Carve c{(uint8_t*)ws};
     const Apply w = apply_ws(c, m, n, k);
     const Mat8 b{(uint8_t*)qw, (uint8_t*)sw};
+    if (in_one(m, n, k)) return layer_in_one(stream, q, b, y);
     if (!at_once(m, n, k)) {
         if (int rc = quantize(stream, q->x, q->dtype, m, k, q->ldx, nullptr, 1, w.a, {}, nullptr, 0, nullptr)) return rc;
         return product(stream, m, n, k, w.a, b, q->bias, q->bias_dtype, q->relu, y, q->dtype, n, w.ws);

@@ -334,7 +334,8 @@ typedef struct {
 int64_t agz_linear_fp8_workspace(int64_t m, int64_t n, int64_t k);
 int64_t agz_linear_fp8_saved(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw);
 /* the same y on weights that are held in 8 bits already (qw [n][pitch], sw as of agz_fp8_quantize with block_rows 128): args->w, ldw, w_dtype are not read;
- * up to 16 rows of together up to 32768 entries in one launch, x held in 8 bits on the way */
+ * up to 16 rows of together up to 32768 entries, and more rows of up to 512 columns (as long as n is not large), in one launch, x held in 8 bits on the way: then
+ * without a workspace (agz_linear_fp8_apply_workspace is 0) */
 int64_t agz_linear_fp8_apply_workspace(int64_t m, int64_t n, int64_t k);
 int  agz_linear_fp8_apply(int device, void *stream, const agz_linear_fp8_args *args, const void *qw, const void *sw, void *y, void *workspace, int64_t workspace_bytes);
 int64_t agz_linear_fp8_backward_workspace(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, int need_db);

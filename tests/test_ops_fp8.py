@@ -261,6 +261,32 @@ def test_few_rows_on_ready_weights(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_short_rows_in_one_launch(dtype):
+    """Up to 512 columns and more than 16 rows, x held in 8 bits on the way: the same bits as in two steps at either side of the rule that takes it (rows, columns, a second
+    tile of columns, four steps), with rows of a wider tensor, NaN, infinities, zeros and rows behind the last."""
+    for m, n, k in ((17, 128, 128), (64, 129, 1), (65, 1, 7), (63, 300, 129), (200, 127, 256), (130, 256, 257), (1000, 82, 384), (129, 130, 511), (8192, 256, 512), (8256, 256, 512),
+                    (20001, 128, 162), (66, 1030, 300), (32769, 260, 100)):
+        x = data(m, k + 3, dtype, 22)[:, 1:k + 1]
+        x[2, 0], x[3, k - 1], x[4, :] = math.nan, -math.inf, 0.0
+        w, b = data(n, k, torch.float32, 23), torch.randn(n, generator=torch.Generator().manual_seed(2)).cuda()
+        ready = ops.Fp8Weight(w.cuda())
+        wide = torch.full((m, k + 3), math.nan, dtype=dtype, device="cuda")
+        wide[:, 1:k + 1] = x.cuda()
+        for relu in (False, True):
+            got = ops.linear_fp8(wide[:, 1:k + 1], ready, b, relu=relu)
+            want = ops.matmul_fp8(ops.quantize_fp8(x.cuda()), ready.matrix, b, relu=relu, dtype=dtype)
+            assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(7), want.nan_to_num(7)), (m, n, k, relu)
+            assert torch.equal(ops.linear_fp8(wide[:, 1:k + 1], w.cuda(), b, relu=relu).nan_to_num(7), want.nan_to_num(7)), (m, n, k, relu)
+        leaf = wide[:, 1:k + 1].detach().requires_grad_()             # weights without a gradient
+        y = ops.linear_fp8(leaf, w.cuda(), b)
+        full = ops.linear_fp8(leaf, w.cuda().requires_grad_(), b)
+        dy = torch.randn(m, n, device="cuda").to(dtype)
+        assert torch.equal(y.nan_to_num(7), full.nan_to_num(7))
+        assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], torch.autograd.grad(full, leaf, dy)[0])
+
+
+@pytest.mark.gpu
 def test_another_stream_and_a_graph():
     def step(x, w, b, g):
         leaves = [t.detach().requires_grad_() for t in (x, w, b)]
@@ -382,9 +408,10 @@ def test_refusals_without_a_gpu():
         assert call() == -1 and match in err(), err()
     app = lambda ch, qw=at, sw=at, y=at, w=ws, n=60000: L.agz_linear_fp8_apply(0, None, C.byref(lib.LinearFp8Args(**{**lin, **ch})), qw, sw, y, w, n)  # noqa: E731
     for call, match in ((lambda: app({"m": -1}), "-1"), (lambda: app({"dtype": 3}), "dtype"), (lambda: app({"x": None}), "required"), (lambda: app({}, qw=None), "required"), (lambda: app({}, sw=at + 1), "required"),
-                        (lambda: app({}, y=at + 1), "required"), (lambda: app({"m": 20}, n=3), "workspace"), (lambda: app({"m": 20}, w=None), "workspace")):
+                        (lambda: app({}, y=at + 1), "required"), (lambda: app({"m": 20, "k": 600}, n=3), "workspace"), (lambda: app({"m": 20, "k": 600}, w=None), "workspace")):
         assert call() == -1 and match in err(), err()
     assert L.agz_linear_fp8_apply_workspace(1, -1, 1) < 0 and L.agz_linear_fp8_apply_workspace(16, 100, 100) == 0
+    assert L.agz_linear_fp8_apply_workspace(20, 100, 100) == 0 and L.agz_linear_fp8_apply_workspace(20, 100, 600) > 0
     assert L.agz_linear_fp8_forward(0, None, None, None, None, 0, 0, None, 0) == -1
     assert L.agz_linear_fp8_workspace(-1, 1, 1) < 0 and L.agz_linear_fp8_saved(1, 1, -1, 1, 1) < 0 and L.agz_linear_fp8_backward_workspace(1, 1 << 31, 1, 1, 1, 1) < 0
     assert L.agz_linear_fp8_saved(5, 6, 7, 0, 0) == 0
