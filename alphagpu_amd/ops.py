@@ -161,7 +161,8 @@ def log_probs(logits, moves=None, mask=None, target=None, top=0):
     _on_gpu(logits, "logits")
     if logits.dtype not in _CODE:
         _float_type(logits, "logits")
-    _rows(logits, "logits")
+    if logits.dim() != 2:
+        _rows(logits, "logits")
     n, a = logits.shape
     dev = logits.device
     if not 1 <= a <= 1 << 30:
