@@ -17,14 +17,16 @@ int fail(int code, const char* fmt, ...) {
 // tensors of one launch, in the kernel's arguments (no table in device memory to keep, copy or wait for): 96 x 32 bytes
 constexpr int AW_MAX = 96;
 constexpr int AW_BLOCK = 128;            // elements per scale
-struct AwTensor { void* p; const void* g; uint32_t n_lo, n_hi, chunk0, block0; };   // chunk0, block0: of this launch
+struct AwTensor { void* p; const void* g; uint32_t n_lo; uint16_t n_hi, count; uint32_t chunk0, block0; };   // count: which of AwPar's; chunk0, block0: of this launch
 struct AwTable { AwTensor t[AW_MAX]; };
+// what the number of steps that a tensor has taken comes to: tensors with equal numbers share one, and a launch has AW_COUNTS of them (most have one: no tensor missed a gradient)
+constexpr int AW_COUNTS = 16;
+struct AwCount { float step_size, inv_root; uint32_t t; };    // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 struct AwPar {
     float b1, b2, c1, c2, eps, keep;          // c1 = 1 - b1, c2 = 1 - b2; keep = 1 - lr decay
-    float step_size, inv_root;                // lr / (1 - b1^t), 1 / sqrt(1 - b2^t): of the host's t
+    AwCount c[AW_COUNTS];                     // of the host's t
     double b1d, b2d, lrd;                     // ... and what a t in device memory needs
-    const int64_t* step_dev;
-    int64_t step;
+    const int64_t *step_dev, *missed_dev;     // (missed_dev: of this launch's first tensor)
     uint32_t seed, tensor0;
     int count;
 };
@@ -111,14 +113,12 @@ __global__ __launch_bounds__(256) void k_adamw(AwTable tab, AwPar a, void* mp, v
         load4(g[k], (const G*)t.g, i, n);
         load4(p[k], (const P*)t.p, i, n);
     }
-    int64_t step = a.step;
-    float step_size = a.step_size, inv_root = a.inv_root;
+    AwCount c = a.c[t.count];
     if (a.step_dev) {
-        step = *a.step_dev;
-        step_size = (float)(a.lrd / (1.0 - aw_pow(a.b1d, step)));
-        inv_root = (float)(1.0 / sqrt(1.0 - aw_pow(a.b2d, step)));
+        const int64_t step = *a.step_dev - (a.missed_dev ? a.missed_dev[lo] : 0);
+        c = {(float)(a.lrd / (1.0 - aw_pow(a.b1d, step))), (float)(1.0 / sqrt(1.0 - aw_pow(a.b2d, step))), (uint32_t)step};
     }
-    const uint32_t key = aw_key(a.seed, (uint32_t)step, a.tensor0 + lo);
+    const uint32_t key = aw_key(a.seed, c.t, a.tensor0 + lo);
 #pragma unroll
     for (int k = 0; k < AW_TURNS; ++k) {
         const int64_t i = i0 + k * 1024;
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void k_adamw(AwTable tab, AwPar a, void* mp, v
             m[k][e] = m[k][e] * a.b1 + g[k][e] * a.c1;
             v[k][e] = v[k][e] * a.b2 + (g[k][e] * g[k][e]) * a.c2;
             r[e] = sqrtf(v[k][e]);
-            p[k][e] = p[k][e] * a.keep - (m[k][e] * step_size) / (r[e] * inv_root + a.eps);
+            p[k][e] = p[k][e] * a.keep - (m[k][e] * c.step_size) / (r[e] * c.inv_root + a.eps);
             if (BITS == 8) {
                 const uint32_t h = aw_mix((uint32_t)(i + e) ^ (key + (uint32_t)(i >> 32) * 0x9E3779B1u));
                 um[e] = h & 0xFFFFu; ur[e] = h >> 16;
@@ -162,6 +162,13 @@ __global__ __launch_bounds__(256) void k_adamw(AwTable tab, AwPar a, void* mp, v
             *(uint32_t*)((uint8_t*)vp + s0 + i) = aw_hold<true>(r, ur, vs + (s0 + i) / AW_BLOCK, first);
         }
     }
+}
+
+// one more missed step for the tensors of a launch that have no gradient
+struct AwMissing { uint32_t bit[AW_MAX / 32]; };
+__global__ __launch_bounds__(AW_MAX) void k_adamw_missed(AwMissing b, int64_t* missed) {
+    const int i = threadIdx.x;
+    if (b.bit[i >> 5] >> (i & 31) & 1) ++missed[i];
 }
 
 }  // namespace ops
@@ -191,6 +198,11 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
     if (o->bits != 8 && o->bits != 32) return fail(AGZ_ERR_ARG, "agz_adamw_step: states of %d bits (8 or 32)", o->bits);
     if (o->bits == 8 && count > 0 && (!m_scale || !v_scale)) return fail(AGZ_ERR_ARG, "agz_adamw_step: 8-bit states need their scales");
     if (!o->step_dev && o->step < 1) return fail(AGZ_ERR_ARG, "agz_adamw_step: step %lld (from 1 on)", (long long)o->step);
+    if (!o->step_dev && o->missed_dev) return fail(AGZ_ERR_ARG, "agz_adamw_step: missed_dev goes with step_dev");
+    if (!aligned(o->step_dev, 8) || !aligned(o->missed_dev, 8)) return fail(AGZ_ERR_ARG, "agz_adamw_step: step_dev and missed_dev are not aligned to 8 bytes");
+    const int64_t* missed = o->step_dev ? nullptr : o->missed;
+    if (missed) for (int i = 0; i < count; ++i)
+        if (missed[i] < 0 || missed[i] >= o->step) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d missed %lld of the %lld steps before this one", i, (long long)missed[i], (long long)o->step - 1);
     if (!(o->beta1 >= 0 && o->beta1 < 1) || !(o->beta2 >= 0 && o->beta2 < 1) || !(o->eps >= 0) || !(o->lr >= 0) || !(o->weight_decay >= 0))
         return fail(AGZ_ERR_ARG, "agz_adamw_step: lr, eps, weight_decay >= 0 and betas in [0, 1)");
     if (agz_adamw_state_elements(count, numel) < 0) return fail(AGZ_ERR_ARG, "agz_adamw_step: a negative or far too large tensor");
@@ -207,28 +219,40 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
     AwPar a{};
     a.b1 = (float)o->beta1; a.b2 = (float)o->beta2; a.c1 = (float)(1.0 - o->beta1); a.c2 = (float)(1.0 - o->beta2);
     a.eps = (float)o->eps; a.keep = (float)(1.0 - o->lr * o->weight_decay);
-    a.b1d = o->beta1; a.b2d = o->beta2; a.lrd = o->lr; a.step_dev = o->step_dev; a.step = o->step_dev ? 0 : o->step;
-    if (!o->step_dev) {
-        a.step_size = (float)(o->lr / (1.0 - std::pow(a.b1d, (double)o->step)));
-        a.inv_root = (float)(1.0 / std::sqrt(1.0 - std::pow(a.b2d, (double)o->step)));
-    }
+    a.b1d = o->beta1; a.b2d = o->beta2; a.lrd = o->lr; a.step_dev = o->step_dev;
     a.seed = o->seed;
-    // launches of at most AW_MAX tensors and AW_MOST blocks
+    // launches of at most AW_MAX tensors, AW_MOST blocks and AW_COUNTS numbers of steps
+    int64_t at[AW_COUNTS];                       // the numbers of steps of this launch (with step_dev: none)
     int i = 0;
     int64_t state_block = 0;
     while (i < count) {
         AwTable tab;
+        AwMissing missing{};
         uint32_t chunks = 0;
         const int64_t base = state_block;
-        int k = 0;
+        int k = 0, counts = 0;
         const int first = i;
         for (; i < count && k < AW_MAX; ++i) {
             const int64_t blocks = cdiv(numel[i], AW_BLOCK);
             if (k > 0 && (state_block - base) + blocks > AW_MOST) break;
-            tab.t[k++] = AwTensor{params[i], grads[i], (uint32_t)numel[i], (uint32_t)(numel[i] >> 32), chunks, (uint32_t)(state_block - base)};
+            int c = 0;
+            if (!grads[i]) missing.bit[k >> 5] |= 1u << (k & 31);
+            else if (!o->step_dev) {
+                const int64_t t = o->step - (missed ? missed[i] : 0);
+                while (c < counts && at[c] != t) ++c;
+                if (c == AW_COUNTS) break;
+                if (c == counts) {
+                    at[counts++] = t;
+                    a.c[c] = {(float)(o->lr / (1.0 - std::pow(a.b1d, (double)t))), (float)(1.0 / std::sqrt(1.0 - std::pow(a.b2d, (double)t))), (uint32_t)t};
+                }
+            }
+            tab.t[k++] = AwTensor{params[i], grads[i], (uint32_t)numel[i], (uint16_t)(numel[i] >> 32), (uint16_t)c, chunks, (uint32_t)(state_block - base)};
             chunks += grads[i] ? (uint32_t)cdiv(blocks, AW_BLOCKS) : 0;
             state_block += blocks;
         }
+        a.missed_dev = o->missed_dev ? o->missed_dev + first : nullptr;
+        if (o->missed_dev && (missing.bit[0] | missing.bit[1] | missing.bit[2]))
+            if (const int rc = launch(k_adamw_missed, dim3(1), dim3(AW_MAX), 0, stream, missing, o->missed_dev + first)) return rc;
         if (chunks == 0) continue;
         a.count = k;
         a.tensor0 = (uint32_t)(o->tensor_base + first);

@@ -52,7 +52,7 @@ class LinearFp8Args(C.Structure):                   # agz_linear_fp8_args
 class AdamWOptions(C.Structure):                    # agz_adamw_options
     _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
                 ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("seed", C.c_uint32), ("tensor_base", C.c_int32),
-                ("step", C.c_int64), ("step_dev", C.c_void_p)]
+                ("step", C.c_int64), ("step_dev", C.c_void_p), ("missed", C.c_void_p), ("missed_dev", C.c_void_p)]
 
 
 def build_library():

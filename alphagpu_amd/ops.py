@@ -407,7 +407,7 @@ def linear_fp8(x, w, bias=None, relu=False):
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # AdamW
 # ---------------------------------------------------------------------------------------------------------------------------------------
-_ADAMW = struct.Struct("=dddddiiiIi4xqq")           # agz_adamw_options
+_ADAMW = struct.Struct("=dddddiiiIi4xqqqq")           # agz_adamw_options
 assert _ADAMW.size == C.sizeof(_lib.AdamWOptions)
 
 
@@ -415,6 +415,8 @@ class AdamW:
     """AdamW (decoupled weight decay) over many tensors in one launch, in place:
 
         m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    t is the number of steps that a tensor has taken: those in which it has no gradient are not among them, and leave it as it is.
 
     params: contiguous tensors of one type on one device that do not overlap.  bits = 32: states m, v in float32.  bits = 8: m and r = sqrt(v) in
     float8_e4m3fn with one power-of-two scale per 128 elements, rounded up or down at random in proportion (from `seed`, the step and the
@@ -451,32 +453,39 @@ class AdamW:
         else:
             self.m, self.r = (torch.zeros(at, dtype=torch.uint8, device=dev).view(FP8) for _ in range(2))
             self.m_scale, self.r_scale = (torch.full((at // 128,), 127, dtype=torch.uint8, device=dev).view(E8M0) for _ in range(2))
-        self.steps = 0
+        self.steps = 0                                       # calls; a tensor's own steps are these less the ones that it missed
+        self._missed, self._any_missed = (C.c_int64 * count)(), False
         self.step_dev = torch.zeros((), dtype=torch.int64, device=dev) if capturable else None
+        self._missed_dev = torch.zeros(count, dtype=torch.int64, device=dev) if capturable else None
 
     def _buffers(self):
         return ("m", "v") if self.bits == 32 else ("m", "m_scale", "r", "r_scale")
 
     def state(self):
-        """{"step": steps taken, and the buffers of the states}: copies, for load_state."""
-        return {"step": self.steps if self.step_dev is None else int(self.step_dev.item()), **{k: getattr(self, k).clone() for k in self._buffers()}}
+        """{"step": steps taken, "missed": how many of them each tensor missed, and the buffers of the states}: copies, for load_state."""
+        step, missed = (self.steps, list(self._missed)) if self.step_dev is None else (int(self.step_dev.item()), self._missed_dev.tolist())
+        return {"step": step, "missed": missed, **{k: getattr(self, k).clone() for k in self._buffers()}}
 
     def load_state(self, state):
+        """What state() returned, of this or an equal optimiser; without "missed" no tensor has missed a step."""
+        step, missed = int(state["step"]), [int(k) for k in state.get("missed", [0] * len(self.params))]
+        _need(step >= 0 and len(missed) == len(self.params) and all(0 <= k <= step for k in missed), f"load_state: step {step}, and as many numbers of missed steps, at most {step}, as tensors ({len(self.params)})")
         for k in self._buffers():
             mine = getattr(self, k)
             _need(k in state and state[k].shape == mine.shape and state[k].dtype == mine.dtype, f"load_state: {k} has to be {mine.dtype} {list(mine.shape)}")
         for k in self._buffers():
             getattr(self, k).view(torch.uint8).copy_(state[k].view(torch.uint8))
-        self.steps = int(state["step"])
+        self.steps, self._missed[:], self._any_missed = step, missed, any(missed)
         if self.step_dev is not None:
-            self.step_dev.fill_(self.steps)
+            self.step_dev.fill_(step)
+            self._missed_dev.copy_(torch.tensor(missed, dtype=torch.int64))
 
     def zero_grad(self):
         for p in self.params:
             p.grad = None
 
     def step(self, grads=None):
-        """One step with `grads` (one per tensor, of one type; None: p.grad).  A tensor whose gradient is None is left as it is."""
+        """One step with `grads` (one per tensor, of one type; None: p.grad).  A tensor whose gradient is None is left as it is and misses the step."""
         params = self.params
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
@@ -499,15 +508,18 @@ class AdamW:
             if not g.is_contiguous():
                 g = grads[i] = g.contiguous()
             at.append(g.data_ptr())
+        missed = missed_dev = 0
         if self.step_dev is None:
             if _capturing():
                 raise RuntimeError("AdamW.step in a graph: capturable=True is needed (a replay has to count its step on the device)")
             counter = 0
+            if self._any_missed:
+                missed = C.addressof(self._missed)
         else:
             self.step_dev.add_(1)
-            counter = self.step_dev.data_ptr()
+            counter, missed_dev = self.step_dev.data_ptr(), self._missed_dev.data_ptr()
         t = self.steps + 1
-        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[own], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter)
+        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[own], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter, missed, missed_dev)
         second, ms, rs = (self.v, None, None) if self.bits == 32 else (self.r, self.m_scale, self.r_scale)
         L = _lib.load_library()
         rc = L.agz_adamw_step(device, _raw_stream(device), o, len(params), self._pointers.pack(*[p.data_ptr() for p in params]), self._pointers.pack(*at), self._numel,
@@ -516,6 +528,11 @@ class AdamW:
             _lib_call(rc, L)
         torch.autograd.graph.increment_version(params)
         self.steps = t
+        if 0 in at and self.step_dev is None:
+            for i, g in enumerate(at):
+                if not g:
+                    self._missed[i] += 1
+                    self._any_missed = True
 
 
 __all__ = ["log_probs", "LogProbs", "quantize_fp8", "matmul_fp8", "linear_fp8", "Fp8Matrix", "Fp8Weight", "AdamW", "TOP_MAX"]

@@ -350,7 +350,8 @@ int  agz_linear_fp8_backward(int device, void *stream, const agz_linear_fp8_args
  * held in e4m3 with one power-of-two scale (e8m0 byte, as in agz_fp8_quantize) per 128 elements and rounded up or down at random in
  * proportion (unbiased: to the nearest, v could no longer shrink, its steps of 1 - b2 are below half a rounding step); r is 0 only where v is.
  * The random bits are a hash of (seed, t, tensor index + tensor_base, element): equal arguments give equal results.
- * A tensor whose gradient is NULL is left as it is, its states too.  Tensors must not overlap; each has at most 2^34 elements. */
+ * A tensor whose gradient is NULL is left as it is, its states too, and the step is none of its own: its t is the call's less the number of steps that it missed, so
+ * that moments that begin late are corrected as those of the first steps are.  Tensors must not overlap; each has at most 2^34 elements. */
 typedef struct {
     double lr, beta1, beta2, eps, weight_decay;
     int32_t param_dtype, grad_dtype;   /* agz_dtype */
@@ -359,6 +360,8 @@ typedef struct {
     int32_t tensor_base;
     int64_t step;                      /* t of this step, from 1 on; ignored where step_dev is given */
     const int64_t *step_dev;           /* t in device memory, read when the step runs (graph replays); NULL: `step` */
+    const int64_t *missed;             /* [count], host: steps before this one that each tensor missed; NULL: none (not read with step_dev) */
+    int64_t *missed_dev;               /* [count], device, 8-byte aligned, with step_dev: the same; the call adds one where the gradient is NULL.  NULL: none */
 } agz_adamw_options;
 int64_t agz_adamw_state_elements(int count, const int64_t *numel);
 int  agz_adamw_step(int device, void *stream, const agz_adamw_options *opt, int count, void *const *params, const void *const *grads, const int64_t *numel,

@@ -339,3 +339,118 @@ def test_refusals_without_a_gpu():
     refused("aligned", g=at + 2)
     assert L.agz_adamw_step(0, None, None, 0, None, None, None, None, None, None, None) == -1
     assert L.agz_adamw_state_elements(3, (C.c_int64 * 3)(1, 0, 129)) == 384 and L.agz_adamw_state_elements(1, (C.c_int64 * 1)(-1)) == -1
+
+
+def late_tensors(calls, capturable=False, bits=32, dense=False, state_at=None, device="cuda"):
+    """40 tensors over `calls` calls: tensor i has a gradient from call i on, odd ones not at every fifth call after that; -> weights and optimiser.  dense: every
+    tensor has the same gradients one call after the other from the first call on, and none behind its last."""
+    sizes = [37 * i % 300 + 1 for i in range(40)]
+    r = torch.Generator().manual_seed(9)
+    ps = [torch.randn(n, generator=r).to(device) for n in sizes]
+    make = lambda: ops.AdamW(ps, bits=bits, seed=3, capturable=capturable, **HYPER)  # noqa: E731
+    opt = make()
+    has = [[c >= i and not (i % 2 and (c - i) % 5 == 4) for c in range(calls)] for i in range(40)]
+    grad = lambda i, k: torch.randn(sizes[i], generator=torch.Generator().manual_seed(100 * i + k)).to(device)  # noqa: E731
+    for c in range(calls):
+        opt.step([(grad(i, c) if c < sum(has[i]) else None) if dense else (grad(i, sum(has[i][:c])) if has[i][c] else None) for i in range(40)])
+        if c == state_at:
+            kept = opt.state()
+            opt = make()
+            opt.load_state(kept)
+    return ps, opt
+
+
+def same_states(one, two):
+    return all(torch.equal(getattr(one, k).view(torch.uint8), getattr(two, k).view(torch.uint8)) for k in one._buffers())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_counts_its_own_steps(bits):
+    """What a tensor's steps are depends on the gradients that it had, not on the calls in which it had none: bit for bit the same, with up to 40 different numbers
+    of steps in a call, with the numbers on the device, and from a saved state on."""
+    want, dense = late_tensors(43, bits=bits, dense=True)
+    for form in (dict(), dict(capturable=True), dict(state_at=20), dict(state_at=20, capturable=True)):
+        got, opt = late_tensors(43, bits=bits, **form)
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and same_states(opt, dense), form
+        assert opt.state()["step"] == 43 and opt.state()["missed"][:4] == [0, 1 + 8, 2, 3 + 8], form
+
+
+@pytest.mark.gpu
+def test_a_late_tensor_against_64_bits():
+    """A tensor that gets its first gradient in the 51st call takes the first step of its own, and one that then misses a call the second in the 53rd; calls without
+    any gradient count for nobody."""
+    p = torch.randn(300, generator=torch.Generator().manual_seed(1))
+    gs = [torch.randn(300, generator=torch.Generator().manual_seed(k)) for k in (2, 3)]
+    first, late = torch.randn(5, device="cuda"), p.cuda()
+    opt = ops.AdamW([first, late], **HYPER)
+    for c in range(50):
+        opt.step([torch.ones(5, device="cuda") if c % 3 else None, None])
+    m = v = torch.zeros(300, dtype=torch.float64)
+    want = p
+    for t, g in enumerate(gs, 1):
+        opt.step([None, g.cuda()])
+        (want, m, v), (tp, _, _) = step64(want, g, m, v, t, **HYPER)
+        # the states held in 32 bits are what the next step begins with
+        assert ((late.cpu().double() - want).abs() <= tp + E32 * want.abs()).all(), t
+        want, m, v = late.cpu().clone(), opt.m[128:428].cpu().clone(), opt.v[128:428].cpu().clone()
+        opt.step([first, None])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_missing_gradients_in_a_graph(bits):
+    """Two graphs of one optimiser, one with a gradient of every tensor and one without the second's, replayed in turns, against a host that counts."""
+    sizes = [200, 131, 50]
+    start = [torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda() for n in sizes]
+    ps, qs = [p.clone() for p in start], [p.clone() for p in start]
+    one, two = ops.AdamW(ps, bits=bits, capturable=True, **HYPER), ops.AdamW(qs, bits=bits, **HYPER)
+    grads = [torch.randn(n, generator=torch.Generator().manual_seed(n + 1)).cuda() for n in sizes]
+    some = [grads[0], None, grads[2]]
+    one.step(some)
+    two.step(some)
+    torch.cuda.synchronize()
+    graphs = []
+    for g in (grads, some):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            one.step(g)
+        graphs.append((graph, g))
+    for k in (1, 0, 0, 1, 1, 0):
+        graph, g = graphs[k]
+        graph.replay()
+        torch.cuda.synchronize()
+        two.step(g)
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and same_states(one, two)
+    one.step(grads)
+    two.step(grads)
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    a, b = one.state(), two.state()
+    assert a["step"] == b["step"] == 8 and a["missed"] == b["missed"] == [0, 4, 0]
+
+
+@pytest.mark.gpu
+def test_states_of_other_lengths_are_refused():
+    p = torch.randn(10, device="cuda")
+    opt = ops.AdamW([p])
+    good = opt.state()
+    for bad in ([], [0, 0], [-1], [5]):
+        with pytest.raises(ValueError, match="load_state"):
+            opt.load_state({**good, "step": 4, "missed": bad})
+    opt.load_state({k: v for k, v in good.items() if k != "missed"})
+    assert opt.state()["missed"] == [0]
+
+
+def test_counts_are_refused_without_a_gpu():
+    L = lib.load_library()
+    buf = (C.c_char * 4096)()
+    at = (C.addressof(buf) + 63) // 64 * 64
+    good = dict(lr=0.1, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, param_dtype=0, grad_dtype=0, bits=32, seed=0, tensor_base=0, step=3, step_dev=None)
+    for missed, grad in ((-1, at), (3, at), (4, None)):
+        held = (C.c_int64 * 1)(missed)
+        o = lib.AdamWOptions(**good, missed=C.addressof(held))
+        assert L.agz_adamw_step(0, None, C.byref(o), 1, (C.c_void_p * 1)(at), (C.c_void_p * 1)(grad), (C.c_int64 * 1)(4), at, at, None, None) == -1
+        assert "missed" in L.agz_ops_last_error().decode()
+    o = lib.AdamWOptions(**good, missed_dev=at)                     # a count on the device belongs to a step on the device
+    assert L.agz_adamw_step(0, None, C.byref(o), 1, (C.c_void_p * 1)(at), (C.c_void_p * 1)(at), (C.c_int64 * 1)(4), at, at, None, None) == -1
+    assert "missed_dev" in L.agz_ops_last_error().decode()
