@@ -411,6 +411,11 @@ _ADAMW = struct.Struct("=dddddiiiIi4xqqqq")           # agz_adamw_options
 assert _ADAMW.size == C.sizeof(_lib.AdamWOptions)
 
 
+def _check_adamw(lr, betas, eps, weight_decay):
+    if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and len(betas) == 2 and all(0 <= b < 1 for b in betas)):
+        raise ValueError(f"lr, eps, weight_decay >= 0 and two betas in [0, 1) are needed, not {lr}, {eps}, {weight_decay}, {betas}")
+
+
 class AdamW:
     """AdamW (decoupled weight decay) over many tensors in one launch, in place:
 
@@ -428,7 +433,7 @@ class AdamW:
         self.params = list(params)
         _need(self.params, "params: none")
         _need(bits in (8, 32), f"bits: 8 or 32, not {bits!r}")
-        _need(lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas), "lr, eps, weight_decay >= 0 and betas in [0, 1) are needed")
+        _check_adamw(lr, betas, eps, weight_decay)
         dev, kind, ends = self.params[0].device if isinstance(self.params[0], torch.Tensor) else None, None, []
         for i, p in enumerate(self.params):
             _on_gpu(p, f"params[{i}]", dev)
@@ -490,6 +495,7 @@ class AdamW:
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} tensors")
+        _check_adamw(self.lr, self.betas, self.eps, self.weight_decay)
         kind, own, device, at = None, self.dtype, self.device.index, []
         for i, (p, g, shape) in enumerate(zip(params, grads, self._shapes)):
             if p.shape != shape or p.get_device() != device or p.dtype is not own or not p.is_contiguous():
@@ -516,10 +522,11 @@ class AdamW:
             if self._any_missed:
                 missed = C.addressof(self._missed)
         else:
-            self.step_dev.add_(1)
             counter, missed_dev = self.step_dev.data_ptr(), self._missed_dev.data_ptr()
         t = self.steps + 1
         o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[own], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter, missed, missed_dev)
+        if counter:
+            self.step_dev.add_(1)                            # (behind everything that can refuse the call)
         second, ms, rs = (self.v, None, None) if self.bits == 32 else (self.r, self.m_scale, self.r_scale)
         L = _lib.load_library()
         rc = L.agz_adamw_step(device, _raw_stream(device), o, len(params), self._pointers.pack(*[p.data_ptr() for p in params]), self._pointers.pack(*at), self._numel,

@@ -454,3 +454,23 @@ def test_counts_are_refused_without_a_gpu():
     o = lib.AdamWOptions(**good, missed_dev=at)                     # a count on the device belongs to a step on the device
     assert L.agz_adamw_step(0, None, C.byref(o), 1, (C.c_void_p * 1)(at), (C.c_void_p * 1)(at), (C.c_int64 * 1)(4), at, at, None, None) == -1
     assert "missed_dev" in L.agz_ops_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_counts_nothing(capturable):
+    p, g = torch.randn(300, device="cuda"), torch.randn(300, device="cuda")
+    opt = ops.AdamW([p], capturable=capturable, **HYPER)
+    opt.step([g])
+    before = p.clone()
+    for name, bad in (("lr", -1.0), ("lr", math.nan), ("betas", (0.9, 1.0)), ("betas", (math.nan, 0.9)), ("betas", (0.9,)), ("eps", -1.0), ("weight_decay", math.nan)):
+        good = getattr(opt, name)
+        setattr(opt, name, bad)
+        with pytest.raises(ValueError, match="needed"):
+            opt.step([g])
+        setattr(opt, name, good)
+        assert opt.state()["step"] == opt.steps == 1 and torch.equal(p, before), name
+    with pytest.raises(ValueError, match="betas"):
+        ops.AdamW([p], betas=(0.9, 0.99, 0.999))
+    opt.step([g])
+    assert opt.state()["step"] == opt.steps == 2 and not torch.equal(p, before)
