@@ -6,7 +6,7 @@
 
 The reference does this in Flux (train.jl:12-15, :50; DenseNet.jl:161-198).  Tensors are torch tensors on a GPU; the work runs on the current
 stream of their device, nothing waits for it, and it can be captured into a graph.  Wrong arguments raise ValueError before anything is
-queued, errors of the library AgzError.  There is no CPU path.  A backward pass that is captured into a graph needs leaves of its own
+queued, errors of the library AgzError.  There is no CPU path, and no forward-mode rule (a tangent is refused).  A backward pass that is captured into a graph needs leaves of its own
 (detach().requires_grad_(), and autograd.grad): gradients that another, living autograd graph accumulates into the same leaves are torch's to order.
 """
 import ctypes as C
@@ -15,6 +15,7 @@ import struct
 from collections import namedtuple
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch._C import _cuda_getCurrentRawStream as _raw_stream     # the current stream's handle without a Stream object around it
 from torch._C import _cuda_isCurrentStreamCapturing as _capturing
 
@@ -54,6 +55,13 @@ def _rows(t, name):
     if t.shape[1] > 1 and t.stride(1) != 1 and t.numel():
         raise ValueError(f"{name}: the columns of a row have to lie next to each other (stride {t.stride(1)}): use contiguous()")
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _no_tangent(**tensors):
+    """Refuses tensors that carry a forward-mode derivative (called where a level is open)."""
+    for name, t in tensors.items():
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name}: no derivatives in forward mode (give the primal, without a tangent)")
 
 
 def _ptr(t):
@@ -189,6 +197,8 @@ def log_probs(logits, moves=None, mask=None, target=None, top=0):
             raise ValueError(f"target: float32 [{n}, {a}], not {target.dtype} {list(target.shape)}")
         if target.requires_grad:
             raise ValueError("target: a constant is needed (detach() it)")
+    if _forward_ad._current_level >= 0:
+        _no_tangent(logits=logits, target=target)
     head = _log_probs_head(logits, moves, mask, target, top)
     if logits.requires_grad and torch.is_grad_enabled():
         return LogProbs(*_LogProbs.apply(logits, head, (moves, mask, target, top)))
@@ -282,6 +292,8 @@ def matmul_fp8(a, b, bias=None, relu=False, dtype=torch.bfloat16):
     _need(a.q.device == b.q.device, "a and b are on different devices")
     _need(dtype in _CODE, f"dtype: float32, bfloat16 or float16, not {dtype}")
     _check_bias(bias, b.rows, a.q.device)
+    if _forward_ad._current_level >= 0:
+        _no_tangent(bias=bias)
     with torch.no_grad():
         return _product(a, b, None if bias is None else bias.detach(), relu, dtype)
 
@@ -392,6 +404,8 @@ def linear_fp8(x, w, bias=None, relu=False):
     if x.shape[-1] != k:
         raise ValueError(f"x has {x.shape[-1]} columns, w {k}")
     _check_bias(bias, n, dev)
+    if _forward_ad._current_level >= 0:
+        _no_tangent(x=x, w=None if ready else w, bias=bias)
     two = x if x.dim() == 2 else x.reshape(-1, k)
     _rows(two, "x")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not ready and w.requires_grad)):

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from alphagpu_amd import lib, ops
 
@@ -417,3 +418,18 @@ def test_refusals_without_a_gpu():
     assert L.agz_linear_fp8_saved(5, 6, 7, 0, 0) == 0
     assert L.agz_fp8_pitch(-1) == -1 and L.agz_fp8_pitch(129) == 256 and L.agz_fp8_scale_pitch(129) == 4 and L.agz_fp8_scale_pitch(513) == 8
     assert L.agz_fp8_matmul_workspace(-1, 1, 1) < 0 and L.agz_fp8_colsum_ws(-1, 1) < 0
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    """There is no forward-mode rule: a tangent of any argument is refused, never dropped; without one a level that is open changes nothing."""
+    x, w, b = torch.randn(4, 64, device="cuda"), torch.randn(8, 64, device="cuda"), torch.randn(8, device="cuda")
+    ready = ops.Fp8Weight(w)
+    want = ops.linear_fp8(x, w, b)
+    with fwd.dual_level():
+        d, dw, db = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, w, b))
+        for bad in (lambda: ops.linear_fp8(d, w, b), lambda: ops.linear_fp8(x, dw, b), lambda: ops.linear_fp8(x, w, db), lambda: ops.linear_fp8(d, ready), lambda: ops.linear_fp8(x, ready, db),
+                    lambda: ops.linear_fp8(d.view(2, 2, 64), w), lambda: ops.matmul_fp8(ops.quantize_fp8(x), ready.matrix, db)):
+            with pytest.raises(ValueError, match="forward mode"):
+                bad()
+        assert torch.equal(ops.linear_fp8(x, w, b), want) and torch.equal(ops.linear_fp8(x, ready, b), want)

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 import torch.utils.checkpoint
 
 from alphagpu_amd import lib, ops
@@ -495,3 +496,26 @@ def test_refusals_without_a_gpu():
     refused("without alternatives", back, (None, None, None, at, at, 4))
     assert L.agz_logprob_workspace(-1, 4, 0) < 0 and L.agz_logprob_workspace(1, 4, 33) < 0
     assert L.agz_logprob_forward(0, None, None) == -1
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    """There is no forward-mode rule: a tangent is refused, never dropped; without one, or where forward mode is off, a level that is open changes nothing."""
+    x, t = torch.randn(4, 9, device="cuda"), torch.rand(4, 9, device="cuda")
+    want = ops.log_probs(x, target=t)
+    with fwd.dual_level():
+        d, dt = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(t, torch.ones_like(t))
+        with pytest.raises(ValueError, match="forward mode"):
+            ops.log_probs(d)
+        with pytest.raises(ValueError, match="forward mode"):
+            ops.log_probs(x, target=dt)
+        with torch.no_grad(), pytest.raises(ValueError, match="forward mode"):      # (no_grad is about the other mode)
+            ops.log_probs(d, top=2)
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.log_probs(fwd.make_dual(x.clone().requires_grad_(), torch.ones_like(x)))
+        got = ops.log_probs(x, target=t)
+        assert torch.equal(got.entropy, want.entropy) and torch.equal(got.target, want.target)
+        plain = ops.log_probs(fwd.unpack_dual(d).primal)
+        assert torch.equal(plain.entropy, want.entropy)
+        with fwd._set_fwd_grad_enabled(False):                     # (as within the forward of a function that has a rule of its own)
+            assert torch.equal(ops.log_probs(d).entropy, want.entropy)
