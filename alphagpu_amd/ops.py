@@ -1,7 +1,8 @@
 """Operators on device tensors: what a network learns with (include/agz.h "operators on tensors in DEVICE memory").
 
     log_probs(logits, moves, ...)            log probabilities of given moves, entropy, best alternatives, expected log probability; differentiable
-    quantize_fp8, matmul_fp8, linear_fp8     matrices in 8 bits with a scale for each block of 128, and their products; differentiable
+    linear_fp8                               a layer with its product in 8 bits, a scale for each block of 128; differentiable
+    quantize_fp8, matmul_fp8                 matrices in 8 bits and their products by themselves; without gradients
     AdamW                                    one step over many tensors, states in 32 or 8 bits
 
 The reference does this in Flux (train.jl:12-15, :50; DenseNet.jl:161-198).  Tensors are torch tensors on a GPU; the work runs on the current
@@ -257,7 +258,7 @@ def _quantize(x, block_rows, straight, transposed, gate=None, colsum=False):
 def quantize_fp8(x, block_rows=1, transposed=False):
     """x [rows, cols] (float32, bfloat16 or float16) -> Fp8Matrix, of x or (transposed) of its transpose, with one scale per block of
     block_rows (1, or 128 for weights) x 128 along the columns of the result.  Scales are the smallest powers of two with |x| <= 448 scale; NaN
-    and infinities become NaN."""
+    and infinities become NaN.  No gradient passes: what is held in 8 bits is a constant."""
     _on_gpu(x, "x")
     _float_type(x, "x")
     _need(block_rows in (1, 128), f"block_rows: 1 or 128, not {block_rows!r}")
@@ -286,12 +287,14 @@ def _check_bias(bias, n, dev):
 
 
 def matmul_fp8(a, b, bias=None, relu=False, dtype=torch.bfloat16):
-    """relu?(a b^T + bias) of two Fp8Matrix with the same number of columns: [a.rows, b.rows] in `dtype`; sums in 32 bits, rounded once."""
+    """relu?(a b^T + bias) of two Fp8Matrix with the same number of columns: [a.rows, b.rows] in `dtype`; sums in 32 bits, rounded once.
+    No gradient passes, so a bias that wants one is refused (linear_fp8 has one)."""
     _need(isinstance(a, Fp8Matrix) and isinstance(b, Fp8Matrix), "a and b: Fp8Matrix (quantize_fp8) are needed")
     _need(a.cols == b.cols, f"a has {a.cols} columns, b {b.cols}")
     _need(a.q.device == b.q.device, "a and b are on different devices")
     _need(dtype in _CODE, f"dtype: float32, bfloat16 or float16, not {dtype}")
     _check_bias(bias, b.rows, a.q.device)
+    _need(bias is None or not (bias.requires_grad and torch.is_grad_enabled()), "bias: a constant is needed (detach() it; linear_fp8 has gradients)")
     if _forward_ad._current_level >= 0:
         _no_tangent(bias=bias)
     with torch.no_grad():

@@ -433,3 +433,14 @@ def test_forward_mode_derivatives_are_refused():
             with pytest.raises(ValueError, match="forward mode"):
                 bad()
         assert torch.equal(ops.linear_fp8(x, w, b), want) and torch.equal(ops.linear_fp8(x, ready, b), want)
+
+
+@pytest.mark.gpu
+def test_a_product_without_gradients_refuses_a_bias_that_wants_one():
+    x, w = matrix(torch.randn(4, 64)), matrix(torch.randn(8, 64), 128)
+    b = torch.randn(8, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="linear_fp8"):
+        ops.matmul_fp8(x, w, b)
+    want = ops.matmul_fp8(x, w, b.detach())
+    with torch.no_grad():
+        assert torch.equal(ops.matmul_fp8(x, w, b), want)
