@@ -221,8 +221,9 @@ class Fp8Matrix:
 
     def dequantize(self):
         """The values it stands for, in float32."""
-        s = self.scale.float()[:, :self.q.shape[1] // 128]
-        return (self.q.float().view(self.rows, -1, 128) * s[:, :, None]).view(self.rows, -1)[:, :self.cols]
+        pitch = self.q.shape[1]
+        s = self.scale.float()[:, :pitch // 128]
+        return (self.q.float().view(self.rows, pitch // 128, 128) * s[:, :, None]).view(self.rows, pitch)[:, :self.cols]
 
     @classmethod
     def of(cls, q, scale, rows, cols):

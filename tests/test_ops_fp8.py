@@ -444,3 +444,18 @@ def test_a_product_without_gradients_refuses_a_bias_that_wants_one():
     want = ops.matmul_fp8(x, w, b.detach())
     with torch.no_grad():
         assert torch.equal(ops.matmul_fp8(x, w, b), want)
+
+
+def test_an_empty_matrix_stands_for_no_values():
+    for rows, cols in ((0, 128), (0, 0), (0, 5), (3, 0)):
+        got = ops.Fp8Matrix(rows, cols, "cpu").dequantize()
+        assert got.shape == (rows, cols) and got.dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_quantizing_nothing():
+    for rows, cols in ((0, 128), (0, 0), (0, 5), (3, 0)):
+        for block in (1, 128):
+            x = torch.empty(rows, cols, device="cuda")
+            assert ops.quantize_fp8(x, block).dequantize().shape == (rows, cols)
+            assert ops.quantize_fp8(x, block, transposed=True).dequantize().shape == (cols, rows)
