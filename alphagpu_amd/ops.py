@@ -12,6 +12,7 @@ queued, errors of the library AgzError.  There is no CPU path, and no forward-mo
 """
 import ctypes as C
 import functools
+import math
 import struct
 from collections import namedtuple
 
@@ -410,7 +411,7 @@ def linear_fp8(x, w, bias=None, relu=False):
     _check_bias(bias, n, dev)
     if _forward_ad._current_level >= 0:
         _no_tangent(x=x, w=None if ready else w, bias=bias)
-    two = x if x.dim() == 2 else x.reshape(-1, k)
+    two = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), k)
     _rows(two, "x")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not ready and w.requires_grad)):
         _need(not ready, "w: gradients need the weights themselves, not Fp8Weight")

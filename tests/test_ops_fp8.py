@@ -459,3 +459,16 @@ def test_quantizing_nothing():
             x = torch.empty(rows, cols, device="cuda")
             assert ops.quantize_fp8(x, block).dequantize().shape == (rows, cols)
             assert ops.quantize_fp8(x, block, transposed=True).dequantize().shape == (cols, rows)
+
+
+@pytest.mark.gpu
+def test_more_dimensions_with_nothing_to_sum():
+    """x [..., 0]: the bias alone, and gradients of nothing, with any number of dimensions."""
+    b = torch.arange(4.0, device="cuda")
+    for shape in ((2, 3, 0), (0,), (2, 0, 0), (5, 0)):
+        x, w, lb = torch.empty(shape, device="cuda", requires_grad=True), torch.empty(4, 0, device="cuda", requires_grad=True), b.clone().requires_grad_()
+        y = ops.linear_fp8(x, w, lb, relu=True)
+        assert y.shape == (*shape[:-1], 4) and torch.equal(y, b.expand_as(y))
+        assert torch.equal(ops.linear_fp8(x.detach(), ops.Fp8Weight(w.detach()), b), y)
+        dx, dw, db = torch.autograd.grad([y], [x, w, lb], [torch.ones_like(y)])
+        assert dx.shape == shape and dw.shape == (4, 0) and torch.equal(db, y.new_tensor([0.0, 1, 1, 1]) * (y.numel() // 4))
