@@ -272,8 +272,10 @@ def quantize_fp8(x, block_rows=1, transposed=False):
 def _product(a, b, bias, relu, dtype):
     L = _lib.load_library()
     dev = a.q.device
-    out = torch.empty((a.rows, b.rows), dtype=dtype, device=dev)
     need = L.agz_fp8_matmul_workspace(a.rows, b.rows, a.cols)
+    if need < 0:
+        raise ValueError(f"matmul_fp8: {a.rows} x {b.rows} x {a.cols} is too large")
+    out = torch.empty((a.rows, b.rows), dtype=dtype, device=dev)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib_call(L.agz_fp8_matmul(dev.index, _raw_stream(dev.index), a.rows, b.rows, a.cols, a.q.data_ptr(), a.scale.data_ptr(), b.q.data_ptr(), b.scale.data_ptr(),
                                _ptr(bias), 0 if bias is None else _CODE[bias.dtype], int(relu), out.data_ptr(), _CODE[dtype], max(b.rows, 1), _ptr(ws), need), L)

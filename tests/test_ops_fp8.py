@@ -472,3 +472,10 @@ def test_more_dimensions_with_nothing_to_sum():
         assert torch.equal(ops.linear_fp8(x.detach(), ops.Fp8Weight(w.detach()), b), y)
         dx, dw, db = torch.autograd.grad([y], [x, w, lb], [torch.ones_like(y)])
         assert dx.shape == shape and dw.shape == (4, 0) and torch.equal(db, y.new_tensor([0.0, 1, 1, 1]) * (y.numel() // 4))
+
+
+@pytest.mark.gpu
+def test_a_product_that_is_too_deep_is_refused_by_name():
+    q = ops.quantize_fp8(torch.zeros(1, 1 << 24, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError, match="too large"):
+        ops.matmul_fp8(q, q)
