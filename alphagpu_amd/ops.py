@@ -237,26 +237,6 @@ class Fp8Matrix:
         return m
 
 
-def _quantize(x, block_rows, straight, transposed, gate=None, colsum=False):
-    """(x in 8 bits or None, its transpose in 8 bits or None, column sums or None) of x [rows, cols]."""
-    L = _lib.load_library()
-    dev = x.device
-    ld = _rows(x, "x")
-    r, c = x.shape
-    a = Fp8Matrix(r, c, dev) if straight else None
-    t = Fp8Matrix(c, r, dev) if transposed else None
-    sums = ws = None
-    need = 0
-    if colsum:
-        sums = torch.empty(c, dtype=torch.float32, device=dev)
-        need = L.agz_fp8_colsum_ws(r, c)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    _lib_call(L.agz_fp8_quantize(dev.index, _raw_stream(dev.index), x.data_ptr(), _CODE[x.dtype], r, c, ld, _ptr(gate), block_rows,
-                                 a and a.q.data_ptr() or None, a and a.scale.data_ptr() or None, t and t.q.data_ptr() or None, t and t.scale.data_ptr() or None,
-                                 _ptr(sums), _ptr(ws), need), L)
-    return a, t, sums
-
-
 def quantize_fp8(x, block_rows=1, transposed=False):
     """x [rows, cols] (float32, bfloat16 or float16) -> Fp8Matrix, of x or (transposed) of its transpose, with one scale per block of
     block_rows (1, or 128 for weights) x 128 along the columns of the result.  Scales are the smallest powers of two with |x| <= 448 scale; NaN
@@ -264,9 +244,13 @@ def quantize_fp8(x, block_rows=1, transposed=False):
     _on_gpu(x, "x")
     _float_type(x, "x")
     _need(block_rows in (1, 128), f"block_rows: 1 or 128, not {block_rows!r}")
-    with torch.no_grad():
-        a, t, _ = _quantize(x.detach(), block_rows, not transposed, bool(transposed))
-    return t if transposed else a
+    L, dev, ld = _lib.load_library(), x.device, _rows(x, "x")
+    r, c = x.shape
+    q = Fp8Matrix(c, r, dev) if transposed else Fp8Matrix(r, c, dev)
+    at = (q.q.data_ptr(), q.scale.data_ptr())
+    _lib_call(L.agz_fp8_quantize(dev.index, _raw_stream(dev.index), x.data_ptr(), _CODE[x.dtype], r, c, ld, None, block_rows,
+                                 *((None, None, *at) if transposed else (*at, None, None)), None, None, 0), L)
+    return q
 
 
 def _product(a, b, bias, relu, dtype):

@@ -479,3 +479,37 @@ def test_a_product_that_is_too_deep_is_refused_by_name():
     q = ops.quantize_fp8(torch.zeros(1, 1 << 24, dtype=torch.bfloat16, device="cuda"))
     with pytest.raises(ValueError, match="too large"):
         ops.matmul_fp8(q, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("block", [1, 128])
+def test_gate_and_column_sums(block, dtype):
+    """agz_fp8_quantize with a gate and column sums, both ways and each way alone: entries behind a gate that is not above 0 (NaN is not) count as 0, whatever they are; sums of what is
+    left, rows x half a step of 32 bits of the sum of their sizes off at most; few columns, odd ends, rows of a wider tensor."""
+    L = lib.load_library()
+    for rows, cols in ((1, 1), (3, 5), (130, 7), (128, 128), (129, 131), (300, 515), (40, 8)):
+        x, gate = data(rows, cols, dtype, 30), torch.randn(rows, cols, generator=torch.Generator().manual_seed(31)).to(dtype)
+        gate[0, 0] = math.nan
+        if rows > 2:
+            gate[2, cols - 1], gate[1, 0], x[2, cols - 1], x[1, 0] = -1.0, 0.0, math.nan, math.inf      # (closed, with NaN and infinity behind)
+        wide = torch.full((2, rows, cols + 3), math.nan, dtype=dtype, device="cuda")
+        wide[0, :, 1:cols + 1], wide[1, :, 1:cols + 1] = x.cuda(), gate.cuda()
+        xs, gs = wide[0, :, 1:cols + 1], wide[1, :, 1:cols + 1]
+        passed = torch.where(gate > 0, x, torch.zeros_like(x))
+        straight = blocks(passed, block)[0]
+        across = blocks(passed.t(), 1)[0] if block == 1 else straight.t()
+        for both in ((True, True), (True, False), (False, True)):
+            a, t = ops.Fp8Matrix(rows, cols, "cuda") if both[0] else None, ops.Fp8Matrix(cols, rows, "cuda") if both[1] else None
+            sums = torch.full((cols,), math.nan, device="cuda") if both[1] else None
+            ws = torch.empty(L.agz_fp8_colsum_ws(rows, cols), dtype=torch.uint8, device="cuda")
+            at = lambda m, k: getattr(m, k).data_ptr() if m is not None else None  # noqa: E731
+            rc = L.agz_fp8_quantize(0, torch.cuda.current_stream().cuda_stream, xs.data_ptr(), ops._CODE[dtype], rows, cols, cols + 3, gs.data_ptr(), block,
+                                    at(a, "q"), at(a, "scale"), at(t, "q"), at(t, "scale"), sums.data_ptr() if both[1] else None, ws.data_ptr(), ws.numel())
+            assert rc == 0, L.agz_ops_last_error()
+            if both[0]:
+                assert torch.equal(a.dequantize().double().cpu(), straight) and not a.q.view(torch.uint8)[:, cols:].any()
+            if both[1]:
+                assert torch.equal(t.dequantize().double().cpu(), across) and not t.q.view(torch.uint8)[:, rows:].any()
+                d = passed.double()
+                assert ((sums.double().cpu() - d.sum(0)).abs() <= rows * 2.0 ** -24 * d.abs().sum(0)).all()
