@@ -538,9 +538,12 @@ class AdamW:
                               self.m.data_ptr(), second.data_ptr(), _ptr(ms), _ptr(rs))
         if rc:
             _lib_call(rc, L)
-        torch.autograd.graph.increment_version(params)
         self.steps = t
-        if 0 in at and self.step_dev is None:
+        if 0 not in at:
+            torch.autograd.graph.increment_version(params)
+            return
+        torch.autograd.graph.increment_version([p for p, g in zip(params, at) if g])
+        if self.step_dev is None:
             for i, g in enumerate(at):
                 if not g:
                     self._missed[i] += 1

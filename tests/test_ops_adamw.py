@@ -474,3 +474,12 @@ def test_a_refused_step_counts_nothing(capturable):
         ops.AdamW([p], betas=(0.9, 0.99, 0.999))
     opt.step([g])
     assert opt.state()["step"] == opt.steps == 2 and not torch.equal(p, before)
+
+
+@pytest.mark.gpu
+def test_a_tensor_without_a_gradient_stays_unchanged_for_autograd():
+    p, q = torch.randn(10, device="cuda", requires_grad=True), torch.randn(10, device="cuda", requires_grad=True)
+    y = (q * q).sum()
+    ops.AdamW([p, q], **HYPER).step([torch.ones(10, device="cuda"), None])
+    y.backward()
+    assert torch.equal(q.grad, 2 * q.detach())
