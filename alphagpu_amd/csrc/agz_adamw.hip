@@ -193,10 +193,13 @@ int64_t agz_adamw_state_elements(int count, const int64_t* numel) {
 int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int count, void* const* params, const void* const* grads, const int64_t* numel,
                    void* m, void* v, void* m_scale, void* v_scale) {
     if (!o) return fail(AGZ_ERR_ARG, "agz_adamw_step: no options");
-    if (count < 0 || (count > 0 && (!params || !grads || !numel || !m || !v))) return fail(AGZ_ERR_ARG, "agz_adamw_step: null argument");
+    if (count < 0 || (count > 0 && (!params || !grads || !numel))) return fail(AGZ_ERR_ARG, "agz_adamw_step: null argument");
     if (!good_dtype(o->param_dtype) || !good_dtype(o->grad_dtype)) return fail(AGZ_ERR_ARG, "agz_adamw_step: unknown dtype");
     if (o->bits != 8 && o->bits != 32) return fail(AGZ_ERR_ARG, "agz_adamw_step: states of %d bits (8 or 32)", o->bits);
-    if (o->bits == 8 && count > 0 && (!m_scale || !v_scale)) return fail(AGZ_ERR_ARG, "agz_adamw_step: 8-bit states need their scales");
+    const int64_t elements = agz_adamw_state_elements(count, numel);
+    if (elements < 0) return fail(AGZ_ERR_ARG, "agz_adamw_step: a negative or far too large tensor");
+    if (elements > 0 && (!m || !v)) return fail(AGZ_ERR_ARG, "agz_adamw_step: null argument");
+    if (o->bits == 8 && elements > 0 && (!m_scale || !v_scale)) return fail(AGZ_ERR_ARG, "agz_adamw_step: 8-bit states need their scales");
     if (!o->step_dev && o->step < 1) return fail(AGZ_ERR_ARG, "agz_adamw_step: step %lld (from 1 on)", (long long)o->step);
     if (!o->step_dev && o->missed_dev) return fail(AGZ_ERR_ARG, "agz_adamw_step: missed_dev goes with step_dev");
     if (!aligned(o->step_dev, 8) || !aligned(o->missed_dev, 8)) return fail(AGZ_ERR_ARG, "agz_adamw_step: step_dev and missed_dev are not aligned to 8 bytes");
@@ -205,8 +208,7 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
         if (missed[i] < 0 || missed[i] >= o->step) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d missed %lld of the %lld steps before this one", i, (long long)missed[i], (long long)o->step - 1);
     if (!(o->beta1 >= 0 && o->beta1 < 1) || !(o->beta2 >= 0 && o->beta2 < 1) || !(o->eps >= 0) || !(o->lr >= 0) || !(o->weight_decay >= 0))
         return fail(AGZ_ERR_ARG, "agz_adamw_step: lr, eps, weight_decay >= 0 and betas in [0, 1)");
-    if (agz_adamw_state_elements(count, numel) < 0) return fail(AGZ_ERR_ARG, "agz_adamw_step: a negative or far too large tensor");
-    if (count > 0 && (!aligned(m, 16) || !aligned(v, 16))) return fail(AGZ_ERR_ARG, "agz_adamw_step: the states have to begin at a multiple of 16 bytes");
+    if (!aligned(m, 16) || !aligned(v, 16)) return fail(AGZ_ERR_ARG, "agz_adamw_step: the states have to begin at a multiple of 16 bytes");
     for (int i = 0; i < count; ++i) {
         if (cdiv(numel[i], AW_BLOCK) > AW_MOST) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d has more than 2^34 elements", i);
         if (numel[i] == 0 || !grads[i]) continue;

@@ -483,3 +483,21 @@ def test_a_tensor_without_a_gradient_stays_unchanged_for_autograd():
     ops.AdamW([p, q], **HYPER).step([torch.ones(10, device="cuda"), None])
     y.backward()
     assert torch.equal(q.grad, 2 * q.detach())
+
+
+def test_nothing_but_empty_tensors_needs_no_states():
+    """Tensors without elements have no states, so there is no buffer to name: not an error of the arguments (without a GPU the call ends with the missing device)."""
+    L = lib.load_library()
+    o = lib.AdamWOptions(lr=0.1, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, param_dtype=0, grad_dtype=0, bits=8, seed=0, tensor_base=0, step=1)
+    rc = L.agz_adamw_step(0, None, C.byref(o), 2, (C.c_void_p * 2)(), (C.c_void_p * 2)(), (C.c_int64 * 2)(0, 0), None, None, None, None)
+    assert rc == (0 if torch.cuda.is_available() else -2), L.agz_ops_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_of_empty_tensors(bits):
+    p = torch.empty(0, 3, device="cuda")
+    opt = ops.AdamW([p], bits=bits)
+    opt.step([torch.empty(0, 3, device="cuda")])
+    opt.load_state(opt.state())
+    assert opt.steps == 1 and p.shape == (0, 3)
