@@ -520,9 +520,13 @@ template <typename T, int VEC, int NV> __global__ __launch_bounds__(256) void k_
     }
 }
 
+// a launch has fewer than 2^32 lanes: 2^24 - 1 workgroups of 256, and at most 32 rows a workgroup
+constexpr int64_t MOST_GROUPS = (1ll << 24) - 1, MOST_ROWS = MOST_GROUPS * 32;
+
 static int check(const char* who, const agz_logprob_args* q) {
     if (!q) return fail(AGZ_ERR_ARG, "%s: no arguments", who);
     if (q->n < 0 || q->a < 1 || q->a > (1ll << 30)) return fail(AGZ_ERR_ARG, "%s: %lld rows of %lld actions (rows >= 0, 1 <= actions <= 2^30)", who, (long long)q->n, (long long)q->a);
+    if (q->n > MOST_ROWS) return fail(AGZ_ERR_ARG, "%s: too many rows", who);
     if (!good_dtype(q->dtype)) return fail(AGZ_ERR_ARG, "%s: unknown dtype %d", who, q->dtype);
     if (q->top < 0 || q->top > AGZ_TOP_MAX) return fail(AGZ_ERR_ARG, "%s: %d alternatives (0 to %d)", who, q->top, AGZ_TOP_MAX);
     if (q->ld < 0 || q->ld_mask < 0 || q->ld_target < 0) return fail(AGZ_ERR_ARG, "%s: a negative stride", who);
@@ -573,13 +577,17 @@ template <typename T, typename F> static int by_length(int64_t a, int top, F&& f
     return AGZ_LP(V, 64, F4);
 #undef AGZ_LP
 }
-// waves of a call: with 256 lanes for four of them fewer than 2^32 lanes (short rows need fewer: the launch itself looks again)
-static bool too_many(int64_t waves) { return waves >= 1ll << 26; }
+// workgroups of a call on rows that are `parts` waves each, or (1) as by_length says
+static int64_t groups_of(int dtype, int64_t n, int64_t a, int top, int64_t parts) {
+    int64_t groups = cdiv(n * parts, 4);
+    if (parts == 1) by_dtype(dtype, [&](auto t) { return by_length<decltype(t)>(a, top, [&](auto, auto g, auto) { groups = cdiv(n, 256 / g()); return 0; }); });
+    return groups;
+}
 
 extern "C" {
 
 int64_t agz_logprob_workspace(int64_t n, int64_t a, int32_t top) {
-    if (n < 0 || a < 1 || a > (1ll << 30) || top < 0 || top > AGZ_TOP_MAX) return -1;
+    if (n < 0 || n > MOST_ROWS || a < 1 || a > (1ll << 30) || top < 0 || top > AGZ_TOP_MAX) return -1;
     if (a <= PART) return 0;
     const int64_t p = parts_of(n, a, top, true).parts, q = parts_of(n, a, top, false).parts;     // (one block more may be longer parts, and fewer)
     return n * (p > q ? p : q) * (int64_t)(sizeof(PartOut) + 8 * top);
@@ -592,13 +600,13 @@ int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
     const int64_t need = agz_logprob_workspace(q->n, q->a, q->top);
     if (need > 0 && (!q->workspace || q->workspace_bytes < need || !aligned(q->workspace, 16)))
         return fail(AGZ_ERR_ARG, "agz_logprob_forward: a workspace of %lld bytes, 16-byte aligned", (long long)need);
-    OnDevice on(device);
-    if (on.rc != AGZ_OK) return on.rc;
-    if (q->n == 0) return AGZ_OK;
     const LpPar p = pack(q);
     const bool plain = !p.mask && !p.target && p.top == 0;
     const Parts w = parts_of(p.n, p.a, p.top, plain);
-    if (too_many(p.n * w.parts)) return fail(AGZ_ERR_ARG, "agz_logprob_forward: too many rows");
+    if (groups_of(q->dtype, p.n, p.a, p.top, p.a <= PART ? 1 : w.parts) > MOST_GROUPS) return fail(AGZ_ERR_ARG, "agz_logprob_forward: too many rows");
+    OnDevice on(device);
+    if (on.rc != AGZ_OK) return on.rc;
+    if (q->n == 0) return AGZ_OK;
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
         if (p.a <= PART)
@@ -622,14 +630,14 @@ int agz_logprob_backward(int device, void* stream, const agz_logprob_args* q, co
         if (g_target && !q->target) return fail(AGZ_ERR_ARG, "agz_logprob_backward: g_target without a target");
         if (g_top && (q->top == 0 || !q->top_move)) return fail(AGZ_ERR_ARG, "agz_logprob_backward: g_top without alternatives");
     }
-    OnDevice on(device);
-    if (on.rc != AGZ_OK) return on.rc;
-    if (q->n == 0) return AGZ_OK;
     LpPar p = pack(q);
     p.g_move = g_move; p.g_entropy = g_entropy; p.g_target = g_target; p.g_top = g_top; p.dx = dx; p.ldd = ldd;
     const bool plain = !p.mask && !g_target && !g_top;
     const int64_t parts = p.a <= PART ? 1 : cdiv(plain ? p.a + MOST_PAD : p.a, PART);
-    if (too_many(p.n * parts)) return fail(AGZ_ERR_ARG, "agz_logprob_backward: too many rows");
+    if (groups_of(q->dtype, p.n, p.a, 0, parts) > MOST_GROUPS) return fail(AGZ_ERR_ARG, "agz_logprob_backward: too many rows");
+    OnDevice on(device);
+    if (on.rc != AGZ_OK) return on.rc;
+    if (q->n == 0) return AGZ_OK;
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
         constexpr int V = 16 / sizeof(T);

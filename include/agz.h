@@ -271,7 +271,7 @@ const char *agz_ops_last_error(void);
  * A row with no allowed entry: entropy 0, move_logp -inf (0 without a move), target_logp 0 without targets and -inf with, no alternatives,
  * gradient 0.  A row with a NaN or +inf in S: NaN everywhere and no alternatives. */
 typedef struct {
-    int64_t n, a;               /* rows, actions (1 <= a <= 2^30) */
+    int64_t n, a;               /* rows (up to 2^26; nearly 2^29 short ones, fewer of several blocks of 2048), actions (1 <= a <= 2^30) */
     const void *logits;         /* [n][a], dtype, row stride ld (elements; any, also 0) */
     int64_t ld;
     int32_t dtype;              /* agz_dtype */

@@ -519,3 +519,44 @@ def test_forward_mode_derivatives_are_refused():
         assert torch.equal(plain.entropy, want.entropy)
         with fwd._set_fwd_grad_enabled(False):                     # (as within the forward of a function that has a rule of its own)
             assert torch.equal(ops.log_probs(d).entropy, want.entropy)
+
+
+def test_many_short_rows_are_not_too_many():
+    """A launch holds fewer than 2^32 lanes: nearly 2^29 rows of which each takes eight of them, 2^26 that take a whole wave.  (Without a GPU a call that is not refused ends with
+    the missing device; the memory behind the addresses is not read then.)"""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses here are no device memory")
+    L = lib.load_library()
+    buf = (C.c_char * 4096)()
+    at = (C.addressof(buf) + 63) // 64 * 64
+    for n, a, dtype, top, forward, backward in ((1 << 26, 81, 1, 0, True, True), ((1 << 26) + 5, 2, 0, 0, True, True), ((1 << 29) - 32, 81, 1, 0, True, True), ((1 << 29) - 31, 81, 1, 0, False, False),
+                                                (1 << 27, 500, 1, 0, True, True), (1 << 28, 500, 1, 0, False, False), ((1 << 26) - 4, 2000, 0, 0, True, True), (1 << 26, 2000, 0, 0, False, False),
+                                                (1 << 26, 1000, 0, 9, False, True), (1 << 62, 2, 0, 0, False, False), (1 << 62, 4000, 0, 0, False, False)):
+        ws = L.agz_logprob_workspace(n, a, top)
+        assert (ws < 0) == (n > (1 << 29) - 32)
+        q = lib.LogProbArgs(n=n, a=a, logits=at, ld=a, dtype=dtype, top=top, stats=at, entropy=at, workspace=at, workspace_bytes=max(ws, 0))
+        for fits, call in ((forward, lambda: L.agz_logprob_forward(0, None, C.byref(q))), (backward, lambda: L.agz_logprob_backward(0, None, C.byref(q), None, at, None, None, at, a))):
+            assert call() == (-2 if fits else -1) and (fits or b"too many rows" in L.agz_ops_last_error()), (n, a, L.agz_ops_last_error())
+
+
+@pytest.mark.gpu
+def test_more_than_2_26_short_rows():
+    """Forward and backward where only the last rows and some in between differ from zeros: those as a short call has them, the others all alike."""
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GiB of free device memory")
+    n, a = (1 << 26) + 37, 3
+    some = torch.tensor([0, 5, 1 << 20, 1 << 25, (1 << 26) - 1, 1 << 26, n - 2, n - 1], device="cuda")
+    few = torch.randn(8, a, generator=torch.Generator().manual_seed(4)).cuda()
+    x = torch.zeros(n, a, device="cuda")
+    x[some] = few
+    def both(x):
+        x = x.requires_grad_()
+        r = ops.log_probs(x, top=1)
+        dx, = torch.autograd.grad([r.entropy], [x], [torch.ones_like(r.entropy)])
+        return r.entropy.detach(), r.top_move, dx
+    want, got = both(few), both(x)
+    for w, g in zip(want, got):
+        assert torch.equal(g[some], w)
+        rest = torch.ones(n, dtype=torch.bool, device="cuda")
+        rest[some] = False
+        assert (g[rest] == g[1]).all()
