@@ -554,16 +554,16 @@ using namespace agz::ops;
 // f(elements per span, lanes per row, spans per lane) for rows of `a` actions: 32 elements a lane at most, and as few lanes as hold the row, since the
 // reductions over them are what short rows spend their time on (200000 rows of 500 bf16: 106 us with 64 lanes a row, 37 us with 16).  A row above 128
 // actions of which more than four alternatives are wanted gets a whole wave: wave_top finds them in one go (40000 rows of 500, 20 alternatives: 64 us,
-// 180 us with 16 lanes that take one after the other; one alternative costs the few lanes less).
-template <typename T, typename F> static int by_length(int64_t a, int top, F&& f) {
+// 180 us with 16 lanes that take one after the other; one alternative costs the few lanes less).  TOPS: alternatives may be wanted.
+template <typename T, bool TOPS, typename F> static int by_length(int64_t a, int top, F&& f) {
     constexpr int V = 16 / sizeof(T), F4 = 32 / V, F3 = F4 * 3 / 4, F2 = F4 / 2, F1 = F4 / 4;
     using std::integral_constant;
 #define AGZ_LP(VEC, G, NV) f(integral_constant<int, VEC>{}, integral_constant<int, G>{}, integral_constant<int, NV>{})
     if (a < V) return AGZ_LP(1, 8, 1);
     if (a <= 8 * V * F1) return AGZ_LP(V, 8, F1);
-    if (sizeof(T) == 4 && a > 64 && a <= 96) return AGZ_LP(V, 8, 3);      // (boards of 81 in 32 bits)
+    if constexpr (sizeof(T) == 4) if (a > 8 * V * F1 && a <= 8 * V * 3) return AGZ_LP(V, 8, 3);      // (65 to 96 actions in 32 bits: three spans a lane, not four)
     if (a <= 8 * V * F2) return AGZ_LP(V, 8, F2);
-    if (top > 4 && a > 128) {
+    if constexpr (TOPS) if (top > 4 && a > 128) {
         if (a <= 64 * V * F1) return AGZ_LP(V, 64, F1);
         if (a <= 64 * V * F2) return AGZ_LP(V, 64, F2);
         return a <= 64 * V * F3 ? AGZ_LP(V, 64, F3) : AGZ_LP(V, 64, F4);
@@ -580,7 +580,7 @@ template <typename T, typename F> static int by_length(int64_t a, int top, F&& f
 // workgroups of a call on rows that are `parts` waves each, or (1) as by_length says
 static int64_t groups_of(int dtype, int64_t n, int64_t a, int top, int64_t parts) {
     int64_t groups = cdiv(n * parts, 4);
-    if (parts == 1) by_dtype(dtype, [&](auto t) { return by_length<decltype(t)>(a, top, [&](auto, auto g, auto) { groups = cdiv(n, 256 / g()); return 0; }); });
+    if (parts == 1) by_dtype(dtype, [&](auto t) { return by_length<decltype(t), true>(a, top, [&](auto, auto g, auto) { groups = cdiv(n, 256 / g()); return 0; }); });
     return groups;
 }
 
@@ -609,10 +609,12 @@ int agz_logprob_forward(int device, void* stream, const agz_logprob_args* q) {
     if (q->n == 0) return AGZ_OK;
     return by_dtype(q->dtype, [&](auto t) {
         using T = decltype(t);
-        if (p.a <= PART)
-            return by_length<T>(p.a, p.top, [&](auto vec, auto g, auto nv) {
-                return launch(plain ? k_logprob<T, vec(), g(), nv(), true> : k_logprob<T, vec(), g(), nv(), false>, dim3((uint32_t)cdiv(p.n, 256 / g())), dim3(256), 0, stream, p);
+        auto whole = [&](auto is_plain) {
+            return by_length<T, !is_plain()>(p.a, p.top, [&](auto vec, auto g, auto nv) {
+                return launch(k_logprob<T, vec(), g(), nv(), is_plain()>, dim3((uint32_t)cdiv(p.n, 256 / g())), dim3(256), 0, stream, p);
             });
+        };
+        if (p.a <= PART) return plain ? whole(std::true_type{}) : whole(std::false_type{});
         constexpr int V = 16 / sizeof(T);
         PartOut* part = (PartOut*)q->workspace;
         uint64_t* keys = (uint64_t*)(part + p.n * w.parts);
@@ -642,7 +644,7 @@ int agz_logprob_backward(int device, void* stream, const agz_logprob_args* q, co
         using T = decltype(t);
         constexpr int V = 16 / sizeof(T);
         if (plain && parts > 1) return launch(k_logprob_grad_part<T, V, PART / 64 / V>, dim3((uint32_t)cdiv(p.n * parts, 4)), dim3(256), 0, stream, p, (int32_t)parts);
-        return by_length<T>(p.a, 0, [&](auto vec, auto g, auto nv) {
+        return by_length<T, false>(p.a, 0, [&](auto vec, auto g, auto nv) {
             return launch(plain ? k_logprob_grad<T, vec(), g(), nv(), true> : k_logprob_grad<T, vec(), g(), nv(), false>, dim3((uint32_t)cdiv(p.n * parts, 256 / g())), dim3(256), 0, stream, p, (int32_t)parts);
         });
     });
