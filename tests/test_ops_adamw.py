@@ -501,3 +501,34 @@ def test_a_step_of_empty_tensors(bits):
     opt.step([torch.empty(0, 3, device="cuda")])
     opt.load_state(opt.state())
     assert opt.steps == 1 and p.shape == (0, 3)
+
+
+@pytest.mark.gpu
+def test_8_bits_round_to_both_sides_in_proportion():
+    """One step of 2^20 equal elements: m and r lie between two neighbours in 8 bits, and their means keep to the exact values from both sides.  An element is up with the
+    probability of its place f (in steps of 2^-16 of a gap), so the mean is off by at most 2^-16 of a gap and six standard errors, gap sqrt(f (1 - f) / n) <= gap / (2 * 2^10),
+    beside a few roundings of 32 bits.  The mean of r^2, which the next step begins with, is the square of the mean and the variance of the rounding, gap^2 f (1 - f)."""
+    n, b1, b2 = 1 << 20, 0.9, 0.999
+    for g, r0, m0 in ((0.6, 0.5625, 0.375), (3e-5, 2.0 ** -15, -(2.0 ** -14)), (700.0, 832.0, 104.0), (0.0, 1.75, 1.625)):
+        p = torch.zeros(n, device="cuda")
+        opt = ops.AdamW([p], lr=0.0, betas=(b1, b2), bits=8, weight_decay=0.0, seed=11)
+        held = ops.AdamW([p], lr=0.0, bits=8)
+        for name, x in (("m", m0), ("r", r0)):
+            q = ops.quantize_fp8(torch.full((n // 128, 128), x, device="cuda"))
+            assert (q.dequantize() == x).all()                      # (all of them are values of 8 bits)
+            getattr(held, name).view(torch.uint8).copy_(q.q.view(torch.uint8).view(-1))
+            getattr(held, name + "_scale").view(torch.uint8).copy_(q.scale.view(torch.uint8)[:, 0])
+        opt.load_state(held.state())
+        g32 = torch.full((n,), g, device="cuda")
+        opt.step([g32])
+        g64 = g32[0].double().item()
+        for codes, scale, x in ((opt.m, opt.m_scale, b1 * m0 + (1 - b1) * g64), (opt.r, opt.r_scale, math.sqrt(b2 * r0 * r0 + (1 - b2) * g64 * g64))):
+            got = held_as(codes, scale).double()
+            gap = 2.0 ** (math.floor(math.log2(abs(x))) - 3)
+            tol = gap * (2.0 ** -16 + 6 / 2 ** 11) + 8 * E32 * (abs(x) + abs(m0) + abs(g64))
+            assert abs(got.mean().item() - x) <= tol, (g, x, got.mean())
+            low = math.floor(abs(x) / gap) * gap
+            assert ((got.abs() == low) | (got.abs() == low + gap)).all()
+            f = (abs(x) - low) / gap
+            # (2 |x| times the mean's own error, and the same six standard errors of the squares' differences, at most 2 (low + gap) gap apart)
+            assert abs(got.square().mean().item() - x * x - gap * gap * f * (1 - f)) <= 2 * (abs(x) + gap) * tol, (g, x)
