@@ -83,8 +83,9 @@ template <bool FLOOR> __device__ __forceinline__ uint32_t aw_hold(const float* x
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
 }
 
-// One pass: every tensor, gradient and state is read and written once.  Bound by memory: 67 M weights in 32 bits 347 us (1.88 GB, 5.4 TB/s), states in 8 bits with bf16
-// gradients 176-193 us (942 MB, 4.9-5.4 TB/s); the eight tensors of a 128-wide network 5.4 us, the launch.
+// One pass: every tensor, gradient and state is read and written once.  Bound by memory: 67 M weights in 32 bits 348 us (1.88 GB, 5.4 TB/s), states in 8 bits with bf16
+// gradients 176-186 us in a run of calls (942 MB, 5.1-5.4 TB/s; launches in a row under a profiler 165 us at first, up to 280 us later); the eleven tensors of a
+// 128-wide network 4.4-5.0 us, the launch.
 template <typename P, typename G, int BITS>
 __global__ __launch_bounds__(256) void k_adamw(AwTable tab, AwPar a, void* mp, void* vp, uint8_t* ms, uint8_t* vs) {
     const int tid = threadIdx.x;

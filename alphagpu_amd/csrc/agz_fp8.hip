@@ -37,8 +37,8 @@ template <typename F> __device__ __forceinline__ float groups_reduce(float x, F&
 // written eight at a time both ways (8 x 8 values: the transpose is a matter of which eight are packed).  A row's largest is a reduction over
 // 16 lanes, a column's one over 4 lanes and, through LDS, the 4 waves.  fmaxf passes NaN over; a largest of infinity means that the block has one, and its largest
 // finite entry is looked for again.
-// Bound by memory: 32768 x 512 bf16 both ways 17.3 us (67 MB, 3.9 TB/s), with the gate and column sums 21.8 us (101 MB, 4.6 TB/s); 8192 x 8192 bf16 both ways 59 us
-// (270 MB, 4.6 TB/s); 8192 x 4096 in 32 bits, blocks of 128 x 128, 43 us (201 MB, 4.6 TB/s).
+// Bound by memory: 32768 x 512 bf16 both ways 17.0 us (67 MB, 4.0 TB/s), with the gate and column sums 22.0 us (101 MB, 4.6 TB/s); 8192 x 8192 bf16 both ways with column
+// sums 62-65 us (270 MB, 4.1-4.4 TB/s); 8192 x 4096 in 32 bits, blocks of 128 x 128, 42-47 us (201 MB, 4.3-4.8 TB/s).
 template <typename T, int BR, bool ROW, bool COL, bool GATE, bool NARROW>
 __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
     __shared__ __attribute__((aligned(16))) float red[4][FB];
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void k_quantize(QuantPar p) {
     }
 }
 
-// the tiles' column sums added up in a fixed order: 64 columns and 16 shares of the tiles per workgroup.  Bound by the launch: 3.8 us for 256 tiles of 512 columns
+// the tiles' column sums added up in a fixed order: 64 columns and 16 shares of the tiles per workgroup.  Bound by the launch: 4.6 us for 256 tiles of 512 columns
 __global__ __launch_bounds__(1024) void k_colsum(const float* part, int64_t tiles, int64_t cols, void* out, int out_dtype) {
     __shared__ float red[16][64];
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
@@ -292,10 +292,12 @@ __device__ __forceinline__ f32x4 mma_wide(const Wide& a, const Wide& b, f32x4 c)
 // writes lanes in order).  WM x WN waves, each BM / WM x BN / WN in tiles of 16 x 16; B is the first operand, so that a lane ends with four
 // neighbouring columns of one row.  Rows and columns outside are read from the last one and not stored.  Scales: a word holds a row's bytes of four steps; the words
 // go through LDS too (a load to registers inside the loop would have to be waited for, and with it the next step's loads).
-// Bound by the matrix unit and, for long k, by the clock, which falls under its load.  Tiles of 256: 8192 x 4096 x 8192 (m x n x k) 221 us = 2.49 PFLOP/s (the
-// library's product with one scale for each whole matrix, without blocks: 3.3), 8192 x 8192 x 4096 259 us = 2.12 (2.76), to 32 bits 405 us = 1.36 (the library's bf16
-// product: 1.57).  Tiles of 128: 32768 x 512 x 512 20.5 us, behind a relu 26.4 us, where loading the four steps, products and results (50 MB) overlap only between the two
-// workgroups of a CU; four workgroups a CU with one buffer each: 23 and 30 us, with 23 to 41 registers spilled.
+// Bound by the matrix unit and, for long k, by the clock, which falls under its load: a product alone is faster than the same among others.  Tiles of 256:
+// 8192 x 4096 x 8192 (m x n x k) 221 us alone = 2.49 PFLOP/s, 237 us in a learning step = 2.32 (the library's product with one scale for each whole matrix, without blocks:
+// 3.3 alone), 8192 x 8192 x 4096 259-261 us = 2.11 (2.76), to 32 bits 405 us alone = 1.36, 438 us in a step = 1.26 (the library's bf16 product: 1.57).  They hold 256
+// registers, and spill 27 or 28 of them in front of their results.  Tiles of 128: 32768 x 512 x 512 21.9 us, behind a relu 30.9 us, where loading the four steps, products
+// and results (50 MB) overlap only between the two workgroups of a CU; four workgroups a CU with one buffer each: 23 and 30 us where two took 20.5 and 26.4, with 23 to
+// 41 registers spilled.
 // ---------------------------------------------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(1))) const void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
@@ -561,7 +563,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_matmul_fp8(MatPar p) {
     else store_tile<f16, TL, BM, BN, WM, WN>(lds, acc, (f16*)p.out, p.ldo, p.m, p.n, m0, n0);
 }
 
-// the slices of the k axis added up, in order.  Bound by memory: 32 slices of 512 x 512 6.8 us (34 MB, 4.9 TB/s)
+// the slices of the k axis added up, in order.  Bound by memory: 32 slices of 512 x 512 6.6 us (34 MB, 5.1 TB/s)
 __global__ __launch_bounds__(256) void k_matmul_join(MatPar p) {
     const int64_t quads = (p.n + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / quads, c = (i - r * quads) * 4;
     if (r >= p.m) return;
@@ -622,7 +624,7 @@ template <typename T> __device__ __forceinline__ int quantize32(const T* x, int 
 // Few rows (up to 16): the weights are read once, straight into the matrix unit's registers, and that is all the time there is.  A wave takes 16
 // columns and every FEW_WAVES-th group of four steps; the waves of a workgroup add up through LDS.  T: uint8_t for a matrix in 8 bits, or the type of
 // x, which every workgroup then holds in 8 bits itself, in LDS (a launch less; as long as its rows are short, x comes from the caches:
-// one row of 8192 and 8192 columns 19.7 us in two launches, 15.4 us in one: 67 MB of weights, 4.4 TB/s).
+// one row of 8192 and 8192 columns 19.7 us in two launches, 14.7-15.4 us in one: 67 MB of weights, 4.4-4.6 TB/s).
 constexpr int FEW_WAVES = 4, FEW_DEEP = 4, FEW_LDS = 32768;
 template <typename T, bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) void k_matmul_fp8_few(MatPar p, const T* x, int64_t ldx) {
     __shared__ f32x4 sum[FEW_WAVES][64];
@@ -691,7 +693,7 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(FEW_WAVES * 64) vo
 
 // More rows on ready weights where the k axis has up to SHORT_STEPS steps: one launch too.  A workgroup turns its SHORT_M rows of x into 8 bits on their way into LDS (the
 // same bits that k_quantize writes, 16 lanes a row and step), the weights' 128 rows come straight from memory, all steps at once; then products and results as in the
-// tiles above.  Bound by latency where a workgroup or two a CU do it all (20001 x 162 -> 128 bf16, relu: 10.2 us a call in a graph, 11.6 MB), by memory above:
+// tiles above.  Bound by latency where a workgroup or two a CU do it all (20001 x 162 -> 128 bf16, relu: 10.2 us a call in a graph, 11.9 us the launch under a profiler, 11.6 MB), by memory above:
 // 200000 x 128 -> 128 30.6 us (102 MB, 3.3 TB/s).
 constexpr int SHORT_STEPS = 4, SHORT_M = 64, SHORT_N = 128;
 template <int KB> struct Short {

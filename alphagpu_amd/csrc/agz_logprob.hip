@@ -123,7 +123,7 @@ template <typename E> __device__ __forceinline__ void wave_list_ranks(const uint
 // The `top` best entries of what a wave holds (NE per lane, -inf: not allowed), largest first: emit(rank, key) from the lane that finds it, emit(rank, 0) behind
 // the last.  Every lane's best: the top-th largest of these 64 is a lower bound of the top-th largest entry.  The entries from that bound on (at most top lanes'
 // shares) go into a list in LDS, and an entry's place is the number of entries before it: all comparisons are independent, where taking the best again and
-// again is a chain of `top` reductions (20 of a row of 131072: part launch 41.5 -> 7 us).
+// again is a chain of `top` reductions (20 of a row of 131072: part launch 41.5 us so, 9-10 us this way).
 constexpr int LIST = AGZ_TOP_MAX * 32;
 template <int NE, typename J, typename E> __device__ __forceinline__ void wave_top(const float (&x)[NE], J&& index, int top, uint64_t* list, E&& emit) {
     static_assert(NE <= 32, "the list holds the shares of AGZ_TOP_MAX lanes");
@@ -207,11 +207,14 @@ template <typename T> __device__ __forceinline__ float given_logit(const LpPar& 
     return !mask || mask[mv] ? v : -INFINITY;
 }
 
-// A row per group of G lanes: rows of up to G NV VEC actions.  One pass: the row is read once and stays in registers: logp_j = d_j - log s and
-// entropy = log s - (sum d e^d) / s with d = x - largest, so nothing is read again once the largest is known.
-// PLAIN: without mask, target and alternatives (fewer registers).
-// Bound by memory where rows are many, by launch and reductions where they are few.  32768 rows of 81 in 32 bits with mask and five alternatives: 8.0 us
-// (13 MB read; 4.3 us without the alternatives); 65536 with mask and target: 10.9 us (48 MB read, 4.4 TB/s; a copy of large tensors reaches 4.8 TB/s on the same card).
+// A row per group of G lanes: rows of up to G NV VEC actions.  One pass over memory: logp_j = d_j - log s and entropy = log s - (sum d e^d) / s with
+// d = x - largest, so the row is not read again once the largest is known.
+// PLAIN: without mask, target and alternatives (fewer registers).  The other builds of fewer than 64 lanes a row and 24 or 32 elements a lane (rows of 129 to
+// 1024 actions) hold most of the row in private memory, 56 and 100 bytes a lane, in all calls: take_best takes an element out at a place that only the run knows.
+// That goes through the caches: 32768 rows with mask and target in 32 bits (bf16) take, of 169 actions 15.2 (14.1) us where the bytes take 10.5 (8.2) at the rate of a
+// copy, of 225 16.9 (16.1) for 14.0 (10.9), of 361 22.2 (20.1) for 22.3 (17.4), of 500 30.8 (27.5) for 30.9 (24.0), of 1000 68.6 (51.1) for 61.6 (47.9).
+// Bound by memory where rows are many, by launch and reductions where they are few.  32768 rows of 81 in 32 bits with mask and five alternatives: 8.0-8.7 us
+// (13 MB read; 4.3 us without the alternatives); 65536 with mask and target: 10.4 us (48 MB read, 4.6 TB/s; a copy of large tensors reaches 4.8 TB/s on the same card).
 template <typename T, int VEC, int G, int NV, bool PLAIN> __global__ __launch_bounds__(256) void k_logprob(LpPar p) {
     const int l = threadIdx.x & (G - 1);
     const int64_t i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -251,7 +254,8 @@ template <typename T, int VEC, int G, int NV, bool PLAIN> __global__ __launch_bo
 // and the lanes are joined once.  (4096 rows of 50001 bf16: a block a wave 221 us.)
 // Without mask and target the spans lie on 16-byte borders of memory wherever the row begins: the first one begins up to seven elements before the row (and is read
 // from the row's start, the elements that are not its own left out), since unaligned spans cost a tenth (50001 against 50000 bf16).
-// Bound by memory: 4096 rows of 50001 bf16 117 us (3.5 TB/s); one row of 131072 with 20 alternatives 9.4 us, 64 waves: launch and wave_top.
+// Bound by memory, and by waves that do not come out even: 4096 rows of 50001 bf16 121 us (3.4 TB/s), 12288 waves where 5120 fit on the card at a time; one row of
+// 131072 with 20 alternatives 9-10 us, 64 waves: launch and wave_top.
 constexpr int PART = 2048, MOST = 16, WAVES_ENOUGH = 8192, MOST_PAD = 7;
 template <typename T, int VEC> __device__ __forceinline__ int pad_of(const T* row) { return (int)((uintptr_t)row / sizeof(T) & (VEC - 1)); }
 __device__ __forceinline__ int64_t span_at(int64_t own, int64_t last) { return own < 0 ? 0 : (own < last ? own : last); }     // last: a - VEC
@@ -347,7 +351,7 @@ template <typename T, int VEC, int NV, bool PLAIN> __global__ __launch_bounds__(
 }
 
 // The parts of a row joined by a wave: sums brought to the largest entry of all, alternatives by the bound of wave_top over the parts' keys.  Bound by the launch and
-// two dependent reads: 5.2 us for 4096 rows of 25 parts, 6.9 us for one row of 64 parts with 20 alternatives each.
+// two dependent reads: 5.7 us for 4096 rows of three parts, 6.6 us for one row of 64 parts with 20 alternatives each.
 constexpr int JOIN_LIST = 1024;
 template <typename T> __global__ __launch_bounds__(256) void k_logprob_join(LpPar p, int32_t parts, const PartOut* part, const uint64_t* keys) {
     const int l = threadIdx.x & 63;
@@ -430,7 +434,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_logprob_join(LpPa
 // ---------------------------------------------------------------------------------------------------------------------------------------
 // the gradient: one pass that reads the row and writes the gradient; a row (or part) per group of G lanes as above.  With the forward pass's largest entry, log sum and
 // entropy every entry stands for itself: g_j = c_j - p_j (sum c + g_entropy (logp_j + entropy)).  Bound by memory: 65536 rows of 81 in 32 bits with mask and target
-// 12.9 us (69 MB, partly from the caches: 5.3 TB/s)
+// 13.1 us (69 MB, partly from the caches: 5.3 TB/s)
 // ---------------------------------------------------------------------------------------------------------------------------------------
 struct GradRow { float mx, ls, gh, gt, gm, whole; int32_t mv; };         // whole: the sum of the cotangents, and gh times the entropy
 __device__ __forceinline__ float grad_at(const GradRow& c, float v, float t, bool hot) {
@@ -489,7 +493,7 @@ template <typename T, int VEC, int G, int NV, bool PLAIN> __global__ __launch_bo
 }
 
 // ... of long rows without mask, target and cotangents of alternatives: a wave per block, spans on 16-byte borders as in the forward pass (the gradient's rows lie
-// like the logits' where their strides agree): 4096 rows of 50001 bf16 144 us (819 MB, 5.7 TB/s; spans that begin where the row begins: 194 us)
+// like the logits' where their strides agree): 4096 rows of 50001 bf16 144-153 us (819 MB, 5.4-5.7 TB/s; spans that begin where the row begins: 194 us)
 template <typename T, int VEC, int NV> __global__ __launch_bounds__(256) void k_logprob_grad_part(LpPar p, int32_t parts) {
     const int l = threadIdx.x & 63;
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), i = w / parts;

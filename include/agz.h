@@ -348,7 +348,9 @@ int  agz_linear_fp8_backward(int device, void *stream, const agz_linear_fp8_args
  * in 32 bits, p rounded once to its type.  The states of all tensors lie in common buffers: tensor i begins at element 128 x sum over the
  * tensors before it of ceil(numel / 128) (agz_adamw_state_elements: their length).  bits = 32: m, v are floats.  bits = 8: m and r = sqrt(v) are
  * held in e4m3 with one power-of-two scale (e8m0 byte, as in agz_fp8_quantize) per 128 elements and rounded up or down at random in
- * proportion (unbiased: to the nearest, v could no longer shrink, its steps of 1 - b2 are below half a rounding step); r is 0 only where v is.
+ * proportion (to the nearest, v could no longer shrink, its steps of 1 - b2 are below half a rounding step): m and r keep their means; r is 0 only where v is, and
+ * below the smallest step of its block it is held as that step.  v = r^2 is larger in the mean, by the variance of r's rounding: under normal gradients v by 4 % and r by 1 % (b2 of 0.99
+ * and 0.999), entries at 1e-5 of their block's largest v by 48 % and r by 14 %: their steps are that much smaller.
  * The random bits are a hash of (seed, t, tensor index + tensor_base, element): equal arguments give equal results.
  * A tensor whose gradient is NULL is left as it is, its states too, and the step is none of its own: its t is the call's less the number of steps that it missed, so
  * that moments that begin late are corrected as those of the first steps are.  Tensors must not overlap; each has at most 2^34 elements. */
