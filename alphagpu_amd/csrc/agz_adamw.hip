@@ -193,6 +193,11 @@ int64_t agz_adamw_state_elements(int count, const int64_t* numel) {
 
 int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int count, void* const* params, const void* const* grads, const int64_t* numel,
                    void* m, void* v, void* m_scale, void* v_scale) {
+    return agz_adamw_step_missed(device, stream, o, nullptr, nullptr, count, params, grads, numel, m, v, m_scale, v_scale);
+}
+
+int agz_adamw_step_missed(int device, void* stream, const agz_adamw_options* o, const int64_t* missed, int64_t* missed_dev, int count, void* const* params, const void* const* grads,
+                          const int64_t* numel, void* m, void* v, void* m_scale, void* v_scale) {
     if (!o) return fail(AGZ_ERR_ARG, "agz_adamw_step: no options");
     if (count < 0 || (count > 0 && (!params || !grads || !numel))) return fail(AGZ_ERR_ARG, "agz_adamw_step: null argument");
     if (!good_dtype(o->param_dtype) || !good_dtype(o->grad_dtype)) return fail(AGZ_ERR_ARG, "agz_adamw_step: unknown dtype");
@@ -202,9 +207,9 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
     if (elements > 0 && (!m || !v)) return fail(AGZ_ERR_ARG, "agz_adamw_step: null argument");
     if (o->bits == 8 && elements > 0 && (!m_scale || !v_scale)) return fail(AGZ_ERR_ARG, "agz_adamw_step: 8-bit states need their scales");
     if (!o->step_dev && o->step < 1) return fail(AGZ_ERR_ARG, "agz_adamw_step: step %lld (from 1 on)", (long long)o->step);
-    if (!o->step_dev && o->missed_dev) return fail(AGZ_ERR_ARG, "agz_adamw_step: missed_dev goes with step_dev");
-    if (!aligned(o->step_dev, 8) || !aligned(o->missed_dev, 8)) return fail(AGZ_ERR_ARG, "agz_adamw_step: step_dev and missed_dev are not aligned to 8 bytes");
-    const int64_t* missed = o->step_dev ? nullptr : o->missed;
+    if (!o->step_dev && missed_dev) return fail(AGZ_ERR_ARG, "agz_adamw_step: missed_dev goes with step_dev");
+    if (!aligned(o->step_dev, 8) || !aligned(missed_dev, 8)) return fail(AGZ_ERR_ARG, "agz_adamw_step: step_dev and missed_dev are not aligned to 8 bytes");
+    if (o->step_dev) missed = nullptr;
     if (missed) for (int i = 0; i < count; ++i)
         if (missed[i] < 0 || missed[i] >= o->step) return fail(AGZ_ERR_ARG, "agz_adamw_step: tensor %d missed %lld of the %lld steps before this one", i, (long long)missed[i], (long long)o->step - 1);
     if (!(o->beta1 >= 0 && o->beta1 < 1) || !(o->beta2 >= 0 && o->beta2 < 1) || !(o->eps >= 0) || !(o->lr >= 0) || !(o->weight_decay >= 0))
@@ -253,9 +258,9 @@ int agz_adamw_step(int device, void* stream, const agz_adamw_options* o, int cou
             chunks += grads[i] ? (uint32_t)cdiv(blocks, AW_BLOCKS) : 0;
             state_block += blocks;
         }
-        a.missed_dev = o->missed_dev ? o->missed_dev + first : nullptr;
-        if (o->missed_dev && (missing.bit[0] | missing.bit[1] | missing.bit[2]))
-            if (const int rc = launch(k_adamw_missed, dim3(1), dim3(AW_MAX), 0, stream, missing, o->missed_dev + first)) return rc;
+        a.missed_dev = missed_dev ? missed_dev + first : nullptr;
+        if (missed_dev && (missing.bit[0] | missing.bit[1] | missing.bit[2]))
+            if (const int rc = launch(k_adamw_missed, dim3(1), dim3(AW_MAX), 0, stream, missing, missed_dev + first)) return rc;
         if (chunks == 0) continue;
         a.count = k;
         a.tensor0 = (uint32_t)(o->tensor_base + first);

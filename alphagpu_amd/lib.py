@@ -52,7 +52,7 @@ class LinearFp8Args(C.Structure):                   # agz_linear_fp8_args
 class AdamWOptions(C.Structure):                    # agz_adamw_options
     _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
                 ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("seed", C.c_uint32), ("tensor_base", C.c_int32),
-                ("step", C.c_int64), ("step_dev", C.c_void_p), ("missed", C.c_void_p), ("missed_dev", C.c_void_p)]
+                ("step", C.c_int64), ("step_dev", C.c_void_p)]
 
 
 def build_library():
@@ -129,7 +129,7 @@ def load_library():
         L.agz_comm_post_status.argtypes = [vp, C.c_int]
         L.agz_comm_get_statuses.argtypes = [vp, C.POINTER(C.c_int32)]
         L.agz_allgather_samples_status.argtypes = [vp, vp, C.c_int, i64p, C.POINTER(C.c_int32)]
-    if hasattr(L, "agz_ops_last_error") or not os.environ.get("AGZ_LIB_PATH"):
+    if hasattr(L, "agz_adamw_step_missed") or not os.environ.get("AGZ_LIB_PATH"):
         i64, i32 = C.c_int64, C.c_int
         L.agz_ops_last_error.argtypes = []
         L.agz_ops_last_error.restype = C.c_char_p
@@ -150,6 +150,7 @@ def load_library():
         L.agz_linear_fp8_backward.argtypes = [i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64]
         L.agz_adamw_state_elements.argtypes = [i32, vp]
         L.agz_adamw_step.argtypes = [i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+        L.agz_adamw_step_missed.argtypes = [i32, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp]
         for n in ("logprob_workspace", "fp8_pitch", "fp8_scale_pitch", "fp8_colsum_ws", "fp8_matmul_workspace", "linear_fp8_workspace", "linear_fp8_saved", "linear_fp8_apply_workspace", "linear_fp8_backward_workspace", "adamw_state_elements"):
             getattr(L, "agz_" + n).restype = i64
     _LIB = L

@@ -412,7 +412,7 @@ def linear_fp8(x, w, bias=None, relu=False):
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # AdamW
 # ---------------------------------------------------------------------------------------------------------------------------------------
-_ADAMW = struct.Struct("=dddddiiiIi4xqqqq")           # agz_adamw_options
+_ADAMW = struct.Struct("=dddddiiiIi4xqq")           # agz_adamw_options
 assert _ADAMW.size == C.sizeof(_lib.AdamWOptions)
 
 
@@ -520,7 +520,7 @@ class AdamW:
             if not g.is_contiguous():
                 g = grads[i] = g.contiguous()
             at.append(g.data_ptr())
-        missed = missed_dev = 0
+        missed = missed_dev = None
         if self.step_dev is None:
             if _capturing():
                 raise RuntimeError("AdamW.step in a graph: capturable=True is needed (a replay has to count its step on the device)")
@@ -530,12 +530,12 @@ class AdamW:
         else:
             counter, missed_dev = self.step_dev.data_ptr(), self._missed_dev.data_ptr()
         t = self.steps + 1
-        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[own], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter, missed, missed_dev)
+        o = _ADAMW.pack(self.lr, *self.betas, self.eps, self.weight_decay, _CODE[own], _CODE[kind or torch.float32], self.bits, self.seed & 0xFFFFFFFF, 0, t, counter)
         if counter:
             self.step_dev.add_(1)                            # (behind everything that can refuse the call)
         second, ms, rs = (self.v, None, None) if self.bits == 32 else (self.r, self.m_scale, self.r_scale)
         L = _lib.load_library()
-        rc = L.agz_adamw_step(device, _raw_stream(device), o, len(params), self._pointers.pack(*[p.data_ptr() for p in params]), self._pointers.pack(*at), self._numel,
+        rc = L.agz_adamw_step_missed(device, _raw_stream(device), o, missed, missed_dev, len(params), self._pointers.pack(*[p.data_ptr() for p in params]), self._pointers.pack(*at), self._numel,
                               self.m.data_ptr(), second.data_ptr(), _ptr(ms), _ptr(rs))
         if rc:
             _lib_call(rc, L)

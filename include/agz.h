@@ -352,8 +352,7 @@ int  agz_linear_fp8_backward(int device, void *stream, const agz_linear_fp8_args
  * below the smallest step of its block it is held as that step.  v = r^2 is larger in the mean, by the variance of r's rounding: under normal gradients v by 4 % and r by 1 % (b2 of 0.99
  * and 0.999), entries at 1e-5 of their block's largest v by 48 % and r by 14 %: their steps are that much smaller.
  * The random bits are a hash of (seed, t, tensor index + tensor_base, element): equal arguments give equal results.
- * A tensor whose gradient is NULL is left as it is, its states too, and the step is none of its own: its t is the call's less the number of steps that it missed, so
- * that moments that begin late are corrected as those of the first steps are.  Tensors must not overlap; each has at most 2^34 elements. */
+ * A tensor whose gradient is NULL is left as it is, its states too.  Tensors must not overlap; each has at most 2^34 elements. */
 typedef struct {
     double lr, beta1, beta2, eps, weight_decay;
     int32_t param_dtype, grad_dtype;   /* agz_dtype */
@@ -362,12 +361,16 @@ typedef struct {
     int32_t tensor_base;
     int64_t step;                      /* t of this step, from 1 on; ignored where step_dev is given */
     const int64_t *step_dev;           /* t in device memory, read when the step runs (graph replays); NULL: `step` */
-    const int64_t *missed;             /* [count], host: steps before this one that each tensor missed; NULL: none (not read with step_dev) */
-    int64_t *missed_dev;               /* [count], device, 8-byte aligned, with step_dev: the same; the call adds one where the gradient is NULL.  NULL: none */
 } agz_adamw_options;
 int64_t agz_adamw_state_elements(int count, const int64_t *numel);
 int  agz_adamw_step(int device, void *stream, const agz_adamw_options *opt, int count, void *const *params, const void *const *grads, const int64_t *numel,
                     void *m, void *v, void *m_scale, void *v_scale);
+/* The same where gradients may be missing: a step without its gradient is none of a tensor's own.  t of tensor i is the call's less the steps that it missed, so that
+ * moments that begin late are corrected as those of the first steps are (agz_adamw_step takes the call's t for all: 3.2 lr instead of lr in such a tensor's first step).
+ * missed [count], host: the steps before this one that each missed, 0 .. step - 1; NULL: none; not read with step_dev.
+ * missed_dev [count], device, 8-byte aligned, with step_dev only: the same, and the call adds one where the gradient is NULL; NULL: none. */
+int  agz_adamw_step_missed(int device, void *stream, const agz_adamw_options *opt, const int64_t *missed, int64_t *missed_dev, int count, void *const *params,
+                           const void *const *grads, const int64_t *numel, void *m, void *v, void *m_scale, void *v_scale);
 
 /*
  * Environment switches read by agz_create (all optional; results never depend on them, the tests use them to reach every

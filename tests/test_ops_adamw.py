@@ -447,12 +447,11 @@ def test_counts_are_refused_without_a_gpu():
     at = (C.addressof(buf) + 63) // 64 * 64
     good = dict(lr=0.1, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, param_dtype=0, grad_dtype=0, bits=32, seed=0, tensor_base=0, step=3, step_dev=None)
     for missed, grad in ((-1, at), (3, at), (4, None)):
-        held = (C.c_int64 * 1)(missed)
-        o = lib.AdamWOptions(**good, missed=C.addressof(held))
-        assert L.agz_adamw_step(0, None, C.byref(o), 1, (C.c_void_p * 1)(at), (C.c_void_p * 1)(grad), (C.c_int64 * 1)(4), at, at, None, None) == -1
+        o = lib.AdamWOptions(**good)
+        assert L.agz_adamw_step_missed(0, None, C.byref(o), (C.c_int64 * 1)(missed), None, 1, (C.c_void_p * 1)(at), (C.c_void_p * 1)(grad), (C.c_int64 * 1)(4), at, at, None, None) == -1
         assert "missed" in L.agz_ops_last_error().decode()
-    o = lib.AdamWOptions(**good, missed_dev=at)                     # a count on the device belongs to a step on the device
-    assert L.agz_adamw_step(0, None, C.byref(o), 1, (C.c_void_p * 1)(at), (C.c_void_p * 1)(at), (C.c_int64 * 1)(4), at, at, None, None) == -1
+    o = lib.AdamWOptions(**good)                                    # a count on the device belongs to a step on the device
+    assert L.agz_adamw_step_missed(0, None, C.byref(o), None, at, 1, (C.c_void_p * 1)(at), (C.c_void_p * 1)(at), (C.c_int64 * 1)(4), at, at, None, None) == -1
     assert "missed_dev" in L.agz_ops_last_error().decode()
 
 
@@ -532,3 +531,27 @@ def test_8_bits_round_to_both_sides_in_proportion():
             f = (abs(x) - low) / gap
             # (2 |x| times the mean's own error, and the same six standard errors of the squares' differences, at most 2 (low + gap) gap apart)
             assert abs(got.square().mean().item() - x * x - gap * gap * f * (1 - f)) <= 2 * (abs(x) + gap) * tol, (g, x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_call_without_counts(bits):
+    """agz_adamw_step takes the call's t, of the host or of the device, for every tensor: the step that ops.AdamW takes where no gradient was missing."""
+    L = lib.load_library()
+    ps, gs = tensors(SETS["odd"], torch.float32, torch.bfloat16, 4)
+    gs = [g.cuda() for g in gs]
+    want = [p.cuda() for p in ps]
+    opt = ops.AdamW(want, bits=bits, seed=6, **HYPER)
+    opt.load_state({**opt.state(), "step": 2, "missed": [0] * len(ps)})
+    opt.step(gs)
+    n = len(ps)
+    for step_dev in (None, torch.full((), 3, dtype=torch.int64, device="cuda")):
+        got = [p.cuda() for p in ps]
+        held = ops.AdamW(got, bits=bits)                          # (its buffers)
+        second, scales = (held.v, (None, None)) if bits == 32 else (held.r, (held.m_scale.data_ptr(), held.r_scale.data_ptr()))
+        o = lib.AdamWOptions(lr=HYPER["lr"], beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.1, param_dtype=0, grad_dtype=1, bits=bits, seed=6, tensor_base=0, step=3 if step_dev is None else 0,
+                             step_dev=None if step_dev is None else step_dev.data_ptr())
+        rc = L.agz_adamw_step(0, torch.cuda.current_stream().cuda_stream, C.byref(o), n, (C.c_void_p * n)(*[p.data_ptr() for p in got]), (C.c_void_p * n)(*[g.data_ptr() for g in gs]),
+                              (C.c_int64 * n)(*[p.numel() for p in ps]), held.m.data_ptr(), second.data_ptr(), *scales)
+        assert rc == 0, L.agz_ops_last_error()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and same_states(held, opt)
