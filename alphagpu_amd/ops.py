@@ -108,6 +108,8 @@ def _log_probs_forward(logits, head, moves, target, top, stats):
     L, need, ws = _lib.load_library(), 0, None
     if a > 1024:                                             # (shorter rows need no workspace)
         need = L.agz_logprob_workspace(n, a, top)
+        if need < 0:
+            raise ValueError(f"logits: {n} rows of {a} actions are too many")
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
     q = _LP.pack(*head, 0 if move is None else move.data_ptr(), entropy.data_ptr(), 0 if expected is None else expected.data_ptr(),
                  tops.data_ptr() if top else 0, top_move.data_ptr() if top else 0, 0 if stats is None else stats.data_ptr(), ws.data_ptr() if need else 0, need)

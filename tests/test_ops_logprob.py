@@ -560,3 +560,14 @@ def test_more_than_2_26_short_rows():
         rest = torch.ones(n, dtype=torch.bool, device="cuda")
         rest[some] = False
         assert (g[rest] == g[1]).all()
+
+
+@pytest.mark.gpu
+def test_too_many_long_rows_are_refused_by_name():
+    """Rows that are one row again and again, so that there may be as many as one likes."""
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("needs 8 GiB of free device memory")
+    with pytest.raises(ValueError, match="too many"):
+        ops.log_probs(torch.zeros(1, 2000, device="cuda").expand(1 << 29, 2000))
+    with pytest.raises(lib.AgzError, match="too many rows"):
+        ops.log_probs(torch.zeros(1, 81, device="cuda").expand(1 << 29, 81))
