@@ -441,6 +441,7 @@ class AdamW:
         self.params = list(params)
         _need(self.params, "params: none")
         _need(bits in (8, 32), f"bits: 8 or 32, not {bits!r}")
+        self._options = None
         _check_adamw(lr, betas, eps, weight_decay)
         dev, kind, ends = self.params[0].device if isinstance(self.params[0], torch.Tensor) else None, None, []
         for i, p in enumerate(self.params):
@@ -503,7 +504,10 @@ class AdamW:
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} tensors")
-        _check_adamw(self.lr, self.betas, self.eps, self.weight_decay)
+        options = (self.lr, self.betas, self.eps, self.weight_decay)
+        if options != self._options:                         # (changed since they were last looked at)
+            _check_adamw(*options)
+            self._options = (float(self.lr), tuple(float(b) for b in self.betas), float(self.eps), float(self.weight_decay))      # (values: a list may change in place)
         kind, own, device, at = None, self.dtype, self.device.index, []
         for i, (p, g, shape) in enumerate(zip(params, grads, self._shapes)):
             if p.shape != shape or p.get_device() != device or p.dtype is not own or not p.is_contiguous():

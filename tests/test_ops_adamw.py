@@ -471,6 +471,16 @@ def test_a_refused_step_counts_nothing(capturable):
         assert opt.state()["step"] == opt.steps == 1 and torch.equal(p, before), name
     with pytest.raises(ValueError, match="betas"):
         ops.AdamW([p], betas=(0.9, 0.99, 0.999))
+    opt.betas = [0.9, 0.99]
+    opt.lr = torch.tensor(opt.lr)
+    for change in (lambda: opt.betas.__setitem__(1, 1.5), lambda: opt.lr.fill_(-1.0)):      # (in place)
+        kept = opt.betas[1], opt.lr.item()
+        change()
+        with pytest.raises(ValueError, match="needed"):
+            opt.step([g])
+        opt.betas[1] = kept[0]
+        opt.lr.fill_(kept[1])
+        assert opt.state()["step"] == opt.steps == 1 and torch.equal(p, before)
     opt.step([g])
     assert opt.state()["step"] == opt.steps == 2 and not torch.equal(p, before)
 
